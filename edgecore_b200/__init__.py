@@ -24,7 +24,7 @@ import numpy as np
 
 __all__ = ["load_library", "Model", "gemm_int8", "gemm_fp16_fp32", "gemm_bf16_fp32",
            "quantize_rows", "linear_int8", "gemm_async", "device_error_take", "attention_force_split", "reference_math", "argmax_key", "argmax_key_decode",
-           "LIB_PATH"]
+           "tree_attention", "tree_attention_work", "tree_commit", "kv_copy", "sample", "tree_mask", "LIB_PATH"]
 
 LIB_PATH = Path(__file__).resolve().parent / "libedgecore_b200.so"
 _LIB: C.CDLL | None = None
@@ -55,6 +55,12 @@ def _declare(lib: C.CDLL) -> None:
         "ec_model_packed": (C.c_longlong, [_vp, _i, _i, _vp, C.c_size_t, _vp]),
         "ec_kv_release": (_i, [_vp, _i]),
         "ec_kv_info": (_i, [_vp, _vp]),
+        "ec_model_kv": (_i, [_vp, _vp]),
+        "ec_tree_attention": (_i, [_vp, _vp, _vp]),
+        "ec_tree_attention_work": (C.c_size_t, [_i, _i, _i, _i, _i, _i]),
+        "ec_tree_commit": (_i, [_vp, _vp, _vp]),
+        "ec_kv_copy": (_i, [_vp, _i, _vp, _vp, _vp, _vp, _vp]),
+        "ec_sample": (_i, [_vp, _vp, _vp, _i, C.c_longlong, _i, _i, _vp, _vp, _vp, _vp, _vp, _vp]),
         "ec_model_set_taps": (_i, [_vp, _i]),
         "ec_model_get_taps": (_i, [_vp, _vp, _i]),
         "ec_model_set_vocab_shard": (_i, [_vp, _i, _i]),
@@ -234,6 +240,178 @@ def argmax_key_decode(key: int) -> tuple[float, int]:
     v, i = C.c_float(), C.c_int()
     load_library().ec_argmax_key_decode(C.c_uint64(key), C.byref(v), C.byref(i))
     return v.value, i.value
+
+
+# ---- serving operators on device tensors --------------------------------------
+
+class _KvPages(C.Structure):
+    """ec_kv_pages"""
+    _fields_ = [("k", _vp), ("v", _vp), ("ld_layer", C.c_longlong), ("ld_page", C.c_longlong), ("ld_pos", C.c_longlong),
+                ("page_table", _vp), ("type", _i), ("n_layers", _i), ("n_pages", _i), ("n_slots", _i),
+                ("pages_per_slot", _i), ("dim", _i)]
+
+
+class _TreeAttn(C.Structure):
+    """ec_tree_attn"""
+    _fields_ = [("q", _vp), ("out", _vp), ("ldq", C.c_longlong), ("ldo", C.c_longlong), ("type", _i), ("n_seq", _i),
+                ("rows", _i), ("n_head", _i), ("n_kv_head", _i), ("head_dim", _i), ("window", _i), ("max_len", _i),
+                ("mask_words", _i), ("scale", _f), ("slots", _vp), ("row_start", _vp), ("base", _vp), ("mask", _vp),
+                ("work", _vp), ("work_bytes", C.c_size_t)]
+
+
+class _TreePath(C.Structure):
+    """ec_tree_path"""
+    _fields_ = [("n_seq", _i), ("rows", _i), ("mask_words", _i), ("max_path", _i), ("slots", _vp), ("row_start", _vp),
+                ("base", _vp), ("mask", _vp), ("tokens", _vp), ("picked", _vp), ("accepted", _vp), ("n_accepted", _vp),
+                ("new_base", _vp)]
+
+
+_TYPES = {"torch.float32": 0, "torch.float16": 1, "torch.bfloat16": 2, "torch.int32": 3, "torch.int64": 4}
+_TYPE_OF: dict = {}
+
+
+def _type(t) -> int:
+    """Code of a tensor's element type (0..2 as the C ABI's EC_T_*, 3 int32, 4 int64; -1: any other)."""
+    d = t.dtype
+    code = _TYPE_OF.get(d)
+    if code is None:
+        code = _TYPE_OF[d] = _TYPES.get(str(d), -1)
+    return code
+
+
+def _vec(t, name: str, code: int, n: int | None = None):
+    """Address of a contiguous vector of the given type and, if given, length."""
+    if t is None:
+        return None
+    if _type(t) != code or t.dim() != 1 or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous 1-D tensor of {list(_TYPES)[code]}")
+    if n is not None and t.shape[0] != n:
+        raise ValueError(f"{name} has {t.shape[0]} elements, {n} are needed")
+    return t.data_ptr()
+
+
+def _words(mask, rows: int):
+    if _type(mask) != 4 or mask.dim() != 2 or not mask.is_contiguous() or mask.shape[0] < rows:
+        raise ValueError(f"mask must be a contiguous int64 tensor [{rows}][words]")
+    return mask.shape[1]
+
+
+def _table(page_table):
+    if _type(page_table) != 3 or page_table.dim() != 2 or not page_table.is_contiguous():
+        raise ValueError("page_table must be a contiguous int32 tensor [slots][pages per slot]")
+    return page_table.shape
+
+
+def _layers(k, v, page_table) -> _KvPages:
+    """The arena of all layers: k and v [layers][pages][64][dim] (dim contiguous, any other strides)."""
+    shape, st = k.shape, k.stride()
+    if len(shape) != 4 or shape[1] < 1 or shape[2] != 64 or st[3] != 1 or v.shape != shape or v.stride() != st or v.dtype != k.dtype:
+        raise ValueError("k and v must be alike: [layers][pages][64][dim] with contiguous positions")
+    slots, per_slot = _table(page_table)
+    return _KvPages(k.data_ptr(), v.data_ptr(), st[0], st[1], st[2], page_table.data_ptr(), _type(k), shape[0], shape[1], slots,
+                    per_slot, shape[3])
+
+
+def tree_mask(parents) -> np.ndarray:
+    """Mask rows (int64 [nodes][ceil(nodes / 64)]) of a drafted tree: parents[i] < i is the parent of node i, -1 for a
+    root; bit j of row i is set when j is i or an ancestor of it."""
+    parents = np.asarray(parents)
+    n = len(parents)
+    out = np.zeros((n, max(1, (n + 63) // 64)), np.uint64)
+    for i in range(n):
+        p = int(parents[i])
+        if p >= i or p < -1:
+            raise ValueError(f"parents[{i}] = {p}: a parent comes before its node (-1: a root)")
+        if p >= 0:
+            out[i] = out[p]
+        out[i, i // 64] |= np.uint64(1 << (i % 64))
+    return out.view(np.int64)
+
+
+def tree_attention_work(n_seq: int, rows: int, n_head: int, n_kv_head: int, head_dim: int, max_len: int) -> int:
+    """Bytes of workspace with which tree_attention splits long caches as far as it pays."""
+    return int(load_library().ec_tree_attention_work(n_seq, rows, n_head, n_kv_head, head_dim, max_len))
+
+
+def tree_attention(out, q, k, v, page_table, row_start, base, mask, *, slots=None, window: int = 0, scale: float = 0.0,
+                   max_len: int = 0, workspace=None, stream=None):
+    """Attention of drafted-token trees over a paged KV arena (ec_tree_attention) on device tensors, enqueued on `stream`.
+
+    q, out [rows][heads * head_dim] (or [rows][heads][head_dim]) fp32 or of the cache's type, any row stride; k, v
+    [pages][64][KV heads][head_dim] fp16 or bf16; page_table int32 [slots][pages per slot]; row_start int32 [sequences + 1],
+    base and slots int32 [sequences]; mask int64 [rows][words] (tree_mask).  workspace: a contiguous tensor, any type."""
+    qs, ks, kst, qst, ost = q.shape, k.shape, k.stride(), q.stride(), out.stride()
+    if len(ks) != 4 or ks[0] < 1 or ks[1] != 64 or kst[3] != 1 or (ks[2] > 1 and kst[2] != ks[3]) or v.shape != ks or v.stride() != kst:
+        raise ValueError("k and v must be alike: [pages][64][KV heads][head_dim] with contiguous positions")
+    if len(qs) not in (2, 3) or out.shape != qs or out.dtype != q.dtype or v.dtype != k.dtype:
+        raise ValueError("q and out must be alike: [rows][heads * head_dim] or [rows][heads][head_dim]")
+    hd = ks[3]
+    wide = qs[1] if len(qs) == 2 else qs[1] * qs[2]
+    if wide % hd or (len(qs) == 3 and qs[2] != hd):
+        raise ValueError(f"rows of {wide} for heads of {hd}")
+    for st in (qst, ost):
+        if (wide and st[-1] != 1) or (len(qs) == 3 and qs[1] > 1 and st[1] != hd):
+            raise ValueError("the rows of q and out must be contiguous")
+    rows, n_seq = qs[0], base.shape[0]
+    slots_n, per_slot = _table(page_table)
+    kv = _KvPages(k.data_ptr(), v.data_ptr(), 0, kst[0], kst[1], page_table.data_ptr(), _type(k), 1, ks[0], slots_n, per_slot,
+                  ks[2] * hd)
+    work = None
+    nbytes = 0
+    if workspace is not None:
+        if not workspace.is_contiguous():
+            raise ValueError("workspace must be contiguous")
+        work, nbytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+    a = _TreeAttn(q.data_ptr(), out.data_ptr(), qst[0], ost[0], _type(q), n_seq, rows, wide // hd, ks[2], hd, window, max_len,
+                  _words(mask, rows), scale, _vec(slots, "slots", 3, n_seq), _vec(row_start, "row_start", 3, n_seq + 1),
+                  _vec(base, "base", 3), mask.data_ptr(), work, nbytes)
+    if load_library().ec_tree_attention(C.addressof(kv), C.addressof(a), stream):
+        raise RuntimeError(last_error())
+    return out
+
+
+def tree_commit(k, v, page_table, row_start, base, mask, tokens, picked, accepted, n_accepted, new_base, *, slots=None,
+                stream=None) -> None:
+    """Accept the confirmed path of every drafted tree and move its K and V rows to the front (ec_tree_commit).
+
+    k, v [layers][pages][64][dim]; tokens, picked int32 [rows]; accepted int32 [sequences][most nodes of a path], n_accepted
+    and new_base int32 [sequences] (new_base may be base) are written; the others as for tree_attention."""
+    kv = _layers(k, v, page_table)
+    n_seq = base.shape[0]
+    rows = tokens.shape[0]
+    if _type(accepted) != 3 or accepted.dim() != 2 or accepted.shape[0] != n_seq or not accepted.is_contiguous():
+        raise ValueError(f"accepted must be a contiguous int32 tensor [{n_seq}][nodes]")
+    a = _TreePath(n_seq, rows, _words(mask, rows), accepted.shape[1], _vec(slots, "slots", 3, n_seq),
+                  _vec(row_start, "row_start", 3, n_seq + 1), _vec(base, "base", 3), mask.data_ptr(), _vec(tokens, "tokens", 3),
+                  _vec(picked, "picked", 3, rows), accepted.data_ptr(), _vec(n_accepted, "n_accepted", 3, n_seq),
+                  _vec(new_base, "new_base", 3, n_seq))
+    if load_library().ec_tree_commit(C.addressof(kv), C.addressof(a), stream):
+        raise RuntimeError(last_error())
+
+
+def kv_copy(k, v, page_table, src, dst, start, end, *, stream=None) -> None:
+    """Copy positions [start[j], end[j]) of slot src[j] to slot dst[j] in every layer (ec_kv_copy); k, v
+    [layers][pages][64][dim], the others int32 vectors of one length."""
+    kv = _layers(k, v, page_table)
+    n = src.shape[0]
+    if load_library().ec_kv_copy(C.addressof(kv), n, _vec(src, "src", 3), _vec(dst, "dst", 3, n), _vec(start, "start", 3, n),
+                                 _vec(end, "end", 3, n), stream):
+        raise RuntimeError(last_error())
+
+
+def sample(ids, logits, u, *, temperature=None, top_k=None, top_p=None, min_p=None, prob=None, stream=None):
+    """Draw one token per row of logits [rows][vocab] (fp32, fp16 or bf16, any row stride) with the uniform numbers u[rows]
+    (ec_sample): temperature, top-k, top-p and min-p per row, each a vector or None for off.  Writes ids int32 [rows] and, if
+    given, prob fp32 [rows]; returns ids."""
+    shape, st = logits.shape, logits.stride()
+    if len(shape) != 2 or (shape[1] > 1 and st[1] != 1):
+        raise ValueError("logits must be [rows][vocab] with contiguous rows")
+    rows = shape[0]
+    if load_library().ec_sample(_vec(ids, "ids", 3, rows), _vec(prob, "prob", 0, rows), logits.data_ptr(), _type(logits), st[0], rows,
+                                shape[1], _vec(temperature, "temperature", 0, rows), _vec(top_k, "top_k", 3, rows),
+                                _vec(top_p, "top_p", 0, rows), _vec(min_p, "min_p", 0, rows), _vec(u, "u", 0, rows), stream):
+        raise RuntimeError(last_error())
+    return ids
 
 
 # ---- model -------------------------------------------------------------------

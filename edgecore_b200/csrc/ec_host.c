@@ -1993,6 +1993,26 @@ EC_EXPORT int ec_kv_info(const GPT2 *g, int *info4)
     return 0;
 }
 
+EC_EXPORT int ec_model_kv(GPT2 *g, ec_kv_pages *kv)
+{
+    ec_dev *d = ec_lookup(g);
+    if (!d || !kv) { ec_seterr("ec_model_kv: no model or NULL view"); return -1; }
+    memset(kv, 0, sizeof *kv);
+    kv->k = d->kc;
+    kv->v = d->vc;
+    kv->ld_layer = (long long)d->layer_kv;
+    kv->ld_page = (long long)EC_KV_PAGE * d->kv;
+    kv->ld_pos = d->kv;
+    kv->page_table = d->d_pt;
+    kv->type = EC_T_F16;
+    kv->n_layers = d->L;
+    kv->n_pages = d->kv_pages;
+    kv->n_slots = d->B;
+    kv->pages_per_slot = d->mp;
+    kv->dim = d->kv;
+    return 0;
+}
+
 EC_EXPORT long long ec_model_packed(const GPT2 *g, int layer, int which, void *out, size_t cap, int *info5)
 {
     ec_dev *d = ec_lookup(g);

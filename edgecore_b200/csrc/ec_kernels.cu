@@ -1396,6 +1396,18 @@ extern "C" int ec_launch_reference_math(const float *x, float *e, float *t, int 
     return (int)cudaGetLastError();
 }
 
+extern "C" int *ec_error_word(void) {
+    static int *word[64];
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return nullptr;
+    if (!word[dev]) {
+        void *p = nullptr;
+        if (cudaGetSymbolAddress(&p, g_ec_err) != cudaSuccess) return nullptr;
+        word[dev] = static_cast<int *>(p);
+    }
+    return word[dev];
+}
+
 extern "C" int ec_kernel_error_take(cudaStream_t stream, int *code) {
     int zero = 0;
     cudaError_t e = cudaMemcpyFromSymbolAsync(code, g_ec_err, sizeof(int), 0, cudaMemcpyDeviceToHost, stream);

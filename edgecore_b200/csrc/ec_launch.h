@@ -226,6 +226,9 @@ int ec_launch_reference_math(const float *x, float *e, float *t, int n, cudaStre
  * indices skipped).  Read and cleared by ec_kernel_error_take. */
 int ec_kernel_error_take(cudaStream_t stream, int *code);
 
+/* Device address of that error word on the current device (NULL: none). */
+int *ec_error_word(void);
+
 /* One-time per-device kernel attribute setup (dynamic shared memory limits). */
 int ec_kernels_init(void);
 

@@ -249,6 +249,130 @@ int ec_linear_int8_noalloc(float *C, const float *X, const int8_t *W,
                            const float *w_scale, const float *bias, int M, int K, int N,
                            void *stream);
 
+/* ---- serving operators on device operands -------------------------------- */
+
+/* Speculative decoding and sampling over a paged KV arena: attention of a
+ * tree of drafted tokens, committing the path of it that the model confirms,
+ * drawing the next token, and copying a slot's rows to other slots.  All
+ * pointers are DEVICE memory of the current device; work is enqueued on
+ * `stream` (cudaStream_t, NULL = legacy default) without a host
+ * synchronisation and without allocating, so every call can be captured
+ * into a CUDA graph.  Indices that come from device memory (slots, pages,
+ * row_start, base) are bounds-checked there: what a bad one names is skipped
+ * or read as page 0, and ec_device_error_take reports code 2. */
+
+enum { EC_T_F32 = 0, EC_T_F16 = 1, EC_T_BF16 = 2 };
+
+/* A paged KV arena: position p of slot s lies in page
+ * page_table[s * pages_per_slot + p / 64], at row p % 64 of it.  Strides are
+ * in elements, multiples of 8; k and v are 16-byte aligned. */
+typedef struct {
+    void *k, *v;               /* layer 0; 16-bit elements of `type`                */
+    long long ld_layer;        /* between layers                                   */
+    long long ld_page;         /* between pages                                    */
+    long long ld_pos;          /* between the 64 positions of a page               */
+    const int *page_table;     /* [n_slots][pages_per_slot] page numbers           */
+    int type;                  /* EC_T_F16 or EC_T_BF16                            */
+    int n_layers, n_pages, n_slots, pages_per_slot;
+    int dim;                   /* elements of one position: KV heads x head_dim    */
+} ec_kv_pages;
+
+/* The arena of a loaded model (fp16, every layer; pages as ec_kv_info counts
+ * them).  A slot's table entries are -1 until calls map its pages. */
+int ec_model_kv(GPT2 *g, ec_kv_pages *kv);
+
+/* Attention of drafted-token trees.  Sequence b owns the rows [row_start[b],
+ * row_start[b+1]) of q and out: the nodes of a tree whose K and V are in the
+ * cache at positions base[b] + node of slot slots[b] (slots NULL: slot b),
+ * after the base[b] committed ones.  Row i attends every committed position
+ * and the node j whose bit (word j / 64, bit j % 64) is set in row i of
+ * `mask` ([rows][mask_words]; ancestors and the node itself for a tree, but
+ * any set of nodes is allowed).  The number of set bits less one is the
+ * node's depth: it stands at position base[b] + depth, and with window > 0
+ * it sees only keys whose position is above that minus window.
+ *   out[i] = sum_j softmax_j(scale * q[i].k[j]) v[j], 0 where i sees nothing
+ * with query head h reading KV head h / (n_head / n_kv_head).  One token a
+ * sequence and mask word 1 is plain decode attention.  q and out have one
+ * type: EC_T_F32, or the cache's own; strides in elements, any alignment of
+ * the element.  head_dim is a multiple of 8 up to 256.  scale 0 means
+ * 1/sqrt(head_dim).  Rows behind row_start[n_seq] are left as they were.
+ * Scores, weights and sums are held in 32 bits; with 16-bit q the weights are
+ * rounded to the cache's type for the product with V.
+ * work (NULL, or 256-byte aligned): partial sums of sequences whose positions
+ * are split over CTAs; without it, or when it is smaller than
+ * ec_tree_attention_work, there is less splitting and the same result up to
+ * rounding.  Calls that can overlap must not share it.  max_len: about the
+ * most positions of a sequence (0: the page table's width); it only steers
+ * the splitting. */
+typedef struct {
+    const void *q;
+    void *out;
+    long long ldq, ldo;        /* row strides of q and out                         */
+    int type;
+    int n_seq, rows;           /* sequences; rows that q, out and mask hold        */
+    int n_head, n_kv_head, head_dim;
+    int window, max_len, mask_words;
+    float scale;
+    const int *slots, *row_start, *base;
+    const unsigned long long *mask;
+    void *work;
+    size_t work_bytes;
+} ec_tree_attn;
+int ec_tree_attention(const ec_kv_pages *kv, const ec_tree_attn *a, void *stream);
+
+/* Bytes of `work` with which ec_tree_attention splits as far as it pays. */
+size_t ec_tree_attention_work(int n_seq, int rows, int n_head, int n_kv_head, int head_dim, int max_len);
+
+/* Accept the part of a drafted tree that the model confirms, and commit its
+ * cache rows.  Sequence b's tree is described as for ec_tree_attention: the
+ * parent of node j is the highest bit below j of mask row j, node 0 is the
+ * root.  tokens[row] is the node's token, picked[row] the model's choice after
+ * it.  The path starts at the root and goes on to the child whose token is
+ * picked[its parent] (the first of equal ones) until there is none or it has
+ * max_path nodes.  Then, in every layer, the K and V of the path's n-th node
+ * move from position base[b] + node to base[b] + n, and
+ *   accepted[b][n]  = picked[n-th node of the path]  (-1 behind the path)
+ *   n_accepted[b]   = nodes on the path = tokens produced
+ *   new_base[b]     = base[b] + n_accepted[b]       (may be base itself)
+ * An empty tree accepts nothing.  Two sequences must not have one slot. */
+typedef struct {
+    int n_seq, rows, mask_words, max_path;
+    const int *slots, *row_start;
+    const int *base;
+    const unsigned long long *mask;
+    const int *tokens, *picked;
+    int *accepted, *n_accepted, *new_base;
+} ec_tree_path;
+int ec_tree_commit(const ec_kv_pages *kv, const ec_tree_path *a, void *stream);
+
+/* Copy the K and V of positions [start[j], end[j]) in every layer from slot
+ * src[j] to slot dst[j], for n_copies jobs (DEVICE int arrays).  A job whose
+ * target is written or read by another job at a common position, or is its
+ * own source, is skipped and reported (code 2), and so is one with a bad
+ * slot or range; an empty range copies nothing. */
+int ec_kv_copy(const ec_kv_pages *kv, int n_copies, const int *src, const int *dst, const int *start,
+               const int *end, void *stream);
+
+/* Draw one token for every row of logits [rows][ld] (vocab of them used,
+ * EC_T_F32 / F16 / BF16).  temperature, top_k, top_p, min_p: per-row DEVICE
+ * arrays, or NULL for all rows off (temperature 1).  Row r, with w_i =
+ * exp((logit_i - max) / temperature):
+ *   1. temperature <= 0 (or NaN): the argmax, lowest index on ties, prob 1;
+ *   2. top_k > 0 keeps the top_k largest, lowest index first among equals;
+ *   3. top_p < 1 keeps, in the same order, up to and with the one at which
+ *      the sum of w reaches top_p times the sum over 2.; the first always;
+ *   4. min_p > 0 drops those with w < min_p, except the first;
+ *   5. the token is the first index, in vocabulary order, at which the sum of
+ *      the kept w exceeds u[r] times their sum (u in [0, 1); above: the last).
+ * ids[r] = the token, prob[r] (may be NULL) = its share of the kept w.  NaN
+ * counts as -inf; among +inf logits all weights are equal; a row without any
+ * logit above -inf gives id -1 and prob 0.  The sums are exact integers of
+ * weights rounded to 2^-(62 - log2 vocab), so a row's result depends on
+ * neither the other rows nor the launch. */
+int ec_sample(int *ids, float *prob, const void *logits, int type, long long ld, int rows, int vocab,
+              const float *temperature, const int *top_k, const float *top_p, const float *min_p,
+              const float *u, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,282 @@
+"""Attention of drafted-token trees over a paged arena (ec_tree_attention) against the formula in 64 bits.
+
+The bound of a value, from the arithmetic the operator documents (scores, weights and sums in 32 bits, q of 16 bits exact,
+fp32 q in two 16-bit parts or exact, with 16-bit q the weights rounded to the cache's type):
+  a score is a sum of hd products in 32 bits, off by at most (hd + 8) 2^-23 of the sum of their magnitudes (twice the
+  rounding bound, since a tensor-core sum may truncate) and 2^-20 of it for the two parts of an fp32 q; its distance to
+  the maximum is rounded once more, 2^-23 of it; a weight is off by that much of itself plus 2^-21 for exp, and both the
+  numerator and the denominator of out = sum w v / sum w move by it: twice the largest, times sum w |v| / sum w;
+  a weight rounded to 16 bits moves by half a step, 2^-11 or 2^-8 of itself (fp32 q: in two parts, 2^-20), and an fp16
+  weight below 2^-14 by at most 2^-25, a part that the largest weight 1 bounds by n 2^-25 max |v|;
+  sums over n keys in 32 bits: n 2^-24 at worst, taken as 2^-20 + n 2^-24 / 8 (tree and tile order);
+  the result is rounded to its type once, half a step."""
+from __future__ import annotations
+
+import math
+
+import numpy as np
+import pytest
+
+import edgecore_b200 as ec
+
+pytestmark = pytest.mark.gpu
+
+HALF_STEP = {"f32": 2.0 ** -24, "f16": 2.0 ** -11, "bf16": 2.0 ** -8}
+
+
+def _types(torch):
+    return {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
+
+
+class Case:
+    """A batch of trees over a shuffled arena whose unused rows hold NaN."""
+
+    def __init__(self, torch, q="f16", kv="f16", heads=4, kv_heads=2, hd=64, sizes=(5,), bases=(100,), window=0, seed=0, mask=None,
+                 words=None, spare_pages=2, q_gain=1.0):
+        rs = np.random.RandomState(seed)
+        ty = _types(torch)
+        self.torch, self.qt, self.kt, self.heads, self.kvh, self.hd, self.window = torch, q, kv, heads, kv_heads, hd, window
+        self.sizes, self.bases = list(sizes), list(bases)
+        n = len(self.sizes)
+        self.start = np.cumsum([0] + self.sizes).astype(np.int32)
+        rows = int(self.start[-1])
+        per = max(1, max(-(-(b + t) // 64) for b, t in zip(self.bases, self.sizes))) + 1
+        pages = n * per + spare_pages
+        self.table = rs.permutation(pages)[: n * per].reshape(n, per).astype(np.int32)
+        self.slots = rs.permutation(n).astype(np.int32)
+        self.w = words or max(1, -(-max(self.sizes + [1]) // 64))
+        if mask is None:
+            mask = np.zeros((rows, self.w), np.uint64)
+            for b, t in enumerate(self.sizes):
+                if t:
+                    parents = [-1] + [int(rs.randint(max(0, i - 6), i)) for i in range(1, t)]
+                    m = ec.tree_mask(parents).view(np.uint64)
+                    mask[self.start[b]:self.start[b + 1], : m.shape[1]] = m
+        self.mask = mask
+        k = torch.full((pages, 64, kv_heads, hd), math.nan, dtype=ty[kv])
+        v = torch.full((pages, 64, kv_heads, hd), math.nan, dtype=ty[kv])
+        for b in range(n):
+            for p in range(self.bases[b] + self.sizes[b]):
+                at = (self.table[self.slots[b], p // 64], p % 64)
+                k[at] = torch.from_numpy(rs.randn(kv_heads, hd)).to(ty[kv])
+                v[at] = torch.from_numpy(rs.randn(kv_heads, hd)).to(ty[kv])
+        self.k, self.v = k.cuda(), v.cuda()
+        self.q = (torch.from_numpy(rs.randn(rows, heads * hd)) * q_gain).to(ty[q]).cuda()
+        self.out = torch.full_like(self.q, 7.0)
+
+    def dev(self, a):
+        return self.torch.from_numpy(np.ascontiguousarray(a)).cuda()
+
+    def run(self, work_bytes=1 << 24, scale=0.0, **kw):
+        work = self.torch.empty(work_bytes, dtype=self.torch.uint8, device="cuda") if work_bytes else None
+        ec.tree_attention(kw.pop("out", self.out), kw.pop("q", self.q), kw.pop("k", self.k), kw.pop("v", self.v), self.dev(self.table),
+                          self.dev(self.start), self.dev(np.array(self.bases, np.int32)), self.dev(self.mask.view(np.int64)),
+                          slots=self.dev(self.slots), window=self.window, scale=scale, workspace=work,
+                          max_len=max(b + t for b, t in zip(self.bases, self.sizes)), **kw)
+        self.torch.cuda.synchronize()
+        assert ec.device_error_take() == 0
+        return kw.get("out", self.out)
+
+    def expect(self, scale=0.0):
+        """The result in 64 bits and the bound of every value."""
+        hd, heads = self.hd, self.heads
+        scale = scale or hd ** -0.5
+        rows = int(self.start[-1])
+        want, tol = np.zeros((rows, heads, hd)), np.zeros((rows, heads, hd))
+        q = self.q.double().cpu().numpy().reshape(rows, heads, hd)
+        r_w = 2.0 ** -20 if self.qt == "f32" else HALF_STEP[self.kt]
+        for b, (t, base) in enumerate(zip(self.sizes, self.bases)):
+            pages = self.table[self.slots[b]]
+            k, v = (x.double().cpu().numpy()[pages].reshape(-1, self.kvh, hd)[: base + t] for x in (self.k, self.v))
+            bits = [[bool(int(self.mask[self.start[b] + i, j // 64]) >> (j % 64) & 1) if j // 64 < self.w else False for j in range(t)]
+                    for i in range(t)]
+            full = [sum(bin(int(x)).count("1") for x in self.mask[self.start[b] + i]) - 1 for i in range(t)]
+            for i in range(t):
+                seen = np.concatenate([np.ones(base, bool), np.array(bits[i], bool)])
+                if self.window:
+                    where = np.concatenate([np.arange(base), base + np.array(full)])
+                    seen &= where > base + full[i] - self.window
+                if not seen.any():
+                    continue
+                for h in range(heads):
+                    kk, vv, qq = k[seen, h * self.kvh // heads], v[seen, h * self.kvh // heads], q[self.start[b] + i, h]
+                    s = kk @ qq * scale
+                    mag = (np.abs(kk) @ np.abs(qq) * scale).max()
+                    w = np.exp(s - s.max())
+                    n = len(s)
+                    row = self.start[b] + i
+                    want[row, h] = w @ vv / w.sum()
+                    move = ((hd + 8) * 2.0 ** -23 + (2.0 ** -20 if self.qt == "f32" else 0)) * mag + (s.max() - s.min()) * 2.0 ** -23 + 2.0 ** -21
+                    tol[row, h] = (2 * move + r_w + 2.0 ** -20 + n * 2.0 ** -27) * (w @ np.abs(vv) / w.sum()) * 1.02 + HALF_STEP[self.qt] * np.abs(want[row, h])
+                    if self.qt == "f16":
+                        tol[row, h] += n * 2.0 ** -25 * np.abs(vv).max() + 2.0 ** -25
+        return want.reshape(rows, -1), tol.reshape(rows, -1)
+
+    def check(self, got=None, **kw):
+        got = self.out if got is None else got
+        want, tol = self.expect(**kw)
+        got = got.double().cpu().numpy().reshape(want.shape)
+        assert np.isfinite(got).all()
+        worst = (np.abs(got - want) - tol).max() if got.size else -1.0
+        assert worst <= 0, f"{worst:.3g} over the bound (error {np.abs(got - want).max():.3g})"
+
+
+@pytest.mark.parametrize("q,kv", [("f16", "f16"), ("bf16", "bf16"), ("f32", "f16"), ("f32", "bf16")])
+@pytest.mark.parametrize("heads,kv_heads,hd", [(14, 2, 64), (12, 2, 128), (4, 4, 64), (3, 1, 80), (2, 2, 8), (4, 2, 256), (5, 5, 40)])
+def test_types_and_heads(cuda, q, kv, heads, kv_heads, hd):
+    c = Case(cuda, q, kv, heads, kv_heads, hd, sizes=(7, 1, 20), bases=(130, 63, 0), seed=hd + heads)
+    c.run()
+    c.check()
+
+
+@pytest.mark.parametrize("size,base", [(1, 0), (1, 1), (1, 63), (1, 64), (1, 65), (2, 127), (17, 47), (64, 0), (64, 1000), (65, 191), (130, 300)])
+@pytest.mark.parametrize("q,kv", [("f16", "f16"), ("f32", "f16"), ("bf16", "bf16")])
+def test_lengths_around_pages_and_words(cuda, size, base, q, kv):
+    c = Case(cuda, q, kv, 6, 2, 64, sizes=(size,), bases=(base,), seed=size + base)
+    c.run()
+    c.check()
+
+
+@pytest.mark.parametrize("work_bytes", [0, 256, 1 << 14, 1 << 24])
+@pytest.mark.parametrize("q,kv,hd", [("f16", "f16", 64), ("f32", "f16", 128), ("bf16", "bf16", 128)])
+def test_long_cache_split_over_ctas(cuda, work_bytes, q, kv, hd):
+    c = Case(cuda, q, kv, 7, 1, hd, sizes=(3, 9), bases=(5000, 777), seed=5)
+    c.run(work_bytes)
+    c.check()
+
+
+@pytest.mark.parametrize("window", [1, 2, 7, 64, 100, 1000])
+@pytest.mark.parametrize("q,kv", [("f16", "f16"), ("f32", "bf16")])
+def test_window(cuda, window, q, kv):
+    c = Case(cuda, q, kv, 4, 2, 64, sizes=(12, 1, 70), bases=(200, 5, 64), window=window, seed=window)
+    c.run()
+    c.check()
+
+
+@pytest.mark.parametrize("q,kv", [("f16", "f16"), ("f32", "f16")])
+def test_rows_that_see_nothing_and_any_mask(cuda, q, kv):
+    rs = np.random.RandomState(3)
+    sizes, bases = (9, 4, 6), (0, 0, 30)
+    mask = (rs.randint(0, 1 << 9, (19, 1))).astype(np.uint64)     # any sets; bits behind a tree's end mean nothing
+    mask[[0, 4, 9, 12]] = 0                                       # sequence 0 and 1 have nothing cached: empty rows
+    mask[9:13] &= np.uint64(15)
+    mask[13:] &= np.uint64(63)
+    c = Case(cuda, q, kv, 4, 2, 64, sizes=sizes, bases=bases, mask=mask, seed=4)
+    c.run()
+    c.check()
+    out = c.out.cpu()
+    assert (out[[0, 4, 9, 12]] == 0).all()
+
+
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("q,kv", [("f16", "f16"), ("f32", "f16"), ("bf16", "bf16")])
+def test_what_a_row_does_not_see_does_not_reach_it(cuda, bad, q, kv):
+    """Two branches; the second one's node holds `bad` in K and V: only the rows that see it may change."""
+    parents = [-1, 0, 0, 1, 2, 3]
+    c = Case(cuda, q, kv, 4, 2, 64, sizes=(6,), bases=(70,), mask=ec.tree_mask(parents).view(np.uint64), seed=6)
+    want, tol = c.expect()
+    page, off = c.table[c.slots[0], (70 + 2) // 64], (70 + 2) % 64
+    c.k[page, off] = bad
+    c.v[page, off] = bad
+    c.run()
+    got = c.out.double().cpu().numpy()
+    clean = [0, 1, 3, 5]
+    assert (np.abs(got - want) <= tol)[clean].all()
+    assert not np.isfinite(got[[2, 4]]).all()
+
+
+def test_window_hides_infinities(cuda):
+    c = Case(cuda, "f16", "f16", 4, 2, 64, sizes=(4,), bases=(200,), mask=ec.tree_mask([-1, 0, 1, 2]).view(np.uint64), window=50, seed=8)
+    want, tol = c.expect()
+    for p in range(0, 152):       # row i sees positions above 150 + i; row 0 still sees 151, the others do not
+        c.v[c.table[c.slots[0], p // 64], p % 64] = math.inf
+        c.k[c.table[c.slots[0], p // 64], p % 64] = math.nan if p < 151 else 0.0
+    c.run()
+    got = c.out.double().cpu().numpy()
+    assert (np.abs(got - want) <= tol)[1:].all()
+    assert not np.isfinite(got[0]).all()
+
+
+def test_strides_three_dimensions_and_rows_behind_the_last_sequence(cuda):
+    c = Case(cuda, "f16", "f16", 6, 2, 64, sizes=(3, 8), bases=(90, 10), seed=9)
+    rows, wide = c.q.shape
+    big_q = cuda.full((rows + 5, wide + 13), 3.0, dtype=cuda.float16, device="cuda")
+    big_o = cuda.full((rows + 5, wide + 21), 5.0, dtype=cuda.float16, device="cuda")
+    big_q[:rows, 1:wide + 1] = c.q
+    c.mask = np.concatenate([c.mask, np.zeros((5, c.w), np.uint64)])
+    q, out = big_q[:, 1:wide + 1], big_o[:, 3:wide + 3]
+    ec.tree_attention(out, q, c.k, c.v, c.dev(c.table), c.dev(c.start), c.dev(np.array(c.bases, np.int32)), c.dev(c.mask.view(np.int64)),
+                      slots=c.dev(c.slots))
+    cuda.cuda.synchronize()
+    assert ec.device_error_take() == 0
+    c.mask = c.mask[:rows]
+    c.check(out[:rows])
+    rest = big_o.clone()
+    rest[:rows, 3:wide + 3] = 5.0
+    assert (rest == 5.0).all()
+    # the heads as a dimension of their own, K and V interleaved in one pool
+    both = cuda.stack([c.k, c.v], dim=2)
+    out3 = cuda.empty((rows, 6, 64), dtype=cuda.float16, device="cuda")
+    c.run(out=out3, q=c.q.view(rows, 6, 64), k=both[:, :, 0], v=both[:, :, 1])
+    c.check(out3)
+
+
+def test_scale_large_scores_and_many_words(cuda):
+    c = Case(cuda, "f32", "f16", 4, 2, 64, sizes=(5,), bases=(300,), seed=10, words=3, q_gain=40.0)
+    c.run()
+    c.check()
+    c.run(scale=0.01)
+    c.check(scale=0.01)
+
+
+def test_empty_trees_between_others(cuda):
+    c = Case(cuda, "f16", "f16", 4, 4, 64, sizes=(0, 3, 0, 0, 2, 0), bases=(10, 64, 0, 70, 128, 3), seed=11)
+    c.run()
+    c.check()
+
+
+def test_bad_indices_are_reported(cuda):
+    c = Case(cuda, "f16", "f16", 4, 2, 64, sizes=(3, 2), bases=(90, 10), seed=12)
+    good = c.table.copy()
+    for spoil in ("page", "slot", "base", "rows"):
+        table, slots, bases, start = good.copy(), c.slots.copy(), list(c.bases), c.start.copy()
+        if spoil == "page":
+            table[slots[1], 0] = 10 ** 6
+        elif spoil == "slot":
+            slots[1] = 2
+        elif spoil == "base":
+            bases[1] = 64 * table.shape[1] - 1
+        else:
+            start[2] = 9
+        ec.tree_attention(c.out, c.q, c.k, c.v, c.dev(table), c.dev(start), c.dev(np.array(bases, np.int32)), c.dev(c.mask.view(np.int64)),
+                          slots=c.dev(slots))
+        assert ec.device_error_take() == 2, spoil
+        assert ec.device_error_take() == 0
+        want, tol = c.expect()
+        got = c.out.double().cpu().numpy()
+        assert (np.abs(got - want) <= tol)[:3].all(), spoil     # the first sequence is untouched by it
+
+
+def test_captured_graph_replays_on_new_data_and_other_stream(cuda):
+    c = Case(cuda, "bf16", "bf16", 7, 1, 128, sizes=(4, 1), bases=(2000, 65), seed=13)
+    c.run()
+    args = (c.dev(c.table), c.dev(c.start), c.dev(np.array(c.bases, np.int32)), c.dev(c.mask.view(np.int64)))
+    slots = c.dev(c.slots)
+    work = cuda.empty(1 << 22, dtype=cuda.uint8, device="cuda")
+    g = cuda.cuda.CUDAGraph()
+    with cuda.cuda.graph(g):
+        ec.tree_attention(c.out, c.q, c.k, c.v, *args, slots=slots, workspace=work, max_len=2004,
+                          stream=cuda.cuda.current_stream().cuda_stream)
+    for gain in (1.0, 0.5):
+        c.q.mul_(gain)
+        c.out.fill_(9.0)
+        g.replay()
+        cuda.cuda.synchronize()
+        c.check()
+    first = c.out.clone()
+    s = cuda.cuda.Stream()
+    c.out.fill_(9.0)
+    s.wait_stream(cuda.cuda.current_stream())
+    ec.tree_attention(c.out, c.q, c.k, c.v, *args, slots=slots, workspace=work, max_len=2004, stream=s.cuda_stream)
+    s.synchronize()
+    assert cuda.equal(c.out, first)      # the same result, bit for bit

@@ -1,0 +1,155 @@
+"""What the serving operators refuse before anything is launched: every bad argument that the host can see, by its message.
+No GPU is needed: the checks of arguments come before the first CUDA call, and a good call on a machine without a device
+(or with host memory on one with a device) is refused too."""
+from __future__ import annotations
+
+import ctypes as C
+
+import numpy as np
+import pytest
+
+import edgecore_b200 as ec
+
+torch = pytest.importorskip("torch")
+
+
+def tree(**kw):
+    rows, n, heads, kvh, hd, pages, words = 6, 2, 4, 2, 64, 5, 1
+    t = dict(q=torch.zeros(rows, heads * hd, dtype=torch.float16), k=torch.zeros(pages, 64, kvh, hd, dtype=torch.float16),
+             v=torch.zeros(pages, 64, kvh, hd, dtype=torch.float16), page_table=torch.zeros(n, 2, dtype=torch.int32),
+             row_start=torch.zeros(n + 1, dtype=torch.int32), base=torch.zeros(n, dtype=torch.int32), mask=torch.zeros(rows, words, dtype=torch.int64))
+    t["out"] = torch.zeros_like(kw.get("q", t["q"]))
+    t.update(kw)
+    return ec.tree_attention(**t)
+
+
+@pytest.mark.parametrize("kw,error,says", [
+    (dict(k=torch.zeros(5, 32, 2, 64, dtype=torch.float16)), ValueError, "k and v"),
+    (dict(v=torch.zeros(4, 64, 2, 64, dtype=torch.float16)), ValueError, "k and v"),
+    (dict(v=torch.zeros(5, 64, 2, 64, dtype=torch.bfloat16)), ValueError, "alike"),
+    (dict(out=torch.zeros(6, 256)), ValueError, "q and out"),
+    (dict(q=torch.zeros(6, 250, dtype=torch.float16)), ValueError, "250"),
+    (dict(q=torch.zeros(6, 2, 128, dtype=torch.float16)), ValueError, "heads of 64"),
+    (dict(q=torch.zeros(256, 6, dtype=torch.float16).T), ValueError, "contiguous"),
+    (dict(q=torch.zeros(6, 192, dtype=torch.float16)), RuntimeError, "3 query heads over 2"),
+    (dict(q=torch.zeros(6, 256, dtype=torch.bfloat16)), RuntimeError, "cache's type"),
+    (dict(q=torch.zeros(6, 256, dtype=torch.float64)), RuntimeError, "cache's type"),
+    (dict(k=torch.zeros(5, 64, 2, 64), v=torch.zeros(5, 64, 2, 64)), RuntimeError, "fp16 or bf16"),
+    (dict(mask=torch.zeros(5, 1, dtype=torch.int64)), ValueError, "mask"),
+    (dict(mask=torch.zeros(6, 1, dtype=torch.int32)), ValueError, "mask"),
+    (dict(mask=torch.zeros(6, 0, dtype=torch.int64)), RuntimeError, "mask_words"),
+    (dict(row_start=torch.zeros(2, dtype=torch.int32)), ValueError, "row_start"),
+    (dict(base=torch.zeros(2, dtype=torch.int64)), ValueError, "base"),
+    (dict(slots=torch.zeros(3, dtype=torch.int32)), ValueError, "slots"),
+    (dict(page_table=torch.zeros(2, 2, dtype=torch.int64)), ValueError, "page_table"),
+    (dict(page_table=torch.zeros(2, 4, dtype=torch.int32)[:, :2]), ValueError, "page_table"),
+    (dict(window=-1), RuntimeError, "window"),
+    (dict(scale=-0.5), RuntimeError, "scale"),
+    (dict(scale=float("nan")), RuntimeError, "scale"),
+    (dict(workspace=torch.zeros(64, 64)[:, :3]), ValueError, "workspace"),
+    (dict(), RuntimeError, "device"),
+])
+def test_tree_attention(built, kw, error, says):
+    with pytest.raises(error, match=says):
+        tree(**kw)
+
+
+@pytest.mark.parametrize("hd", [4, 12, 264])
+def test_head_dim(built, hd):
+    with pytest.raises(RuntimeError, match="head_dim|aligned"):
+        tree(q=torch.zeros(6, 2 * hd, dtype=torch.float16), k=torch.zeros(5, 64, 2, hd, dtype=torch.float16), v=torch.zeros(5, 64, 2, hd, dtype=torch.float16))
+
+
+def test_nothing_to_do_is_no_error(built):
+    e = torch.zeros(0, dtype=torch.int32)
+    tree(base=e, row_start=torch.zeros(1, dtype=torch.int32))
+    tree(q=torch.zeros(0, 256, dtype=torch.float16), mask=torch.zeros(0, 1, dtype=torch.int64))
+    ec.sample(e, torch.zeros(0, 7), torch.zeros(0))
+    k = torch.zeros(2, 5, 64, 128, dtype=torch.float16)
+    ec.kv_copy(k, k.clone(), torch.zeros(1, 2, dtype=torch.int32), e, e, e, e)
+
+
+def commit(**kw):
+    n, rows = 2, 6
+    i = lambda *s: torch.zeros(*s, dtype=torch.int32)  # noqa: E731
+    k = torch.zeros(3, 5, 64, 128, dtype=torch.float16)
+    t = dict(k=k, v=k.clone(), page_table=i(n, 2), row_start=i(n + 1), base=i(n), mask=torch.zeros(rows, 1, dtype=torch.int64), tokens=i(rows), picked=i(rows),
+             accepted=i(n, 4), n_accepted=i(n), new_base=i(n))
+    t.update(kw)
+    ec.tree_commit(**t)
+
+
+@pytest.mark.parametrize("kw,error,says", [
+    (dict(k=torch.zeros(3, 5, 64, 128)), ValueError, "alike"),
+    (dict(k=torch.zeros(3, 5, 64, 128), v=torch.zeros(3, 5, 64, 128)), RuntimeError, "fp16 or bf16"),
+    (dict(k=torch.zeros(3, 5, 64, 100, dtype=torch.float16), v=torch.zeros(3, 5, 64, 100, dtype=torch.float16)), RuntimeError, "aligned"),
+    (dict(picked=torch.zeros(5, dtype=torch.int32)), ValueError, "picked"),
+    (dict(accepted=torch.zeros(3, 4, dtype=torch.int32)), ValueError, "accepted"),
+    (dict(accepted=torch.zeros(2, 0, dtype=torch.int32)), RuntimeError, "max_path"),
+    (dict(n_accepted=torch.zeros(1, dtype=torch.int32)), ValueError, "n_accepted"),
+    (dict(new_base=torch.zeros(2)), ValueError, "new_base"),
+    (dict(), RuntimeError, "device"),
+])
+def test_tree_commit(built, kw, error, says):
+    with pytest.raises(error, match=says):
+        commit(**kw)
+
+
+@pytest.mark.parametrize("kw,error,says", [
+    (dict(dst=torch.zeros(3, dtype=torch.int32)), ValueError, "dst"),
+    (dict(start=torch.zeros(2)), ValueError, "start"),
+    (dict(end=torch.zeros(4, dtype=torch.int32)[::2]), ValueError, "end"),
+    (dict(), RuntimeError, "device"),
+])
+def test_kv_copy(built, kw, error, says):
+    i = torch.zeros(2, dtype=torch.int32)
+    k = torch.zeros(3, 5, 64, 128, dtype=torch.float16)
+    with pytest.raises(error, match=says):
+        ec.kv_copy(**(dict(k=k, v=k.clone(), page_table=torch.zeros(2, 2, dtype=torch.int32), src=i, dst=i, start=i, end=i) | kw))
+
+
+@pytest.mark.parametrize("kw,error,says", [
+    (dict(ids=torch.zeros(3, dtype=torch.int64)), ValueError, "ids"),
+    (dict(u=torch.zeros(2)), ValueError, "u has"),
+    (dict(u=torch.zeros(3, dtype=torch.float64)), ValueError, "u must"),
+    (dict(top_k=torch.zeros(3)), ValueError, "top_k"),
+    (dict(top_p=torch.zeros(1)), ValueError, "top_p"),
+    (dict(min_p=torch.zeros(3, dtype=torch.float16)), ValueError, "min_p"),
+    (dict(temperature=torch.zeros(6)[::2]), ValueError, "temperature"),
+    (dict(prob=torch.zeros(4)), ValueError, "prob"),
+    (dict(logits=torch.zeros(3, 9, dtype=torch.float64)), RuntimeError, "type"),
+    (dict(logits=torch.zeros(9, 3).T), ValueError, "logits"),
+    (dict(logits=torch.zeros(3, 0)), RuntimeError, "vocab"),
+    (dict(logits=torch.zeros(1, 9).expand(3, 9)), RuntimeError, "stride"),
+    (dict(), RuntimeError, "device"),
+])
+def test_sample(built, kw, error, says):
+    with pytest.raises(error, match=says):
+        ec.sample(**(dict(ids=torch.zeros(3, dtype=torch.int32), logits=torch.zeros(3, 9), u=torch.zeros(3)) | kw))
+
+
+def test_c_entries_refuse_null(built):
+    lib = ec.load_library()
+    assert lib.ec_tree_attention(None, None, None) == -1 and "arena" in ec.last_error()
+    assert lib.ec_tree_commit(None, None, None) == -1
+    assert lib.ec_kv_copy(None, 1, None, None, None, None, None) == -1
+    assert lib.ec_sample(None, None, None, 0, 1, 1, 1, None, None, None, None, None, None) == -1
+    assert lib.ec_model_kv(None, None) == -1
+    k = torch.zeros(1, 5, 64, 128, dtype=torch.float16)
+    kv = ec._layers(k, k.clone(), torch.zeros(1, 2, dtype=torch.int32))
+    assert lib.ec_tree_attention(C.addressof(kv), None, None) == -1 and "no arguments" in ec.last_error()
+    for field, value in (("n_pages", 0), ("pages_per_slot", 1 << 26), ("ld_pos", 120), ("ld_pos", 132), ("k", kv.k + 2), ("type", 0)):
+        bad = ec._layers(k, k.clone(), torch.zeros(1, 2, dtype=torch.int32))
+        setattr(bad, field, value)
+        assert lib.ec_tree_commit(C.addressof(bad), C.addressof(ec._TreePath(1, 0, 1, 1)), None) == -1, field
+
+
+def test_tree_mask():
+    m = ec.tree_mask([-1, 0, 0, 1, 3, -1])
+    assert m.dtype == np.int64 and m[:, 0].tolist() == [1, 3, 5, 11, 27, 32]
+    deep = ec.tree_mask([-1] + list(range(129))).view(np.uint64)
+    assert deep.shape == (130, 3) and deep[129].tolist() == [2 ** 64 - 1, 2 ** 64 - 1, 3]
+    assert ec.tree_mask([]).shape == (0, 1)
+    for bad in ([0], [-2], [-1, 1], [-1, 0, 5]):
+        with pytest.raises(ValueError):
+            ec.tree_mask(bad)
