@@ -106,13 +106,13 @@ EC_EXPORT int ec_tree_attention(const ec_kv_pages *kv, const ec_tree_attn *a, vo
     if ((long long)a->n_kv_head * a->head_dim != kv->dim)
         return refuse("%s: %d KV heads of %d in an arena of dim %d", fn, a->n_kv_head, a->head_dim, kv->dim);
     const long long wide = (long long)a->n_head * a->head_dim;
-    if (wide > (1 << 24)) return refuse("%s: %d heads of %d", fn, a->n_head, a->head_dim);
+    if (wide > (1 << 24) || a->n_kv_head > 65535) return refuse("%s: %d heads of %d", fn, a->n_head, a->head_dim);
     if (a->rows > 1 && (a->ldq < wide || a->ldo < wide))
         return refuse("%s: row strides %lld / %lld below %lld", fn, a->ldq, a->ldo, wide);
     if (a->mask_words < 1) return refuse("%s: mask_words %d", fn, a->mask_words);
     if (a->window < 0 || a->max_len < 0) return refuse("%s: window %d, max_len %d", fn, a->window, a->max_len);
     if (!(a->scale >= 0.0f) || a->scale > 3.0e38f) return refuse("%s: scale %g", fn, (double)a->scale);
-    if ((long long)a->rows * (a->n_head / a->n_kv_head) > 0x7fffffffLL) return refuse("%s: %d rows", fn, a->rows);
+    if ((long long)a->rows * (a->n_head / a->n_kv_head) > 0x3fffffffLL || a->n_seq > 0x3fffffff) return refuse("%s: %d rows", fn, a->rows);
     if (a->work && ((uintptr_t)a->work & 255)) return refuse("%s: work must be 256-byte aligned", fn);
     if (a->n_seq == 0 || a->rows == 0) return 0;
     int dev, sms;
