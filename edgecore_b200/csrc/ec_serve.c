@@ -182,6 +182,8 @@ EC_EXPORT int ec_sample(int *ids, float *prob, const void *logits, int type, lon
     static const char fn[] = "ec_sample";
     if (type != EC_T_F32 && type != EC_T_F16 && type != EC_T_BF16) return refuse("%s: type %d", fn, type);
     if (rows < 0 || vocab < 1) return refuse("%s: rows %d, vocab %d", fn, rows, vocab);
+    if (vocab > EC_SAMPLE_MAX_VOCAB) return refuse("%s: vocab %d (at most %d)", fn, vocab, EC_SAMPLE_MAX_VOCAB);
+    if (rows > 0x07ffffff) return refuse("%s: rows %d", fn, rows);
     if (rows > 1 && ld < vocab) return refuse("%s: row stride %lld below vocab %d", fn, ld, vocab);
     if (rows == 0) return 0;
     int dev, sms;
@@ -191,5 +193,7 @@ EC_EXPORT int ec_sample(int *ids, float *prob, const void *logits, int type, lon
     if (on_device(fn, dev, o, (int)(sizeof o / sizeof o[0]))) return -1;
     if ((uintptr_t)logits & (uintptr_t)(type == EC_T_F32 ? 3 : 1)) return refuse("%s: logits must be aligned to their element", fn);
     const ec_sample_args a = {ids, prob, logits, ld, type, rows, vocab, temperature, top_k, top_p, min_p, u};
-    return launched(fn, ec_launch_sample(&a, sms, (cudaStream_t)stream));
+    int *err = ec_error_word();
+    if (!err) return refuse("%s: no device error word", fn);
+    return launched(fn, ec_launch_sample(&a, sms, err, (cudaStream_t)stream));
 }

@@ -31,7 +31,8 @@ typedef struct {
     const int *top_k;
     const float *top_p, *min_p, *u;
 } ec_sample_args;
-int ec_launch_sample(const ec_sample_args *a, int num_sms, cudaStream_t stream);
+int ec_launch_sample(const ec_sample_args *a, int num_sms, int *err, cudaStream_t stream);
+#define EC_SAMPLE_MAX_VOCAB 750000   /* a cluster of 16 CTAs holds a row in shared memory */
 
 #ifdef __cplusplus
 }

@@ -367,8 +367,9 @@ int ec_kv_copy(const ec_kv_pages *kv, int n_copies, const int *src, const int *d
  * ids[r] = the token, prob[r] (may be NULL) = its share of the kept w.  NaN
  * counts as -inf; among +inf logits all weights are equal; a row without any
  * logit above -inf gives id -1 and prob 0.  The sums are exact integers of
- * weights rounded to 2^-(62 - log2 vocab), so a row's result depends on
- * neither the other rows nor the launch. */
+ * weights rounded to a multiple of 2^-s, s = min(50, 62 - ceil(log2 vocab)),
+ * so a row's result depends on neither the other rows nor the launch.  vocab
+ * is at most 750000. */
 int ec_sample(int *ids, float *prob, const void *logits, int type, long long ld, int rows, int vocab,
               const float *temperature, const int *top_k, const float *top_p, const float *min_p,
               const float *u, void *stream);
