@@ -24,7 +24,7 @@ namespace {
 typedef unsigned long long u64;
 constexpr int SA_THREADS = 512, SA_WARPS = SA_THREADS / 32;
 constexpr int SA_BINS = 1024, SA_LIST = 2048, SA_PER = SA_LIST / SA_THREADS;
-constexpr int SA_TAB = 128;                       // entries of the 2^(j/128) table
+constexpr int SA_TAB = 512;                       // entries of the 2^(j/512) table
 constexpr int SA_MAX_CTAS = 16;
 
 template <int T> struct SaElt { typedef float V; };
@@ -57,7 +57,7 @@ struct SaCtl {                 // what the first CTA tells the others
 };
 
 struct SaShared {
-    double tab[SA_TAB];        // 2^(j / 128)
+    double tab[SA_TAB];        // 2^(j / 512)
     u64 part[SA_WARPS + 1];
     u64 sums[SA_MAX_CTAS];     // each CTA's weight
     float high[SA_MAX_CTAS], low[SA_MAX_CTAS];
@@ -72,31 +72,34 @@ struct SaShared {
     };
 };
 
-// w(v) * 2^shift in double, not yet rounded to an integer.  With t = (v - max)
-// log2(e) / T = j/128 + f, |f| <= 1/256: 2^t = 2^(j div 128) tab[j mod 128]
-// e^(f ln 2), the last as its Taylor sum to the fourth power (0.0028^5 / 120,
-// 2^-49 of it).  Below 2^-(shift + 2) it is 0, and so it is for NaN.
+// w(v) * 2^shift in double, not yet rounded to an integer.  With t = 512 (v -
+// max) log2(e) / T = j + f, |f| <= 1/2: 2^(t/512) = 2^(j div 512) tab[j mod
+// 512] e^(f ln 2 / 512), the last as its Taylor sum to the third power
+// (0.00068^4 / 24 = 2^-46.7 of it is left out).  0 for v below `floor`, where
+// it is less than 2^-(shift + 2), and for NaN.
 struct SaWeight {
-    double mx, c;
+    double mx, c;              // c: 512 log2(e) / T
+    float floor;
     int shift;
     const double *tab;
     EC_DEV double operator()(float v) const {
-        const double t = ((double)v - mx) * c;
-        if (!(t >= -(double)(shift + 2))) return 0.0;
+        if (!(v >= floor)) return 0.0;
         const double magic = 6755399441055744.0;      // 1.5 * 2^52
-        const double kd = __fma_rn(t, 128.0, magic);
+        const double d = (double)v - mx;
+        const double kd = __fma_rn(d, c, magic);
         const int j = __double2loint(kd);
-        const double f = __fma_rn(kd - magic, -1.0 / 128.0, t);
-        double p = __fma_rn(f, 9.618129107628477e-3, 5.550410866482158e-2);   // ln2^n / n!
-        p = __fma_rn(f, p, 2.402265069591007e-1);
-        p = __fma_rn(f, p, 6.931471805599453e-1);
+        const double f = __fma_rn(d, c, magic - kd);
+        double p = __fma_rn(f, 4.1353783506767136e-10, 9.163913992275265e-7);   // (ln2 / 512)^n / n!
+        p = __fma_rn(f, p, 1.3538030870311431e-3);
         p = __fma_rn(f, p, 1.0);
         const double s = p * tab[j & (SA_TAB - 1)];
-        return __hiloint2double(__double2hiint(s) + (((j >> 7) + shift) << 20), __double2loint(s));
+        return __hiloint2double(__double2hiint(s) + (((j >> 9) + shift) << 20), __double2loint(s));
     }
-    static EC_DEV u64 whole(double w) {                // w < 2^52, rounded to nearest
-        return (u64)__double_as_longlong(w + 4503599627370496.0) & 0xfffffffffffffull;
-    }
+    // A weight (below 2^52) rounded to nearest, plus RAW: sums of these wrap
+    // and are put right by the number of terms.
+    static constexpr u64 RAW = 0x4330000000000000ull;
+    static EC_DEV u64 raw(double w) { return (u64)__double_as_longlong(w + 4503599627370496.0); }
+    static EC_DEV u64 whole(double w) { return raw(w) - RAW; }
 };
 
 EC_DEV u64 sa_warp_sum(u64 v) {
@@ -143,29 +146,297 @@ EC_DEV void sa_sort(u64 *list, int n) {
 
 EC_DEV int sa_pow2(int n) { return n <= 1 ? 1 : 1 << (32 - __clz(n - 1)); }
 
+// A CTA's share of a row in shared memory, in whole 16-byte blocks; places
+// that are not the row's hold -inf.
+template <int T> struct SaRow {
+    typedef typename SaElt<T>::V V;
+    static constexpr int ELT = sizeof(V), PER = 16 / ELT;
+    SaShared &s;
+    const uint4 *blocks;
+    int n, ibase;              // blocks; index in the row of place 0
+    SaWeight weight;
+    float mx, per_bin;
+    float cut_v;               // kept: larger, or equal and up to index cut_i
+    int cut_i;
+    bool cut;
+
+    EC_DEV float at(int place) const { return sa_value<T>(reinterpret_cast<const V *>(blocks)[place]); }
+    EC_DEV bool kept(float v, int place) const { return v > cut_v || (v == cut_v && place + ibase <= cut_i); }
+    EC_DEV int bin(float v) const { return min((int)(fminf(mx - v, FLT_MAX) * per_bin), SA_BINS - 1); }   // of v >= weight.floor
+
+    // f(value, place) for blocks [b0, b1), taken by threads t of `threads`
+    template <typename F> EC_DEV void each(int b0, int b1, int t, int threads, F f) const {
+#pragma unroll 2
+        for (int b = b0 + t; b < b1; b += threads) {
+            const uint4 u = blocks[b];
+            if constexpr (T == EC_T_F32) {
+                const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+                for (int j = 0; j < 4; ++j) f(__uint_as_float(w[j]), b * 4 + j);
+            } else {
+                const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+                for (int j = 0; j < 8; ++j) f(ec_h2f((uint16_t)(w[j / 2] >> (16 * (j % 2))), T == EC_T_BF16), b * 8 + j);
+            }
+        }
+    }
+    // Raw weights (SaWeight::raw) of what is kept and weighs at least `least`,
+    // summed; `terms` counts them.
+    template <bool CUT, bool LEAST> EC_DEV u64 sum(int b0, int b1, int t, int threads, double least) const {
+        u64 raw = 0;
+        int terms = 0;
+        each(b0, b1, t, threads, [&](float v, int p) {
+            if (CUT && !kept(v, p)) return;
+            const double w = weight(v);
+            if (LEAST && !(w >= least)) return;
+            raw += SaWeight::raw(w);
+            ++terms;
+        });
+        return raw - (u64)terms * SaWeight::RAW;
+    }
+    EC_DEV u64 sum(int b0, int b1, int t, int threads, double least) const {
+        return least > 0.0 ? (cut ? sum<true, true>(b0, b1, t, threads, least) : sum<false, true>(b0, b1, t, threads, least))
+                           : (cut ? sum<true, false>(b0, b1, t, threads, least) : sum<false, false>(b0, b1, t, threads, least));
+    }
+};
+
+// Finds the candidate at which the running count (MASS: weight, among those
+// kept so far) over the order reaches what is wanted, and cuts there.  With
+// `whole`, everything up to it may be left unsorted in the first CTA's list
+// instead, each CTA's number in its `first`; returns true then.  All CTAs of
+// the cluster call it alike.
+template <bool MASS, int T>
+EC_DEV bool sa_select(cg::cluster_group &cl, SaRow<T> &row, u64 want, float top_p, bool whole) {
+    SaShared &s = row.s;
+    const int ctas = (int)cl.num_blocks(), me = (int)cl.block_rank(), tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    u64 above = 0, prefix = 0;
+    int bits = 64, bin = -1;   // from the second round: candidates of `bin` whose rank's top 64 - bits bits are `prefix`
+    const float floor = row.weight.floor;
+    auto in_class = [&](float v, int p) {
+        if (!(v >= floor) || row.bin(v) != bin || (MASS && row.cut && !row.kept(v, p))) return false;
+        return bits == 64 || (sa_rank(v, p + row.ibase) >> bits) == prefix;
+    };
+    for (;;) {
+        __syncthreads();
+        for (int b = tid; b < SA_BINS; b += SA_THREADS) s.h.count[b] = s.h.limb[0][b] = s.h.limb[1][b] = s.h.limb[2][b] = 0;
+        if (tid == 0) s.count = 0;
+        __syncthreads();
+        const int step = bits - 10 > 0 ? bits - 10 : 0;
+        auto add = [&](float v, int b) {
+            atomicAdd(&s.h.count[b], 1u);
+            if (MASS) {
+                const u64 w = SaWeight::whole(row.weight(v));
+                if (w & 0xffff) atomicAdd(&s.h.limb[0][b], (uint32_t)(w & 0xffff));
+                if (w >> 16 & 0xffff) atomicAdd(&s.h.limb[1][b], (uint32_t)(w >> 16 & 0xffff));
+                if (w >> 32) atomicAdd(&s.h.limb[2][b], (uint32_t)(w >> 32));
+            }
+        };
+        if (bin < 0)
+            row.each(0, row.n, tid, SA_THREADS, [&](float v, int p) {
+                if (v >= floor && (!MASS || !row.cut || row.kept(v, p))) add(v, row.bin(v));
+            });
+        else
+            row.each(0, row.n, tid, SA_THREADS, [&](float v, int p) {
+                if (in_class(v, p)) add(v, SA_BINS - 1 - (int)((sa_rank(v, p + row.ibase) >> step) & (SA_BINS - 1)));
+            });
+        cl.sync();
+        if (me == 0) {   // join the histograms, find the crossing
+            u64 cnt[2] = {0, 0}, sum[2] = {0, 0};
+            for (int c = 0; c < ctas; ++c) {
+                const SaShared *o = cl.map_shared_rank(&s, c);
+                const uint2 q = reinterpret_cast<const uint2 *>(o->h.count)[tid];
+                cnt[0] += q.x;
+                cnt[1] += q.y;
+                if (MASS)
+#pragma unroll
+                    for (int l = 0; l < 3; ++l) {
+                        const uint2 m = reinterpret_cast<const uint2 *>(o->h.limb[l])[tid];
+                        sum[0] += (u64)m.x << (16 * l);
+                        sum[1] += (u64)m.y << (16 * l);
+                    }
+            }
+            if (!MASS) { sum[0] = cnt[0]; sum[1] = cnt[1]; }
+            u64 total;
+            u64 before = above + sa_scan(sum[0] + sum[1], s, total);
+            if (MASS && bin < 0) want = max(1ull, min(total, (u64)ceil((double)top_p * (double)total)));
+            if (tid == 0) s.ctl.bin = -1;
+            __syncthreads();
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+                if (before < want && before + sum[q] >= want) {
+                    s.ctl.bin = 2 * tid + q;
+                    s.ctl.crowd = (int)cnt[q];
+                    s.ctl.above = before;
+                    s.ctl.want = want;
+                }
+                before += sum[q];
+            }
+            __syncthreads();
+            // all up to the crossing, where they fit the list and it is asked for
+            const bool all = whole && bin < 0 && s.ctl.bin >= 0 && s.ctl.above + s.ctl.crowd <= SA_LIST;
+            if (warp == 0) {
+                int c = 0;
+                if (lane < ctas && s.ctl.bin >= 0 && !all) c = (int)cl.map_shared_rank(&s, lane)->h.count[s.ctl.bin];
+                int sum32 = c;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const int u = __shfl_up_sync(0xffffffffu, sum32, o);
+                    if (lane >= o) sum32 += u;
+                }
+                if (lane < ctas) s.ctl.at[lane] = all ? -1 : sum32 - c;
+            }
+            __syncthreads();
+            if (tid < ctas) cl.map_shared_rank(&s, tid)->ctl = s.ctl;
+        }
+        cl.sync();
+        const int crossing = s.ctl.bin, crowd = s.ctl.crowd, place = s.ctl.at[me];
+        if (crossing < 0) return false;   // fewer than wanted have any weight: nothing to cut
+        want = s.ctl.want;
+        above = s.ctl.above;
+        u64 *list = cl.map_shared_rank(&s, 0)->l.rank;
+        if (place < 0) {                  // everything up to the crossing goes to the list
+            int c = 0;
+            for (int b = tid; b <= crossing; b += SA_THREADS) c += (int)s.h.count[b];
+            u64 total;
+            sa_scan((u64)c, s, total);
+            if (tid == 0) cl.map_shared_rank(&s, 0)->first[me] = (int)total;
+            cl.sync();
+            int at = 0;
+            for (int q = 0; q < me; ++q) at += cl.map_shared_rank(&s, 0)->first[q];
+            row.each(0, row.n, tid, SA_THREADS, [&](float v, int p) {
+                if (v >= floor && row.bin(v) <= crossing) list[at + atomicAdd(&s.count, 1)] = sa_rank(v, p + row.ibase);
+            });
+            cl.sync();
+            return true;
+        }
+        if (bin < 0) {
+            bin = crossing;
+        } else {
+            prefix = prefix << (bits - step) | ((u64)(SA_BINS - 1 - crossing) & ((1ull << (bits - step)) - 1));
+            bits = step;
+        }
+        if (crowd > SA_LIST) continue;
+        row.each(0, row.n, tid, SA_THREADS, [&](float v, int p) {
+            if (in_class(v, p)) list[place + atomicAdd(&s.count, 1)] = sa_rank(v, p + row.ibase);
+        });
+        cl.sync();
+        if (me == 0) {
+            const int size = sa_pow2(crowd);
+            for (int i = tid; i < size; i += SA_THREADS)
+                if (i >= crowd) s.l.rank[i] = 0;
+            sa_sort(s.l.rank, size);
+            u64 w[SA_PER], sum = 0, total;
+#pragma unroll
+            for (int j = 0; j < SA_PER; ++j) {
+                const int i = tid * SA_PER + j;
+                w[j] = i >= crowd ? 0ull : MASS ? SaWeight::whole(row.weight(sa_rank_value(s.l.rank[i]))) : 1ull;
+                sum += w[j];
+            }
+            u64 before = above + sa_scan(sum, s, total);
+#pragma unroll
+            for (int j = 0; j < SA_PER; ++j) {
+                if (before < want && before + w[j] >= want) s.ctl.cut = s.l.rank[tid * SA_PER + j];
+                before += w[j];
+            }
+            __syncthreads();
+            if (tid < ctas) cl.map_shared_rank(&s, tid)->ctl.cut = s.ctl.cut;
+        }
+        cl.sync();
+        row.cut = true;
+        row.cut_v = sa_rank_value(s.ctl.cut);
+        row.cut_i = sa_rank_index(s.ctl.cut);
+        return false;
+    }
+}
+
+// The point u of a sum of whole weights: the running sum has to exceed it.
+EC_DEV u64 sa_point(float u, u64 total) {
+    const double x = u > 0.0f ? (double)u * (double)total : 0.0;
+    return x >= (double)total ? total - 1 : min((u64)x, total - 1);
+}
+
+// The draw from the first CTA's list of `size` candidates, of which the first
+// top_k in the order count.
+template <int T>
+EC_DEV void sa_draw_list(const ec_sample_args &a, SaRow<T> &row, int r, int size, int top_k, float top_p, double least) {
+    SaShared &s = row.s;
+    const int tid = threadIdx.x, full = sa_pow2(size);
+    for (int i = tid; i < full; i += SA_THREADS)
+        if (i >= size) s.l.rank[i] = 0;
+    sa_sort(s.l.rank, full);
+    u64 w[SA_PER], sum = 0, total;
+    double wd[SA_PER];
+#pragma unroll
+    for (int j = 0; j < SA_PER; ++j) {
+        const int i = tid * SA_PER + j;
+        wd[j] = i < top_k && i < size ? row.weight(sa_rank_value(s.l.rank[i])) : 0.0;
+        w[j] = SaWeight::whole(wd[j]);
+        sum += w[j];
+    }
+    u64 before = sa_scan(sum, s, total);
+    const u64 want = top_p < 1.0f ? max(1ull, min(total, (u64)ceil((double)top_p * (double)total))) : total;
+    u64 kept = 0;
+#pragma unroll
+    for (int j = 0; j < SA_PER; ++j) {   // kept: what comes before `want` is reached, and weighs enough
+        const int i = tid * SA_PER + j;
+        const bool keep = w[j] > 0 && before < want && (wd[j] >= least || i == 0);
+        before += w[j];
+        kept += keep ? w[j] : 0ull;
+        s.l.w[i] = (u64)__double_as_longlong(wd[j]);
+        s.l.rank[i] = keep ? (u64)(uint32_t)~sa_rank_index(s.l.rank[i]) << 32 | (uint32_t)i : 0ull;   // lowest index largest
+    }
+    sa_scan(kept, s, total);
+    const int most = sa_pow2(min(size, top_k));
+    sa_sort(s.l.rank, most);
+    const u64 target = sa_point(a.u[r], total);
+    sum = 0;
+#pragma unroll
+    for (int j = 0; j < SA_PER; ++j) {
+        const int i = tid * SA_PER + j;
+        const u64 k = i < most ? s.l.rank[i] : 0ull;
+        wd[j] = k ? __longlong_as_double((long long)s.l.w[(uint32_t)k]) : 0.0;
+        w[j] = SaWeight::whole(wd[j]);
+        sum += w[j];
+    }
+    u64 all;
+    before = sa_scan(sum, s, all);
+#pragma unroll
+    for (int j = 0; j < SA_PER; ++j) {
+        if (before <= target && target < before + w[j]) {
+            a.ids[r] = (int)~(uint32_t)(s.l.rank[tid * SA_PER + j] >> 32);
+            if (a.prob) a.prob[r] = (float)(wd[j] / (double)total);
+        }
+        before += w[j];
+    }
+}
+
 // One cluster of CTAs per row: each keeps its share of the row in shared
 // memory, so that the logits are read from HBM once.
 template <int T>
-__global__ void __launch_bounds__(SA_THREADS) k_sample(const ec_sample_args a, int shift, int share, int *err) {
+__global__ void __launch_bounds__(SA_THREADS, 2) k_sample(const ec_sample_args a, int shift, int share, int *err) {
     EC_PDL_ENTER();
-    typedef typename SaElt<T>::V V;
-    constexpr int ELT = sizeof(V), PER16 = 16 / ELT;
+    typedef SaRow<T> Row;
+    typedef typename Row::V V;
+    constexpr int ELT = Row::ELT, PER = Row::PER;
     extern __shared__ __align__(128) unsigned char smem[];
     SaShared &s = *reinterpret_cast<SaShared *>(smem);
     V *vals = reinterpret_cast<V *>(smem + (sizeof(SaShared) + 127) / 128 * 128);
     cg::cluster_group cl = cg::this_cluster();
     const int ctas = (int)cl.num_blocks(), me = (int)cl.block_rank();
     const int r = (int)blockIdx.x / ctas, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const float temperature = a.temperature ? a.temperature[r] : 1.0f, min_p = a.min_p ? a.min_p[r] : 0.0f, top_p = a.top_p ? a.top_p[r] : 1.0f;
+    const int top_k = a.top_k ? a.top_k[r] : 0;
 
     // Shares are cut at 16-byte blocks of memory: element i of the row is
     // element i + skew of the block that holds its first one.
-    const V *row = static_cast<const V *>(a.logits) + (size_t)r * a.ld;
-    const int skew = (int)((reinterpret_cast<uintptr_t>(row) & 15) / ELT);
+    const V *src = static_cast<const V *>(a.logits) + (size_t)r * a.ld;
+    const int skew = (int)((reinterpret_cast<uintptr_t>(src) & 15) / ELT);
     const long long lo = max((long long)me * share, (long long)skew), hi = min((long long)(me + 1) * share, (long long)skew + a.vocab);
-    const int n = (int)max(0ll, hi - lo), off = (int)(lo - (long long)me * share), i0 = (int)(lo - skew);   // vals[off + e] is element i0 + e
+    const int n = (int)max(0ll, hi - lo), off = n > 0 ? (int)(lo - (long long)me * share) : 0, i0 = (int)(lo - skew);   // vals[off + e] is element i0 + e
+    const int blocks = (off + n + PER - 1) / PER;
     {
-        // 16-byte blocks wholly inside the row by one bulk copy, the rest element by element
-        const int b0 = (off + PER16 - 1) / PER16 * PER16, b1 = (off + n) / PER16 * PER16;
+        // blocks wholly inside the row by one bulk copy, the rest element by element
+        const int b0 = (off + PER - 1) / PER * PER, b1 = (off + n) / PER * PER;
         const bool bulk = b1 > b0;
         uint64_t *bar = reinterpret_cast<uint64_t *>(&s.bar);
         if (tid == 0) {
@@ -173,26 +444,32 @@ __global__ void __launch_bounds__(SA_THREADS) k_sample(const ec_sample_args a, i
             ec_fence_mbar_init();
             if (bulk) {
                 ec_mbar_expect_tx(bar, (uint32_t)((b1 - b0) * ELT));
-                ec_bulk_g2s(vals + b0, row + i0 + (b0 - off), (uint32_t)((b1 - b0) * ELT), bar);
+                ec_bulk_g2s(vals + b0, src + i0 + (b0 - off), (uint32_t)((b1 - b0) * ELT), bar);
             }
         }
-        const int head = bulk ? b0 - off : n, tail = bulk ? b1 - off : n;
-        for (int e = tid; e < head; e += SA_THREADS) vals[off + e] = row[i0 + e];
-        for (int e = tail + tid; e < n; e += SA_THREADS) vals[off + e] = row[i0 + e];
-        if (tid < SA_TAB) s.tab[tid] = exp2((double)tid / SA_TAB);
-        if (tid == 0) s.found = 0;
+        for (int e = tid; e < blocks * PER; e += SA_THREADS) {
+            if (bulk && e >= b0 && e < b1) {
+                if (e + SA_THREADS < b1) e += (b1 - 1 - e) / SA_THREADS * SA_THREADS - SA_THREADS;
+                continue;
+            }
+            vals[e] = e >= off && e < off + n ? src[i0 + e - off] : (V)(T == EC_T_F32 ? -INFINITY : T == EC_T_F16 ? 0xfc00 : 0xff80);
+        }
+        for (int j = tid; j < SA_TAB; j += SA_THREADS) s.tab[j] = exp2((double)j / SA_TAB);
         __syncthreads();
         if (bulk) ec_mbar_wait(bar, 0, err);   // a wait that gave up is reported; the row's result is then void
     }
-    const V *mine = vals + off;
+    Row row = {s, reinterpret_cast<const uint4 *>(vals), blocks, i0 - off};
 
-    // largest and smallest finite logit
+    // largest logit and, where the range of a histogram needs it, the smallest
+    const bool cuts = top_k > 0 || top_p < 1.0f;
     float mx = -INFINITY, mn = INFINITY;
-    for (int e = tid; e < n; e += SA_THREADS) {
-        const float v = sa_value<T>(mine[e]);
-        mx = fmaxf(mx, v);
-        if (fabsf(v) < INFINITY) mn = fminf(mn, v);
-    }
+    if (cuts)
+        row.each(0, blocks, tid, SA_THREADS, [&](float v, int) {
+            mx = fmaxf(mx, v);
+            if (fabsf(v) < INFINITY) mn = fminf(mn, v);
+        });
+    else
+        row.each(0, blocks, tid, SA_THREADS, [&](float v, int) { mx = fmaxf(mx, v); });
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
@@ -210,8 +487,6 @@ __global__ void __launch_bounds__(SA_THREADS) k_sample(const ec_sample_args a, i
     cl.sync();
     for (int c = 0; c < ctas; ++c) { mx = fmaxf(mx, s.high[c]); mn = fminf(mn, s.low[c]); }
 
-    const float temperature = a.temperature ? a.temperature[r] : 1.0f, min_p = a.min_p ? a.min_p[r] : 0.0f, top_p = a.top_p ? a.top_p[r] : 1.0f;
-    const int top_k = a.top_k ? a.top_k[r] : 0;
     if (mx == -INFINITY) {
         if (me == 0 && tid == 0) {
             a.ids[r] = -1;
@@ -221,8 +496,9 @@ __global__ void __launch_bounds__(SA_THREADS) k_sample(const ec_sample_args a, i
     }
     if (!(temperature > 0.0f) || min_p > 1.0f || top_k == 1 || top_p <= 0.0f) {   // one candidate is left: the first of the largest
         int first = 0x7fffffff;
-        for (int e = tid; e < n && first == 0x7fffffff; e += SA_THREADS)
-            if (sa_value<T>(mine[e]) == mx) first = i0 + e;
+        row.each(0, blocks, tid, SA_THREADS, [&](float v, int p) {
+            if (v == mx) first = min(first, p + row.ibase);
+        });
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) first = min(first, __shfl_xor_sync(0xffffffffu, first, o));
         __syncthreads();
@@ -238,259 +514,39 @@ __global__ void __launch_bounds__(SA_THREADS) k_sample(const ec_sample_args a, i
         }
         return;
     }
-    const bool infinite = mx == INFINITY;   // logits of +inf weigh the same, all others nothing
-    auto value = [&](int e) {
-        const float v = sa_value<T>(mine[e]);
-        return !infinite ? v : v == INFINITY ? 0.0f : -INFINITY;
-    };
-    if (infinite) mx = mn = 0.0f;
-    const SaWeight weight = {(double)mx, 1.4426950408889634 / (double)temperature, shift, s.tab};
-    // Bins over max - logit: up to where weights vanish, or the smallest logit.
+    if (mx == INFINITY) {   // logits of +inf weigh the same, all others nothing
+        for (int e = tid; e < blocks * PER; e += SA_THREADS)
+            vals[e] = sa_value<T>(vals[e]) == INFINITY ? (V)0 : (V)(T == EC_T_F32 ? -INFINITY : T == EC_T_F16 ? 0xfc00 : 0xff80);
+        __syncthreads();
+        mx = mn = 0.0f;
+    }
+    // Below `vanish` from the largest a weight is 0: only what lies above is
+    // ever a candidate.  (floor is the smallest float from there on.)
     const double vanish = (double)temperature * 0.6931471805599453 * (shift + 3);
-    const float reach = vanish < (double)FLT_MAX ? (float)vanish : FLT_MAX;
-    const float range = fmaxf(fminf(reach, mx - mn), 1e-30f), per_bin = (float)SA_BINS / range;
-    auto bin_of = [&](float v) {   // -1: no weight
-        const float x = fminf(mx - v, FLT_MAX);
-        return v > -INFINITY && x <= reach ? min((int)(x * per_bin), SA_BINS - 1) : -1;
-    };
-
-    u64 cut = 0;                            // rank of the last candidate kept
-    float cut_v = -INFINITY;
-    int cut_i = 0x7fffffff;
-    auto kept = [&](float v, int i) { return v > cut_v || (v == cut_v && i <= cut_i); };
-
-    // Finds the candidate at which the running count (or weight, among those
-    // kept so far) over the order reaches what is wanted, and cuts there.
-    // With `whole`, everything up to it may be left sorted in the first CTA's
-    // list instead; returns true then (all CTAs alike).
-    auto select = [&](const bool mass, u64 want, const bool whole) -> bool {
-        u64 above = 0, prefix = 0;
-        int bits = 64, bin = -1;            // candidates of `bin` whose rank's top 64 - bits bits are `prefix`
-        for (;;) {
-            __syncthreads();
-            for (int b = tid; b < SA_BINS; b += SA_THREADS) s.h.count[b] = s.h.limb[0][b] = s.h.limb[1][b] = s.h.limb[2][b] = 0;
-            if (tid == 0) s.count = 0;
-            __syncthreads();
-            const int step = bits - 10 > 0 ? bits - 10 : 0;
-            for (int e = tid; e < n; e += SA_THREADS) {
-                const float v = value(e);
-                int b = bin_of(v);
-                if (b < 0 || (mass && !kept(v, i0 + e))) continue;
-                if (bin >= 0) {
-                    const u64 k = sa_rank(v, i0 + e);
-                    if (b != bin || (bits < 64 && (k >> bits) != prefix)) continue;
-                    b = SA_BINS - 1 - (int)((k >> step) & (SA_BINS - 1));
-                }
-                atomicAdd(&s.h.count[b], 1u);
-                if (mass) {
-                    const u64 w = SaWeight::whole(weight(v));
-                    if (w & 0xffff) atomicAdd(&s.h.limb[0][b], (uint32_t)(w & 0xffff));
-                    if (w >> 16 & 0xffff) atomicAdd(&s.h.limb[1][b], (uint32_t)(w >> 16 & 0xffff));
-                    if (w >> 32) atomicAdd(&s.h.limb[2][b], (uint32_t)(w >> 32));
-                }
-            }
-            cl.sync();
-            if (me == 0) {   // join the histograms, find the crossing
-                u64 cnt[2] = {0, 0}, sum[2] = {0, 0};
-                for (int c = 0; c < ctas; ++c) {
-                    const SaShared *o = cl.map_shared_rank(&s, c);
-                    const uint2 q = reinterpret_cast<const uint2 *>(o->h.count)[tid];
-                    cnt[0] += q.x;
-                    cnt[1] += q.y;
-                    if (mass)
-#pragma unroll
-                        for (int l = 0; l < 3; ++l) {
-                            const uint2 m = reinterpret_cast<const uint2 *>(o->h.limb[l])[tid];
-                            sum[0] += (u64)m.x << (16 * l);
-                            sum[1] += (u64)m.y << (16 * l);
-                        }
-                }
-                if (!mass) { sum[0] = cnt[0]; sum[1] = cnt[1]; }
-                u64 total;
-                u64 before = above + sa_scan(sum[0] + sum[1], s, total);
-                if (mass && bin < 0) {
-                    want = (u64)ceil((double)top_p * (double)total);
-                    want = want < 1 ? 1 : want > total ? total : want;
-                }
-                if (tid == 0) s.ctl.bin = -1;
-                __syncthreads();
-#pragma unroll
-                for (int q = 0; q < 2; ++q) {
-                    if (before < want && before + sum[q] >= want) {
-                        s.ctl.bin = 2 * tid + q;
-                        s.ctl.crowd = (int)cnt[q];
-                        s.ctl.above = before;
-                        s.ctl.want = want;
-                    }
-                    before += sum[q];
-                }
-                __syncthreads();
-                // all up to the crossing, where they fit the list and it is asked for
-                const bool all = whole && bin < 0 && s.ctl.bin >= 0 && s.ctl.above + s.ctl.crowd <= SA_LIST;
-                if (warp == 0) {
-                    int c = 0;
-                    if (lane < ctas && s.ctl.bin >= 0 && !all) c = (int)cl.map_shared_rank(&s, lane)->h.count[s.ctl.bin];
-                    int sum32 = c;
-#pragma unroll
-                    for (int o = 1; o < 32; o <<= 1) {
-                        const int u = __shfl_up_sync(0xffffffffu, sum32, o);
-                        if (lane >= o) sum32 += u;
-                    }
-                    if (lane < ctas) s.ctl.at[lane] = all ? -1 : sum32 - c;
-                }
-                __syncthreads();
-                if (tid < ctas) cl.map_shared_rank(&s, tid)->ctl = s.ctl;
-            }
-            cl.sync();
-            const SaCtl ctl = s.ctl;
-            want = ctl.want;
-            if (ctl.bin < 0) return false;   // fewer than wanted have any weight: nothing to cut
-            above = ctl.above;
-            if (ctl.at[0] < 0) {             // everything up to the crossing goes to the list
-                // how many of this CTA's do, for its place in it
-                int c = 0;
-                for (int b = tid; b <= ctl.bin; b += SA_THREADS) c += (int)s.h.count[b];
-                u64 total;
-                sa_scan((u64)c, s, total);
-                if (tid == 0) cl.map_shared_rank(&s, 0)->first[me] = (int)total;
-                cl.sync();
-                const SaShared *o = cl.map_shared_rank(&s, 0);
-                int at = 0;
-                for (int q = 0; q < me; ++q) at += o->first[q];
-                u64 *list = cl.map_shared_rank(&s, 0)->l.rank;
-                cl.sync();                   // the first CTA's counts are read: its list may be written over them
-                for (int e = tid; e < n; e += SA_THREADS) {
-                    const float v = value(e);
-                    const int b = bin_of(v);
-                    if (b >= 0 && b <= ctl.bin) list[at + atomicAdd(&s.count, 1)] = sa_rank(v, i0 + e);
-                }
-                cl.sync();
-                return true;
-            }
-            if (bin < 0) {
-                bin = ctl.bin;
-            } else {
-                prefix = prefix << (bits - step) | ((u64)(SA_BINS - 1 - ctl.bin) & ((1ull << (bits - step)) - 1));
-                bits = step;
-            }
-            if (ctl.crowd > SA_LIST) continue;
-            u64 *list = cl.map_shared_rank(&s, 0)->l.rank;
-            for (int e = tid; e < n; e += SA_THREADS) {
-                const float v = value(e);
-                if (bin_of(v) != bin || (mass && !kept(v, i0 + e))) continue;
-                const u64 k = sa_rank(v, i0 + e);
-                if (bits < 64 && (k >> bits) != prefix) continue;
-                list[ctl.at[me] + atomicAdd(&s.count, 1)] = k;
-            }
-            cl.sync();
-            if (me == 0) {
-                const int size = sa_pow2(ctl.crowd);
-                for (int i = tid; i < size; i += SA_THREADS)
-                    if (i >= ctl.crowd) s.l.rank[i] = 0;
-                sa_sort(s.l.rank, size);
-                u64 w[SA_PER], sum = 0, total;
-#pragma unroll
-                for (int j = 0; j < SA_PER; ++j) {
-                    const int i = tid * SA_PER + j;
-                    w[j] = i >= ctl.crowd ? 0ull : mass ? SaWeight::whole(weight(sa_rank_value(s.l.rank[i]))) : 1ull;
-                    sum += w[j];
-                }
-                u64 before = above + sa_scan(sum, s, total);
-#pragma unroll
-                for (int j = 0; j < SA_PER; ++j) {
-                    if (before < want && before + w[j] >= want) s.ctl.cut = s.l.rank[tid * SA_PER + j];
-                    before += w[j];
-                }
-                __syncthreads();
-                if (tid < ctas) cl.map_shared_rank(&s, tid)->ctl.cut = s.ctl.cut;
-            }
-            cl.sync();
-            cut = s.ctl.cut;
-            cut_v = sa_rank_value(cut);
-            cut_i = sa_rank_index(cut);
-            return false;
-        }
-    };
-
-    const float u = a.u[r];
-    auto point = [&](u64 total) -> u64 {   // the sum has to exceed it
-        const double x = u > 0.0f ? (double)u * (double)total : 0.0;
-        return x >= (double)total ? total - 1 : min((u64)x, total - 1);
-    };
+    const float floor = fmaxf(__double2float_ru((double)mx - vanish), -FLT_MAX);
+    row.weight = {(double)mx, 512.0 * 1.4426950408889634 / (double)temperature, floor, shift, s.tab};
+    row.mx = mx;
+    row.per_bin = (float)SA_BINS / fmaxf(fminf(mx - floor, mx - mn), 1e-30f);
+    row.cut_v = -INFINITY;
+    row.cut_i = 0x7fffffff;
+    row.cut = false;
     const double least = min_p > 0.0f ? (double)min_p * (double)(1ull << shift) : 0.0;
 
-    if (top_k > 0 && top_k < a.vocab && select(false, (u64)top_k, top_k <= SA_LIST / 2)) {
+    if (top_k > 0 && top_k < a.vocab && sa_select<false>(cl, row, (u64)top_k, top_p, top_k <= SA_LIST / 2)) {
         if (me != 0) return;
-        // the list holds at least top_k candidates, in no order yet
         int size = 0;
         for (int c = 0; c < ctas; ++c) size += s.first[c];
-        const int full = sa_pow2(size);
-        for (int i = tid; i < full; i += SA_THREADS)
-            if (i >= size) s.l.rank[i] = 0;
-        sa_sort(s.l.rank, full);
-        u64 w[SA_PER], sum = 0, total;
-        double wd[SA_PER];
-#pragma unroll
-        for (int j = 0; j < SA_PER; ++j) {
-            const int i = tid * SA_PER + j;
-            wd[j] = i < top_k && i < size ? weight(sa_rank_value(s.l.rank[i])) : 0.0;
-            w[j] = SaWeight::whole(wd[j]);
-            sum += w[j];
-        }
-        u64 before = sa_scan(sum, s, total);
-        const u64 want = top_p < 1.0f ? max(1ull, min(total, (u64)ceil((double)top_p * (double)total))) : total;
-        u64 kept_sum = 0;
-#pragma unroll
-        for (int j = 0; j < SA_PER; ++j) {   // kept: what comes before `want` is reached, and weighs enough
-            const int i = tid * SA_PER + j;
-            const bool keep = w[j] > 0 && before < want && (wd[j] >= least || i == 0);
-            before += w[j];
-            if (!keep) w[j] = 0;
-            kept_sum += w[j];
-            s.l.w[i] = (u64)__double_as_longlong(wd[j]);
-            s.l.rank[i] = keep ? (u64)(uint32_t)~sa_rank_index(s.l.rank[i]) << 32 | (uint32_t)i : 0ull;   // lowest index largest
-        }
-        sa_scan(kept_sum, s, total);
-        const int kept_n = sa_pow2(min(size, top_k));
-        sa_sort(s.l.rank, kept_n);
-        const u64 target = point(total);
-        sum = 0;
-#pragma unroll
-        for (int j = 0; j < SA_PER; ++j) {
-            const int i = tid * SA_PER + j;
-            const u64 k = i < kept_n ? s.l.rank[i] : 0ull;
-            wd[j] = k ? __longlong_as_double((long long)s.l.w[(uint32_t)k]) : 0.0;
-            w[j] = SaWeight::whole(wd[j]);
-            sum += w[j];
-        }
-        u64 all;
-        before = sa_scan(sum, s, all);
-#pragma unroll
-        for (int j = 0; j < SA_PER; ++j) {
-            if (before <= target && target < before + w[j]) {
-                a.ids[r] = (int)~(uint32_t)(s.l.rank[tid * SA_PER + j] >> 32);
-                if (a.prob) a.prob[r] = (float)(wd[j] / (double)total);
-            }
-            before += w[j];
-        }
+        sa_draw_list(a, row, r, size, top_k, top_p, least);
         return;
     }
-    if (top_p < 1.0f) select(true, 0, false);
+    if (top_p < 1.0f) sa_select<true>(cl, row, 0ull, top_p, false);
 
     // Weights of the kept candidates in vocabulary order: of each warp's
     // contiguous piece, of the CTAs, then of the piece that holds the point.
-    const int piece = ((n + SA_WARPS - 1) / SA_WARPS + 31) / 32 * 32;
-    auto drawn = [&](int e) -> u64 {
-        const float v = value(e);
-        if (!kept(v, i0 + e)) return 0ull;
-        const double w = weight(v);
-        return w >= least ? SaWeight::whole(w) : 0ull;
-    };
-    u64 sum = 0;
-    for (int e = warp * piece + lane; e < min(n, (warp + 1) * piece); e += 32) sum += drawn(e);
-    sum = sa_warp_sum(sum);
+    const int piece = (blocks + SA_WARPS - 1) / SA_WARPS;
+    const u64 part = sa_warp_sum(row.sum(warp * piece, min(blocks, (warp + 1) * piece), lane, 32, least));
     __syncthreads();
-    if (lane == 0) s.part[warp] = sum;
+    if (lane == 0) s.part[warp] = part;
     __syncthreads();
     u64 total = 0;
     for (int w = 0; w < SA_WARPS; ++w) total += s.part[w];
@@ -502,18 +558,21 @@ __global__ void __launch_bounds__(SA_THREADS) k_sample(const ec_sample_args a, i
         if (c == me) before = total;
         total += s.sums[c];
     }
-    const u64 target = point(total);
+    const u64 target = sa_point(a.u[r], total);
     if (target < before || target >= before + s.sums[me]) return;
     int w = 0;
     while (before + s.part[w] <= target) before += s.part[w++];
-    const int e1 = min(n, (w + 1) * piece);
-    for (int b = w * piece; b < e1; b += SA_THREADS) {
-        const u64 x = b + tid < e1 ? drawn(b + tid) : 0ull;
+    const int end = min(blocks, (w + 1) * piece) * PER;
+    for (int p0 = w * piece * PER; p0 < end; p0 += SA_THREADS) {
+        const int p = p0 + tid;
+        const float v = p < end ? row.at(p) : -INFINITY;
+        const double x = !row.cut || row.kept(v, p) ? row.weight(v) : 0.0;
+        const u64 mine = x >= least ? SaWeight::whole(x) : 0ull;
         u64 all;
-        const u64 start = before + sa_scan(x, s, all);
-        if (start <= target && target < start + x) {
-            a.ids[r] = i0 + b + tid;
-            if (a.prob) a.prob[r] = (float)(weight(value(b + tid)) / (double)total);
+        const u64 start = before + sa_scan(mine, s, all);
+        if (start <= target && target < start + mine) {
+            a.ids[r] = p + row.ibase;
+            if (a.prob) a.prob[r] = (float)(x / (double)total);
         }
         before += all;
     }
