@@ -8,14 +8,17 @@
 // Candidates are ordered by (logit, then lowest index).  Top-k and top-p are
 // cuts in that order, found without sorting the row: a histogram over max -
 // logit gives the bin in which the running count or weight crosses, and only
-// the candidates of that bin are sorted; a bin of more than SA_LIST of them
-// (equal logits) is first cut down by the bits of their order.  A top-k of up
-// to SA_LIST candidates is gathered whole and handled from the sorted list.
+// the candidates of that bin are put in order; a bin of more than SA_LIST of
+// them (equal logits) is first cut down by the bits of their order.  A top-k of
+// up to SA_FAST needs no histogram: at least top_k candidates lie at or above
+// the top_k-th largest of the maxima of SA_TOPS groups of the row, and those
+// few are gathered and handled by one CTA.
 #include "ec_common.cuh"
 #include "ec_serve.h"
 
 #include <cooperative_groups.h>
 #include <float.h>
+#include <stddef.h>
 
 namespace cg = cooperative_groups;
 
@@ -23,7 +26,10 @@ namespace {
 
 typedef unsigned long long u64;
 constexpr int SA_THREADS = 512, SA_WARPS = SA_THREADS / 32;
-constexpr int SA_BINS = 1024, SA_LIST = 2048, SA_PER = SA_LIST / SA_THREADS;
+constexpr int SA_WORDS = 4096;                    // words of a histogram: bins of counts, or two halves of weights
+constexpr int SA_LIST = 1024, SA_PER = SA_LIST / SA_THREADS;
+constexpr int SA_TOPS = 256, SA_FAST = 192;       // 192 of 256: about 1.4 * 256 candidates
+constexpr int SA_FEW = 256;                       // candidates that are ordered by counting
 constexpr int SA_TAB = 512;                       // entries of the 2^(j/512) table
 constexpr int SA_MAX_CTAS = 16;
 
@@ -38,62 +44,61 @@ template <int T> EC_DEV float sa_value(typename SaElt<T>::V v) {
 
 // Position of a candidate in the order, larger first: order-preserving bits of
 // the logit (-0 as +0), then the lower index.
-EC_DEV u64 sa_rank(float v, int i) {
+EC_DEV uint32_t sa_bits(float v) {
     const uint32_t b = __float_as_uint(v == 0.0f ? 0.0f : v);
-    return (u64)((b & 0x80000000u) ? ~b : (b | 0x80000000u)) << 32 | (uint32_t)~i;
+    return b ^ ((uint32_t)((int)b >> 31) | 0x80000000u);
 }
-EC_DEV float sa_rank_value(u64 r) {
-    const uint32_t k = (uint32_t)(r >> 32);
-    return __uint_as_float((k & 0x80000000u) ? (k & 0x7fffffffu) : ~k);
-}
+EC_DEV float sa_bits_value(uint32_t k) { return __uint_as_float((k & 0x80000000u) ? (k & 0x7fffffffu) : ~k); }
+EC_DEV u64 sa_rank(float v, int i) { return (u64)sa_bits(v) << 32 | (uint32_t)~i; }
+EC_DEV float sa_rank_value(u64 r) { return sa_bits_value((uint32_t)(r >> 32)); }
 EC_DEV int sa_rank_index(u64 r) { return (int)~(uint32_t)r; }
 
-struct SaCtl {                 // what the first CTA tells the others
-    int bin, crowd;            // crossing bin (-1: none), candidates in it
-    u64 above;                 // count or weight before it
-    u64 want;                  // what has to be reached
-    u64 cut;                   // rank of the last candidate kept
-    int at[SA_MAX_CTAS];       // where each CTA's candidates go in the list
-};
-
 struct SaShared {
-    double tab[SA_TAB];        // 2^(j / 512)
+    double tab[SA_TAB];        // 2^(j / 512 + shift)
+    double part2[48];          // its factors 2^(i / 16 + shift), 2^(i / 512)
     u64 part[SA_WARPS + 1];
     u64 sums[SA_MAX_CTAS];     // each CTA's weight
-    float high[SA_MAX_CTAS], low[SA_MAX_CTAS];
+    u64 slices[SA_MAX_CTAS][SA_MAX_CTAS];   // [CTA][slice of the bins]: count or weight
+    alignas(16) float high[SA_MAX_CTAS];
+    alignas(16) float low[SA_MAX_CTAS];
     int first[SA_MAX_CTAS];
+    alignas(16) uint32_t tops[SA_TOPS];   // maxima of the row's groups, in order-preserving bits
     float red[2 * SA_WARPS];
-    int count, found;
-    SaCtl ctl;
+    uint32_t top;              // the top_k-th of them
+    int count, place, taken;   // taken (first CTA): places of the list given away
+    int bin;                   // crossing
+    u64 above, cut;
     u64 bar;
-    union {
-        struct { uint32_t count[SA_BINS], limb[3][SA_BINS]; } h;   // weights in 16-bit limbs
-        struct { u64 rank[SA_LIST], w[SA_LIST]; } l;
+    u64 rank[SA_LIST];         // candidates; in the first CTA those of the cluster
+    union alignas(16) {
+        uint32_t hist[SA_WORDS];
+        u64 w[SA_LIST];
     };
 };
 
 // w(v) * 2^shift in double, not yet rounded to an integer.  With t = 512 (v -
 // max) log2(e) / T = j + f, |f| <= 1/2: 2^(t/512) = 2^(j div 512) tab[j mod
 // 512] e^(f ln 2 / 512), the last as its Taylor sum to the third power
-// (0.00068^4 / 24 = 2^-46.7 of it is left out).  0 for v below `floor`, where
-// it is less than 2^-(shift + 2), and for NaN.
+// (0.00068^4 / 24 = 2^-46.7 of it is left out).  Nothing (2^-1000) for v below
+// `floor`, where it is less than 2^-(shift + 2), for NaN and where `is` is
+// false.  Nine double operations and no branch: the double pipe is what a
+// draw without cuts is bound by.
 struct SaWeight {
     double mx, c;              // c: 512 log2(e) / T
     float floor;
-    int shift;
-    const double *tab;
-    EC_DEV double operator()(float v) const {
-        if (!(v >= floor)) return 0.0;
+    const double *tab;         // 2^(j / 512 + shift)
+    EC_DEV double operator()(float v, bool is = true) const {
         const double magic = 6755399441055744.0;      // 1.5 * 2^52
-        const double d = (double)v - mx;
+        const double d = (double)fmaxf(v, floor) - mx;
         const double kd = __fma_rn(d, c, magic);
         const int j = __double2loint(kd);
         const double f = __fma_rn(d, c, magic - kd);
-        double p = __fma_rn(f, 4.1353783506767136e-10, 9.163913992275265e-7);   // (ln2 / 512)^n / n!
+        double p = __fma_rn(f, 4.1353783506767136e-10, 9.163913992275265e-07);   // (ln2 / 512)^n / n!
         p = __fma_rn(f, p, 1.3538030870311431e-3);
         p = __fma_rn(f, p, 1.0);
         const double s = p * tab[j & (SA_TAB - 1)];
-        return __hiloint2double(__double2hiint(s) + (((j >> 9) + shift) << 20), __double2loint(s));
+        const int e = is && v >= floor ? (j & ~(SA_TAB - 1)) << 11 : -(1000 << 20);
+        return __hiloint2double(__double2hiint(s) + e, __double2loint(s));
     }
     // A weight (below 2^52) rounded to nearest, plus RAW: sums of these wrap
     // and are put right by the number of terms.
@@ -101,6 +106,9 @@ struct SaWeight {
     static EC_DEV u64 raw(double w) { return (u64)__double_as_longlong(w + 4503599627370496.0); }
     static EC_DEV u64 whole(double w) { return raw(w) - RAW; }
 };
+
+static_assert(offsetof(SaShared, tops) % 16 == 0 && offsetof(SaShared, high) % 16 == 0 && offsetof(SaShared, low) % 16 == 0 && offsetof(SaShared, hist) % 16 == 0 && offsetof(SaShared, bar) % 8 == 0 &&
+              alignof(SaShared) <= 128, "vector accesses");
 
 EC_DEV u64 sa_warp_sum(u64 v) {
 #pragma unroll
@@ -130,19 +138,69 @@ EC_DEV u64 sa_scan(u64 v, SaShared &s, u64 &total) {
     return before + sum - v;
 }
 
-// Sort list[0, n) (n a power of two), largest first.
-EC_DEV void sa_sort(u64 *list, int n) {
-    for (int k = 2; k <= n; k <<= 1)
+// Sort list[0, n), largest first; n a power of two of at most PER * SA_THREADS.
+// A thread holds PER neighbours: pairs up to 32 * PER apart are exchanged in
+// registers, only the others (10 of 66 steps for 2048) through shared memory.
+template <int PER> EC_DEV void sa_sort_per(u64 *list, int n) {
+    const int tid = threadIdx.x;
+    const bool in = tid * PER < n;
+    u64 v[PER];
+    __syncthreads();
+#pragma unroll
+    for (int q = 0; q < PER; ++q) v[q] = in && tid * PER + q < n ? list[tid * PER + q] : 0ull;
+    for (int k = 2; k <= n; k <<= 1) {
         for (int j = k >> 1; j > 0; j >>= 1) {
-            __syncthreads();
-            for (int p = threadIdx.x; p < n / 2; p += SA_THREADS) {
-                const int i = 2 * p - (p & (j - 1)), o = i + j;
-                const u64 a = list[i], b = list[o];
-                if ((a < b) == ((i & k) == 0)) { list[i] = b; list[o] = a; }
+            if (j >= 32 * PER) {
+                __syncthreads();
+                if (in)
+#pragma unroll
+                    for (int q = 0; q < PER; ++q) list[tid * PER + q] = v[q];
+                __syncthreads();
+                if (in)
+#pragma unroll
+                    for (int q = 0; q < PER; ++q) {
+                        const int i = tid * PER + q;
+                        const u64 o = list[i ^ j];
+                        const bool larger = ((i & j) == 0) == ((i & k) == 0);
+                        v[q] = (v[q] < o) == larger ? o : v[q];
+                    }
+            } else if (j >= PER) {
+#pragma unroll
+                for (int q = 0; q < PER; ++q) {
+                    const int i = tid * PER + q;
+                    const u64 o = __shfl_xor_sync(0xffffffffu, v[q], j / PER);
+                    const bool larger = ((i & j) == 0) == ((i & k) == 0);
+                    v[q] = (v[q] < o) == larger ? o : v[q];
+                }
+            } else {
+#pragma unroll
+                for (int d = PER / 2; d > 0; d >>= 1)
+                    if (j == d)
+#pragma unroll
+                        for (int q = 0; q < PER; ++q)
+                            if ((q & d) == 0) {
+                                const bool down = ((tid * PER + q) & k) == 0;
+                                const u64 x = v[q], y = v[q + d];
+                                const bool swap = (x < y) == down;
+                                v[q] = swap ? y : x;
+                                v[q + d] = swap ? x : y;
+                            }
             }
         }
+    }
+    __syncthreads();
+    if (in)
+#pragma unroll
+        for (int q = 0; q < PER; ++q)
+            if (tid * PER + q < n) list[tid * PER + q] = v[q];
     __syncthreads();
 }
+
+__noinline__ __device__ void sa_sort(u64 *list, int n) {   // one copy: cold code costs more than the call
+    if (n <= SA_THREADS) sa_sort_per<1>(list, n);
+    else sa_sort_per<2>(list, n);
+}
+static_assert(SA_LIST <= 2 * SA_THREADS, "sa_sort");
 
 EC_DEV int sa_pow2(int n) { return n <= 1 ? 1 : 1 << (32 - __clz(n - 1)); }
 
@@ -155,14 +213,18 @@ template <int T> struct SaRow {
     const uint4 *blocks;
     int n, ibase;              // blocks; index in the row of place 0
     SaWeight weight;
-    float mx, per_bin;
+    float mx, reach, per_bin;  // 1 / range of a histogram, bins per unit
     float cut_v;               // kept: larger, or equal and up to index cut_i
     int cut_i;
     bool cut;
 
     EC_DEV float at(int place) const { return sa_value<T>(reinterpret_cast<const V *>(blocks)[place]); }
     EC_DEV bool kept(float v, int place) const { return v > cut_v || (v == cut_v && place + ibase <= cut_i); }
-    EC_DEV int bin(float v) const { return min((int)(fminf(mx - v, FLT_MAX) * per_bin), SA_BINS - 1); }   // of v >= weight.floor
+    // Bin of v >= weight.floor: (max - v) in bins rounded to nearest, by the low
+    // bits of a sum with 2^23.
+    EC_DEV int bin(float v, int bins) const {
+        return (int)min(__float_as_uint(fmaf(mx - v, per_bin, 8388608.0f)) - 0x4b000000u, (uint32_t)(bins - 1));
+    }
 
     // f(value, place) for blocks [b0, b1), taken by threads t of `threads`
     template <typename F> EC_DEV void each(int b0, int b1, int t, int threads, F f) const {
@@ -180,18 +242,15 @@ template <int T> struct SaRow {
             }
         }
     }
-    // Raw weights (SaWeight::raw) of what is kept and weighs at least `least`,
-    // summed; `terms` counts them.
+    // Sum of the weights of what is kept and weighs at least `least`.
     template <bool CUT, bool LEAST> EC_DEV u64 sum(int b0, int b1, int t, int threads, double least) const {
         u64 raw = 0;
-        int terms = 0;
         each(b0, b1, t, threads, [&](float v, int p) {
-            if (CUT && !kept(v, p)) return;
-            const double w = weight(v);
-            if (LEAST && !(w >= least)) return;
-            raw += SaWeight::raw(w);
-            ++terms;
+            const double w = weight(v, !CUT || kept(v, p));
+            const u64 x = SaWeight::raw(w);
+            raw += LEAST && !(w >= least) ? SaWeight::RAW : x;
         });
+        const int terms = b1 - b0 > t ? ((b1 - b0 - t - 1) / threads + 1) * PER : 0;
         return raw - (u64)terms * SaWeight::RAW;
     }
     EC_DEV u64 sum(int b0, int b1, int t, int threads, double least) const {
@@ -200,154 +259,190 @@ template <int T> struct SaRow {
     }
 };
 
-// Finds the candidate at which the running count (MASS: weight, among those
-// kept so far) over the order reaches what is wanted, and cuts there.  With
-// `whole`, everything up to it may be left unsorted in the first CTA's list
-// instead, each CTA's number in its `first`; returns true then.  All CTAs of
-// the cluster call it alike.
-template <bool MASS, int T>
-EC_DEV bool sa_select(cg::cluster_group &cl, SaRow<T> &row, u64 want, float top_p, bool whole) {
+// The candidates that `in` lets through, gathered in the first CTA's list (in
+// any order); true when they fit.  The first CTA's `taken` was 0 when the
+// cluster last met.  All CTAs of the cluster call it alike; it ends with the
+// cluster meeting.
+template <int T, typename F> EC_DEV bool sa_gather(cg::cluster_group &cl, const SaRow<T> &row, F in) {
     SaShared &s = row.s;
+    const int me = (int)cl.block_rank(), tid = threadIdx.x;
+    // the first CTA writes into the list at once, the others by way of their own
+    int *counter = me == 0 ? &s.taken : &s.count;
+    __syncthreads();
+    if (tid == 0) s.count = 0;
+    __syncthreads();
+    row.each(0, row.n, tid, SA_THREADS, [&](float v, int p) {
+        if (in(v, p)) {
+            const int at = atomicAdd(counter, 1);
+            if (at < SA_LIST) s.rank[at] = sa_rank(v, p + row.ibase);
+        }
+    });
+    if (me != 0) {
+        __syncthreads();
+        if (tid == 0) s.place = s.count ? atomicAdd(&cl.map_shared_rank(&s, 0)->taken, s.count) : 0;
+        __syncthreads();
+        u64 *list = cl.map_shared_rank(s.rank, 0);
+        for (int i = tid; i < min(s.count, SA_LIST); i += SA_THREADS)
+            if (s.place + i < SA_LIST) list[s.place + i] = s.rank[i];
+    }
+    cl.sync();
+    return cl.map_shared_rank(&s, 0)->taken <= SA_LIST;
+}
+
+// Finds the candidate at which the running count (MASS: weight, among those
+// kept so far) over the order reaches what is wanted, and cuts there.  All
+// CTAs of the cluster call it alike.
+template <bool MASS, int T>
+EC_DEV void sa_select(cg::cluster_group &cl, SaRow<T> &row, u64 want, float top_p) {
+    SaShared &s = row.s;
+    constexpr int BINS = MASS ? SA_WORDS / 2 : SA_WORDS, EACH = BINS / SA_THREADS;   // weights: low words, then high words
     const int ctas = (int)cl.num_blocks(), me = (int)cl.block_rank(), tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int slice = BINS / ctas;
     u64 above = 0, prefix = 0;
     int bits = 64, bin = -1;   // from the second round: candidates of `bin` whose rank's top 64 - bits bits are `prefix`
+    constexpr int STEP = MASS ? 11 : 12;
     const float floor = row.weight.floor;
+    row.per_bin = row.reach * BINS;
     auto in_class = [&](float v, int p) {
-        if (!(v >= floor) || row.bin(v) != bin || (MASS && row.cut && !row.kept(v, p))) return false;
+        if (!(v >= floor) || row.bin(v, BINS) != bin || (MASS && row.cut && !row.kept(v, p))) return false;
         return bits == 64 || (sa_rank(v, p + row.ibase) >> bits) == prefix;
     };
+    auto sum_of = [&](const uint32_t *h, int b) { return MASS ? (u64)h[b] + ((u64)h[BINS + b] << 32) : (u64)h[b]; };
     for (;;) {
         __syncthreads();
-        for (int b = tid; b < SA_BINS; b += SA_THREADS) s.h.count[b] = s.h.limb[0][b] = s.h.limb[1][b] = s.h.limb[2][b] = 0;
-        if (tid == 0) s.count = 0;
+        for (int b = tid; b < SA_WORDS / 4; b += SA_THREADS) reinterpret_cast<uint4 *>(s.hist)[b] = make_uint4(0u, 0u, 0u, 0u);
+        if (tid == 0) s.taken = 0;
         __syncthreads();
-        const int step = bits - 10 > 0 ? bits - 10 : 0;
+        const int step = bits - STEP > 0 ? bits - STEP : 0;
         auto add = [&](float v, int b) {
-            atomicAdd(&s.h.count[b], 1u);
-            if (MASS) {
+            if (!MASS) {
+                atomicAdd(&s.hist[b], 1u);
+            } else {
                 const u64 w = SaWeight::whole(row.weight(v));
-                if (w & 0xffff) atomicAdd(&s.h.limb[0][b], (uint32_t)(w & 0xffff));
-                if (w >> 16 & 0xffff) atomicAdd(&s.h.limb[1][b], (uint32_t)(w >> 16 & 0xffff));
-                if (w >> 32) atomicAdd(&s.h.limb[2][b], (uint32_t)(w >> 32));
+                const uint32_t lo = (uint32_t)w, old = atomicAdd(&s.hist[b], lo);
+                const uint32_t hi = (uint32_t)(w >> 32) + (old + lo < lo);   // with the carry of the low word
+                if (hi) atomicAdd(&s.hist[BINS + b], hi);
             }
         };
         if (bin < 0)
             row.each(0, row.n, tid, SA_THREADS, [&](float v, int p) {
-                if (v >= floor && (!MASS || !row.cut || row.kept(v, p))) add(v, row.bin(v));
+                if (v >= floor && (!MASS || !row.cut || row.kept(v, p))) add(v, row.bin(v, BINS));
             });
         else
             row.each(0, row.n, tid, SA_THREADS, [&](float v, int p) {
-                if (in_class(v, p)) add(v, SA_BINS - 1 - (int)((sa_rank(v, p + row.ibase) >> step) & (SA_BINS - 1)));
+                if (in_class(v, p)) add(v, BINS - 1 - (int)((sa_rank(v, p + row.ibase) >> step) & (BINS - 1)));
             });
+        __syncthreads();
+        // Every CTA tells the others its sum of each slice of the bins, so that
+        // all know the slice of the crossing and join its bins themselves.
+        for (int sl = warp; sl < ctas; sl += SA_WARPS) {
+            u64 t = 0;
+            for (int b = lane; b < slice; b += 32) t += sum_of(s.hist, sl * slice + b);
+            t = sa_warp_sum(t);
+            if (lane < ctas) cl.map_shared_rank(&s, lane)->slices[me][sl] = t;
+        }
         cl.sync();
-        if (me == 0) {   // join the histograms, find the crossing
-            u64 cnt[2] = {0, 0}, sum[2] = {0, 0};
-            for (int c = 0; c < ctas; ++c) {
-                const SaShared *o = cl.map_shared_rank(&s, c);
-                const uint2 q = reinterpret_cast<const uint2 *>(o->h.count)[tid];
-                cnt[0] += q.x;
-                cnt[1] += q.y;
-                if (MASS)
+        u64 mine = 0, total = above;
+        for (int c = 0; c < ctas; ++c) mine += lane < ctas ? s.slices[c][lane] : 0ull;
+        int at = ctas;
+        u64 before = above;
+        if (MASS && bin < 0) {
+            const u64 all = sa_warp_sum(mine);
+            want = max(1ull, min(all, (u64)ceil((double)top_p * (double)all)));
+        }
+        for (int c = 0; c < ctas; ++c) {
+            const u64 t = __shfl_sync(0xffffffffu, mine, c);
+            if (at == ctas && total + t >= want) { at = c; before = total; }
+            total += t;
+        }
+        if (at == ctas) {   // fewer than wanted have any weight: nothing to cut
+            cl.sync();      // `slices` is read
+            return;
+        }
+        // a thread's bins of that slice, from all CTAs at once
+        u64 sum[EACH] = {};
+        mine = 0;
+        const int each = (slice + SA_THREADS - 1) / SA_THREADS;
 #pragma unroll
-                    for (int l = 0; l < 3; ++l) {
-                        const uint2 m = reinterpret_cast<const uint2 *>(o->h.limb[l])[tid];
-                        sum[0] += (u64)m.x << (16 * l);
-                        sum[1] += (u64)m.y << (16 * l);
+        for (int q = 0; q < EACH; ++q)
+            if (q < each && tid * each + q < slice) {
+                const int b = at * slice + tid * each + q;
+                if (ctas > 4) {
+                    uint32_t lo[SA_MAX_CTAS], hi[SA_MAX_CTAS];
+#pragma unroll
+                    for (int c = 0; c < SA_MAX_CTAS; ++c) {
+                        lo[c] = c < ctas ? *cl.map_shared_rank(s.hist + b, c) : 0u;
+                        hi[c] = MASS && c < ctas ? *cl.map_shared_rank(s.hist + BINS + b, c) : 0u;
                     }
-            }
-            if (!MASS) { sum[0] = cnt[0]; sum[1] = cnt[1]; }
-            u64 total;
-            u64 before = above + sa_scan(sum[0] + sum[1], s, total);
-            if (MASS && bin < 0) want = max(1ull, min(total, (u64)ceil((double)top_p * (double)total)));
-            if (tid == 0) s.ctl.bin = -1;
-            __syncthreads();
 #pragma unroll
-            for (int q = 0; q < 2; ++q) {
-                if (before < want && before + sum[q] >= want) {
-                    s.ctl.bin = 2 * tid + q;
-                    s.ctl.crowd = (int)cnt[q];
-                    s.ctl.above = before;
-                    s.ctl.want = want;
+                    for (int c = 0; c < SA_MAX_CTAS; ++c) sum[q] += (u64)lo[c] + ((u64)hi[c] << 32);
+                } else {
+                    for (int c = 0; c < ctas; ++c) sum[q] += sum_of(cl.map_shared_rank(s.hist, c), b);
                 }
-                before += sum[q];
+                mine += sum[q];
             }
-            __syncthreads();
-            // all up to the crossing, where they fit the list and it is asked for
-            const bool all = whole && bin < 0 && s.ctl.bin >= 0 && s.ctl.above + s.ctl.crowd <= SA_LIST;
-            if (warp == 0) {
-                int c = 0;
-                if (lane < ctas && s.ctl.bin >= 0 && !all) c = (int)cl.map_shared_rank(&s, lane)->h.count[s.ctl.bin];
-                int sum32 = c;
+        before += sa_scan(mine, s, total);
 #pragma unroll
-                for (int o = 1; o < 32; o <<= 1) {
-                    const int u = __shfl_up_sync(0xffffffffu, sum32, o);
-                    if (lane >= o) sum32 += u;
-                }
-                if (lane < ctas) s.ctl.at[lane] = all ? -1 : sum32 - c;
+        for (int q = 0; q < EACH; ++q) {
+            if (sum[q] && before < want && before + sum[q] >= want) {
+                s.bin = at * slice + tid * each + q;
+                s.above = before;
             }
-            __syncthreads();
-            if (tid < ctas) cl.map_shared_rank(&s, tid)->ctl = s.ctl;
+            before += sum[q];
         }
-        cl.sync();
-        const int crossing = s.ctl.bin, crowd = s.ctl.crowd, place = s.ctl.at[me];
-        if (crossing < 0) return false;   // fewer than wanted have any weight: nothing to cut
-        want = s.ctl.want;
-        above = s.ctl.above;
-        u64 *list = cl.map_shared_rank(&s, 0)->l.rank;
-        if (place < 0) {                  // everything up to the crossing goes to the list
-            int c = 0;
-            for (int b = tid; b <= crossing; b += SA_THREADS) c += (int)s.h.count[b];
-            u64 total;
-            sa_scan((u64)c, s, total);
-            if (tid == 0) cl.map_shared_rank(&s, 0)->first[me] = (int)total;
-            cl.sync();
-            int at = 0;
-            for (int q = 0; q < me; ++q) at += cl.map_shared_rank(&s, 0)->first[q];
-            row.each(0, row.n, tid, SA_THREADS, [&](float v, int p) {
-                if (v >= floor && row.bin(v) <= crossing) list[at + atomicAdd(&s.count, 1)] = sa_rank(v, p + row.ibase);
-            });
-            cl.sync();
-            return true;
-        }
+        __syncthreads();
+        above = s.above;
         if (bin < 0) {
-            bin = crossing;
+            bin = s.bin;
         } else {
-            prefix = prefix << (bits - step) | ((u64)(SA_BINS - 1 - crossing) & ((1ull << (bits - step)) - 1));
+            prefix = prefix << (bits - step) | ((u64)(BINS - 1 - s.bin) & ((1ull << (bits - step)) - 1));
             bits = step;
         }
-        if (crowd > SA_LIST) continue;
-        row.each(0, row.n, tid, SA_THREADS, [&](float v, int p) {
-            if (in_class(v, p)) list[place + atomicAdd(&s.count, 1)] = sa_rank(v, p + row.ibase);
-        });
-        cl.sync();
-        if (me == 0) {
-            const int size = sa_pow2(crowd);
-            for (int i = tid; i < size; i += SA_THREADS)
-                if (i >= crowd) s.l.rank[i] = 0;
-            sa_sort(s.l.rank, size);
+        if (sa_gather(cl, row, in_class)) break;
+        cl.sync();          // `taken` is read
+    }
+    if (me == 0) {
+        const int n = s.taken;
+        if (n <= SA_FEW) {   // the weight before a candidate: a loop over the others, shared out over 512 / n threads
+            const int group = n <= 32 ? 16 : n <= 64 ? 8 : n <= 128 ? 4 : 2, i = tid / group;
+            for (int j = tid; j < n; j += SA_THREADS) s.w[j] = MASS ? SaWeight::whole(row.weight(sa_rank_value(s.rank[j]))) : 1ull;
+            __syncthreads();
+            const u64 r = i < n ? s.rank[i] : 0ull;
+            u64 before = 0;
+            for (int j = tid % group; j < n; j += group) before += s.rank[j] > r ? s.w[j] : 0ull;
+            for (int o = 1; o < group; o <<= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
+            before += above;
+            if (i < n && before < want && before + s.w[i] >= want) s.cut = r;
+        } else {
+            const int size = sa_pow2(n);
+            for (int i = n + tid; i < size; i += SA_THREADS) s.rank[i] = 0;
+            sa_sort(s.rank, size);
             u64 w[SA_PER], sum = 0, total;
 #pragma unroll
             for (int j = 0; j < SA_PER; ++j) {
                 const int i = tid * SA_PER + j;
-                w[j] = i >= crowd ? 0ull : MASS ? SaWeight::whole(row.weight(sa_rank_value(s.l.rank[i]))) : 1ull;
+                w[j] = i >= n ? 0ull : MASS ? SaWeight::whole(row.weight(sa_rank_value(s.rank[i]))) : 1ull;
                 sum += w[j];
             }
             u64 before = above + sa_scan(sum, s, total);
 #pragma unroll
             for (int j = 0; j < SA_PER; ++j) {
-                if (before < want && before + w[j] >= want) s.ctl.cut = s.l.rank[tid * SA_PER + j];
+                if (before < want && before + w[j] >= want) s.cut = s.rank[tid * SA_PER + j];
                 before += w[j];
             }
-            __syncthreads();
-            if (tid < ctas) cl.map_shared_rank(&s, tid)->ctl.cut = s.ctl.cut;
         }
-        cl.sync();
-        row.cut = true;
-        row.cut_v = sa_rank_value(s.ctl.cut);
-        row.cut_i = sa_rank_index(s.ctl.cut);
-        return false;
+        __syncthreads();
+        if (tid < ctas) cl.map_shared_rank(&s, tid)->cut = s.cut;
     }
+    cl.sync();
+    row.cut = true;
+    row.cut_v = sa_rank_value(s.cut);
+    row.cut_i = sa_rank_index(s.cut);
 }
+
+// The other half of the arrival at the kernel's start: no CTA of the cluster
+// is still to come.
+EC_DEV void sa_cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 
 // The point u of a sum of whole weights: the running sum has to exceed it.
 EC_DEV u64 sa_point(float u, u64 total) {
@@ -360,16 +455,61 @@ EC_DEV u64 sa_point(float u, u64 total) {
 template <int T>
 EC_DEV void sa_draw_list(const ec_sample_args &a, SaRow<T> &row, int r, int size, int top_k, float top_p, double least) {
     SaShared &s = row.s;
-    const int tid = threadIdx.x, full = sa_pow2(size);
+    const int tid = threadIdx.x;
+    if (size <= SA_FEW) {   // by counting, as in sa_select
+        const int group = size <= 32 ? 16 : size <= 64 ? 8 : size <= 128 ? 4 : 2, i = tid / group;
+        if (tid == 0) s.above = 0;
+        __syncthreads();
+        for (int j = tid; j < size; j += SA_THREADS) s.w[j] = SaWeight::whole(row.weight(sa_rank_value(s.rank[j])));
+        __syncthreads();
+        const u64 mine = i < size ? s.rank[i] : 0ull;
+        int place = 0;
+        u64 before = 0;
+        for (int j = tid % group; j < size; j += group)
+            if (s.rank[j] > mine) {
+                ++place;
+                before += s.w[j];
+            }
+        for (int o = 1; o < group; o <<= 1) {
+            place += __shfl_xor_sync(0xffffffffu, place, o);
+            before += __shfl_xor_sync(0xffffffffu, before, o);
+        }
+        if (i < size && place == min(top_k, size) - 1) s.above = before + s.w[i];   // the sum over the first top_k
+        __syncthreads();
+        const u64 total = s.above, want = top_p < 1.0f ? max(1ull, min(total, (u64)ceil((double)top_p * (double)total))) : total;
+        const double w = i < size ? row.weight(sa_rank_value(mine)) : 0.0;
+        const bool keep = i < size && place < top_k && before < want && (w >= least || place == 0);
+        __syncthreads();
+        if (!keep && i < size && tid % group == 0) s.w[i] = 0;
+        __syncthreads();
+        u64 kept = 0;
+        before = 0;
+        for (int j = tid % group; j < size; j += group) {
+            const u64 x = s.w[j];
+            kept += x;
+            before += (uint32_t)s.rank[j] > (uint32_t)mine ? x : 0ull;   // a lower index
+        }
+        for (int o = 1; o < group; o <<= 1) {
+            kept += __shfl_xor_sync(0xffffffffu, kept, o);
+            before += __shfl_xor_sync(0xffffffffu, before, o);
+        }
+        const u64 target = sa_point(a.u[r], kept);
+        if (keep && tid % group == 0 && before <= target && target < before + s.w[i]) {
+            a.ids[r] = sa_rank_index(mine);
+            if (a.prob) a.prob[r] = (float)(w / (double)kept);
+        }
+        return;
+    }
+    const int full = sa_pow2(size);
     for (int i = tid; i < full; i += SA_THREADS)
-        if (i >= size) s.l.rank[i] = 0;
-    sa_sort(s.l.rank, full);
+        if (i >= size) s.rank[i] = 0;
+    sa_sort(s.rank, full);
     u64 w[SA_PER], sum = 0, total;
     double wd[SA_PER];
 #pragma unroll
     for (int j = 0; j < SA_PER; ++j) {
         const int i = tid * SA_PER + j;
-        wd[j] = i < top_k && i < size ? row.weight(sa_rank_value(s.l.rank[i])) : 0.0;
+        wd[j] = i < top_k && i < size ? row.weight(sa_rank_value(s.rank[i])) : 0.0;
         w[j] = SaWeight::whole(wd[j]);
         sum += w[j];
     }
@@ -382,19 +522,19 @@ EC_DEV void sa_draw_list(const ec_sample_args &a, SaRow<T> &row, int r, int size
         const bool keep = w[j] > 0 && before < want && (wd[j] >= least || i == 0);
         before += w[j];
         kept += keep ? w[j] : 0ull;
-        s.l.w[i] = (u64)__double_as_longlong(wd[j]);
-        s.l.rank[i] = keep ? (u64)(uint32_t)~sa_rank_index(s.l.rank[i]) << 32 | (uint32_t)i : 0ull;   // lowest index largest
+        s.w[i] = (u64)__double_as_longlong(wd[j]);
+        s.rank[i] = keep ? (u64)(uint32_t)~sa_rank_index(s.rank[i]) << 32 | (uint32_t)i : 0ull;   // lowest index largest
     }
     sa_scan(kept, s, total);
     const int most = sa_pow2(min(size, top_k));
-    sa_sort(s.l.rank, most);
+    sa_sort(s.rank, most);
     const u64 target = sa_point(a.u[r], total);
     sum = 0;
 #pragma unroll
     for (int j = 0; j < SA_PER; ++j) {
         const int i = tid * SA_PER + j;
-        const u64 k = i < most ? s.l.rank[i] : 0ull;
-        wd[j] = k ? __longlong_as_double((long long)s.l.w[(uint32_t)k]) : 0.0;
+        const u64 k = i < most ? s.rank[i] : 0ull;
+        wd[j] = k ? __longlong_as_double((long long)s.w[(uint32_t)k]) : 0.0;
         w[j] = SaWeight::whole(wd[j]);
         sum += w[j];
     }
@@ -403,7 +543,7 @@ EC_DEV void sa_draw_list(const ec_sample_args &a, SaRow<T> &row, int r, int size
 #pragma unroll
     for (int j = 0; j < SA_PER; ++j) {
         if (before <= target && target < before + w[j]) {
-            a.ids[r] = (int)~(uint32_t)(s.l.rank[tid * SA_PER + j] >> 32);
+            a.ids[r] = (int)~(uint32_t)(s.rank[tid * SA_PER + j] >> 32);
             if (a.prob) a.prob[r] = (float)(wd[j] / (double)total);
         }
         before += w[j];
@@ -414,18 +554,28 @@ EC_DEV void sa_draw_list(const ec_sample_args &a, SaRow<T> &row, int r, int size
 // memory, so that the logits are read from HBM once.
 template <int T>
 __global__ void __launch_bounds__(SA_THREADS, 2) k_sample(const ec_sample_args a, int shift, int share, int *err) {
-    EC_PDL_ENTER();
     typedef SaRow<T> Row;
     typedef typename Row::V V;
     constexpr int ELT = Row::ELT, PER = Row::PER;
     extern __shared__ __align__(128) unsigned char smem[];
     SaShared &s = *reinterpret_cast<SaShared *>(smem);
+    if (threadIdx.x < SA_MAX_CTAS) {
+        s.high[threadIdx.x] = -INFINITY;
+        s.low[threadIdx.x] = INFINITY;
+    }
+    // this CTA has started, and what others write first is set (sa_cluster_wait)
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    EC_PDL_ENTER();
     V *vals = reinterpret_cast<V *>(smem + (sizeof(SaShared) + 127) / 128 * 128);
     cg::cluster_group cl = cg::this_cluster();
     const int ctas = (int)cl.num_blocks(), me = (int)cl.block_rank();
     const int r = (int)blockIdx.x / ctas, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const float temperature = a.temperature ? a.temperature[r] : 1.0f, min_p = a.min_p ? a.min_p[r] : 0.0f, top_p = a.top_p ? a.top_p[r] : 1.0f;
     const int top_k = a.top_k ? a.top_k[r] : 0;
+
+    // Below `vanish` from the largest a weight is 0: only what lies above is
+    // ever a candidate.
+    const double vanish = (double)temperature * 0.6931471805599453 * (shift + 3), per_nat = 512.0 * 1.4426950408889634 / (double)temperature;
 
     // Shares are cut at 16-byte blocks of memory: element i of the row is
     // element i + skew of the block that holds its first one.
@@ -454,8 +604,10 @@ __global__ void __launch_bounds__(SA_THREADS, 2) k_sample(const ec_sample_args a
             }
             vals[e] = e >= off && e < off + n ? src[i0 + e - off] : (V)(T == EC_T_F32 ? -INFINITY : T == EC_T_F16 ? 0xfc00 : 0xff80);
         }
-        for (int j = tid; j < SA_TAB; j += SA_THREADS) s.tab[j] = exp2((double)j / SA_TAB);
+        if (tid == 0) { s.taken = 0; s.top = 0xffffffffu; }
+        if (tid < 48) s.part2[tid] = exp2(tid < 16 ? (double)tid / 16 + shift : (double)(tid - 16) / SA_TAB);
         __syncthreads();
+        for (int j = tid; j < SA_TAB; j += SA_THREADS) s.tab[j] = s.part2[j / 32] * s.part2[16 + j % 32];
         if (bulk) ec_mbar_wait(bar, 0, err);   // a wait that gave up is reported; the row's result is then void
     }
     Row row = {s, reinterpret_cast<const uint4 *>(vals), blocks, i0 - off};
@@ -470,22 +622,46 @@ __global__ void __launch_bounds__(SA_THREADS, 2) k_sample(const ec_sample_args a
         });
     else
         row.each(0, blocks, tid, SA_THREADS, [&](float v, int) { mx = fmaxf(mx, v); });
+    // the few candidates of a small top-k are found by the maxima of SA_TOPS
+    // groups of threads, `group` lanes each
+    const bool fast = top_k > 1 && top_k <= SA_FAST && top_k < a.vocab;
+    const int group = SA_THREADS * ctas / SA_TOPS;
+    float group_mx = -INFINITY;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
+    for (int o = 1; o < 32; o <<= 1) {
+        if (o == group) group_mx = mx;
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
         mn = fminf(mn, __shfl_xor_sync(0xffffffffu, mn, o));
     }
+    if (group == 32) group_mx = mx;
     if (lane == 0) { s.red[warp] = mx; s.red[SA_WARPS + warp] = mn; }
     __syncthreads();
-    for (int w = 0; w < SA_WARPS; ++w) { mx = fmaxf(mx, s.red[w]); mn = fminf(mn, s.red[SA_WARPS + w]); }
-    cl.sync();   // every CTA of the cluster has started: its shared memory may be written
+    if (warp == 0) {
+        mx = s.red[lane % SA_WARPS];
+        mn = s.red[SA_WARPS + lane % SA_WARPS];
+#pragma unroll
+        for (int o = SA_WARPS / 2; o > 0; o >>= 1) {
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+            mn = fminf(mn, __shfl_xor_sync(0xffffffffu, mn, o));
+        }
+    }
+    sa_cluster_wait();   // every CTA of the cluster has started: its shared memory may be written
     if (tid < ctas) {
         SaShared *o = cl.map_shared_rank(&s, tid);
         o->high[me] = mx;
         o->low[me] = mn;
     }
+    if (fast)
+        for (int c = lane % group; c < ctas; c += group) cl.map_shared_rank(&s, c)->tops[(me * SA_THREADS + tid) / group] = sa_bits(group_mx);
     cl.sync();
-    for (int c = 0; c < ctas; ++c) { mx = fmaxf(mx, s.high[c]); mn = fminf(mn, s.low[c]); }
+    mx = -INFINITY;
+    mn = INFINITY;
+#pragma unroll
+    for (int c = 0; c < SA_MAX_CTAS / 4; ++c) {
+        const float4 h = reinterpret_cast<const float4 *>(s.high)[c], l = reinterpret_cast<const float4 *>(s.low)[c];
+        mx = fmaxf(fmaxf(fmaxf(mx, h.x), fmaxf(h.y, h.z)), h.w);
+        mn = fminf(fminf(fminf(mn, l.x), fminf(l.y, l.z)), l.w);
+    }
 
     if (mx == -INFINITY) {
         if (me == 0 && tid == 0) {
@@ -514,32 +690,52 @@ __global__ void __launch_bounds__(SA_THREADS, 2) k_sample(const ec_sample_args a
         }
         return;
     }
-    if (mx == INFINITY) {   // logits of +inf weigh the same, all others nothing
+    const bool infinite = mx == INFINITY;
+    if (infinite) {   // logits of +inf weigh the same, all others nothing
         for (int e = tid; e < blocks * PER; e += SA_THREADS)
             vals[e] = sa_value<T>(vals[e]) == INFINITY ? (V)0 : (V)(T == EC_T_F32 ? -INFINITY : T == EC_T_F16 ? 0xfc00 : 0xff80);
         __syncthreads();
         mx = mn = 0.0f;
     }
-    // Below `vanish` from the largest a weight is 0: only what lies above is
-    // ever a candidate.  (floor is the smallest float from there on.)
-    const double vanish = (double)temperature * 0.6931471805599453 * (shift + 3);
+    // floor: the smallest float that is not below
     const float floor = fmaxf(__double2float_ru((double)mx - vanish), -FLT_MAX);
-    row.weight = {(double)mx, 512.0 * 1.4426950408889634 / (double)temperature, floor, shift, s.tab};
+    row.weight = {(double)mx, per_nat, floor, s.tab};
     row.mx = mx;
-    row.per_bin = (float)SA_BINS / fmaxf(fminf(mx - floor, mx - mn), 1e-30f);
+    row.reach = 1.0f / fmaxf(fminf(mx - floor, mx - mn), 1e-30f);
     row.cut_v = -INFINITY;
     row.cut_i = 0x7fffffff;
     row.cut = false;
     const double least = min_p > 0.0f ? (double)min_p * (double)(1ull << shift) : 0.0;
 
-    if (top_k > 0 && top_k < a.vocab && sa_select<false>(cl, row, (u64)top_k, top_p, top_k <= SA_LIST / 2)) {
-        if (me != 0) return;
-        int size = 0;
-        for (int c = 0; c < ctas; ++c) size += s.first[c];
-        sa_draw_list(a, row, r, size, top_k, top_p, least);
-        return;
+    if (top_k > 0 && top_k < a.vocab) {
+        bool listed = false;
+        if (fast && !infinite) {
+            // the top_k-th largest of the maxima is the smallest that fewer
+            // than top_k exceed: two threads count for a value
+            const uint32_t v = s.tops[tid / 2];
+            int larger = 0;
+#pragma unroll 4
+            for (int j = tid % 2; j < SA_TOPS / 4; j += 2) {
+                const uint4 q = reinterpret_cast<const uint4 *>(s.tops)[j];
+                larger += (q.x > v) + (q.y > v) + (q.z > v) + (q.w > v);
+            }
+            larger += __shfl_xor_sync(0xffffffffu, larger, 1);
+            const uint32_t least_top = __reduce_min_sync(0xffffffffu, larger < top_k ? v : 0xffffffffu);
+            if (lane == 0) atomicMin(&s.top, least_top);
+            __syncthreads();
+            const float top = sa_bits_value(s.top);
+            if (top > -INFINITY) listed = sa_gather(cl, row, [&](float x, int) { return x >= top; });
+        }
+        if (listed) {
+            if (me != 0) return;
+            sa_draw_list(a, row, r, s.taken, top_k, top_p, least);
+            cl.sync();   // the others have read `taken` (and left)
+            return;
+        }
+        if (fast && !infinite) cl.sync();   // `taken` is read
+        sa_select<false>(cl, row, (u64)top_k, top_p);
     }
-    if (top_p < 1.0f) sa_select<true>(cl, row, 0ull, top_p, false);
+    if (top_p < 1.0f) sa_select<true>(cl, row, 0ull, top_p);
 
     // Weights of the kept candidates in vocabulary order: of each warp's
     // contiguous piece, of the CTAs, then of the piece that holds the point.
@@ -548,12 +744,13 @@ __global__ void __launch_bounds__(SA_THREADS, 2) k_sample(const ec_sample_args a
     __syncthreads();
     if (lane == 0) s.part[warp] = part;
     __syncthreads();
-    u64 total = 0;
-    for (int w = 0; w < SA_WARPS; ++w) total += s.part[w];
-    if (tid < ctas) cl.map_shared_rank(&s, tid)->sums[me] = total;
+    if (warp == 0) {
+        u64 t = lane < SA_WARPS ? s.part[lane] : 0ull;
+        t = sa_warp_sum(t);
+        if (lane < ctas) cl.map_shared_rank(&s, lane)->sums[me] = t;
+    }
     cl.sync();
-    u64 before = 0;
-    total = 0;
+    u64 before = 0, total = 0;
     for (int c = 0; c < ctas; ++c) {
         if (c == me) before = total;
         total += s.sums[c];
@@ -566,7 +763,7 @@ __global__ void __launch_bounds__(SA_THREADS, 2) k_sample(const ec_sample_args a
     for (int p0 = w * piece * PER; p0 < end; p0 += SA_THREADS) {
         const int p = p0 + tid;
         const float v = p < end ? row.at(p) : -INFINITY;
-        const double x = !row.cut || row.kept(v, p) ? row.weight(v) : 0.0;
+        const double x = row.weight(v, !row.cut || row.kept(v, p));
         const u64 mine = x >= least ? SaWeight::whole(x) : 0ull;
         u64 all;
         const u64 start = before + sa_scan(mine, s, all);
