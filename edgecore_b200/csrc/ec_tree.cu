@@ -7,11 +7,18 @@
 // One pass over the pages with a running maximum m and sum l per row:
 //   s = scale * q.k (masked: -inf), m' = max(m, s), p = 2^((s - m') log2 e),
 //   l = l 2^((m - m') log2 e) + sum p,  o = o 2^((m - m') log2 e) + p V
-// and out = o / l (0 where nothing was seen).  Positions of a sequence can be
-// split over CTAs: each writes (m, l, o) of its pages and k_tree_join adds
-// them up in the order of the pages.
+// and out = o / l (0 where nothing was seen).  The pages are the work: small
+// calls give every row tile to the CTAs of a cluster, which join their (m, l,
+// o) through each other's shared memory; larger ones cut the pages of all
+// tiles, one after the other, into equal pieces, one per resident CTA, so that
+// ragged sequences keep every SM busy to the end, and k_tree_join adds up the
+// tiles that a border cuts, in the order of their pages.
 #include "ec_common.cuh"
 #include "ec_serve.h"
+
+#include <cooperative_groups.h>
+
+namespace cg = cooperative_groups;
 
 namespace {
 
@@ -22,69 +29,150 @@ constexpr int PAGE = EC_KV_PAGE;
 
 struct TaGeo {            // chosen by the launcher
     int group;            // query heads per KV head
-    int nsplit, chunk;    // CTAs a sequence's pages are split over at most, pages per CTA at least
-    int tiles;            // upper bound on row tiles of all sequences
+    unsigned div_mul;     // row / group = (row * div_mul) >> div_shift for rows below 2^30 (group > 1)
+    int div_shift;
+    int cluster;          // CTAs of a cluster that share a tile's pages
     float scale2;         // scale * log2 e
-    float *part;          // [tiles][n_kv_head][nsplit][MT][hdp] o, then [...][MT] (m, l)
+    float *part;          // pieces: [CTA][2][MT][hdp] o, then [CTA][2][MT] (m, l)
 };
 
-struct TaTile {           // one row tile
-    int b, first;         // sequence, its first row in the tile's (node, head) numbering
+EC_DEV int ta_node(const TaGeo &g, int row) {
+    return g.group == 1 ? row : (int)(((unsigned long long)(unsigned)row * g.div_mul) >> g.div_shift);
+}
+
+struct TaTile {           // one row tile of one KV head
+    int first;            // its first row in the sequence's (node, head) numbering
+    int kh;
     int r0, t, base, slot;
     int page0, page1;     // pages that hold visible positions
 };
 
-EC_DEV int ta_splits(const TaTile &s, const TaGeo &g, int &chunk) {
-    const int n = s.page1 - s.page0;
-    chunk = max(g.chunk, (n + g.nsplit - 1) / g.nsplit);
-    return n > 0 ? (n + chunk - 1) / chunk : 1;
+struct TaSeq {            // a sequence, in the lane that holds it
+    int r0, t, base, slot, page0, pages, tiles;   // a bad one has no tiles
+};
+
+EC_DEV TaSeq ta_seq(const ec_kv_pages &kv, const ec_tree_attn &a, const TaGeo &g, int mt, int i, int *err) {
+    TaSeq q = {};
+    if (i >= a.n_seq) return q;
+    q.r0 = a.row_start[i];
+    const long long t = (long long)a.row_start[i + 1] - q.r0;
+    q.base = a.base[i];
+    q.slot = a.slots ? a.slots[i] : i;
+    if (q.r0 < 0 || t < 0 || q.r0 + t > a.rows || q.base < 0 || q.slot < 0 || q.slot >= kv.n_slots ||
+        q.base + t > (long long)kv.pages_per_slot * PAGE) {
+        atomicCAS(err, 0, EC_KERR_BAD_INDEX);
+        return q;
+    }
+    q.t = (int)t;
+    q.tiles = (int)((t * g.group + mt - 1) / mt);
+    const int lo = a.window > 0 && q.base > a.window ? q.base - a.window : 0;   // no row sees a position below it
+    q.page0 = lo / PAGE;
+    q.pages = (q.base + q.t + PAGE - 1) / PAGE - q.page0;
+    return q;
 }
 
-// The row tile `ti` of `mt` rows in the sequences' order; false when there is
-// none, or its sequence has a bad index (recorded).  Called by whole warps.
-EC_DEV bool ta_find(const ec_kv_pages &kv, const ec_tree_attn &a, const TaGeo &g, int ti, int mt, TaTile &s, int *err) {
-    const int lane = threadIdx.x & 31;
-    int before = 0, b = -1, local = 0;
-    for (int b0 = 0; b0 < a.n_seq && b < 0; b0 += 32) {
-        const int i = b0 + lane;
-        int n = 0;
-        if (i < a.n_seq) {
-            const long long t = (long long)a.row_start[i + 1] - a.row_start[i];
-            const bool bad = t < 0 || t > a.rows;
-            if (bad) atomicCAS(err, 0, EC_KERR_BAD_INDEX);
-            n = bad ? 0 : (int)((t * g.group + mt - 1) / mt);
-        }
-        int sum = n;
+EC_DEV TaTile ta_tile(const TaSeq &q, int l, int tile, int kh, int mt) {   // from the sequence that lane l holds
+    TaTile s;
+    s.first = tile * mt;
+    s.kh = kh;
+    s.r0 = __shfl_sync(0xffffffffu, q.r0, l);
+    s.t = __shfl_sync(0xffffffffu, q.t, l);
+    s.base = __shfl_sync(0xffffffffu, q.base, l);
+    s.slot = __shfl_sync(0xffffffffu, q.slot, l);
+    s.page0 = __shfl_sync(0xffffffffu, q.page0, l);
+    s.page1 = s.page0 + __shfl_sync(0xffffffffu, q.pages, l);
+    return s;
+}
+
+EC_DEV int ta_scan(int v) {   // inclusive, over the warp
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int v = __shfl_up_sync(0xffffffffu, sum, o);
-            if (lane >= o) sum += v;
-        }
-        const unsigned hit = __ballot_sync(0xffffffffu, before + sum > ti);
+    for (int o = 1; o < 32; o <<= 1) {
+        const int u = __shfl_up_sync(0xffffffffu, v, o);
+        if ((int)(threadIdx.x & 31) >= o) v += u;
+    }
+    return v;
+}
+
+// The row tile `ti` in the sequences' order; false when there is none.  Called
+// by whole warps.
+EC_DEV bool ta_find(const ec_kv_pages &kv, const ec_tree_attn &a, const TaGeo &g, int ti, int kh, int mt, TaTile &s, int *err) {
+    int before = 0;
+    for (int b0 = 0; b0 < a.n_seq; b0 += 32) {
+        const TaSeq q = ta_seq(kv, a, g, mt, b0 + (threadIdx.x & 31), err);
+        const int sum = before + ta_scan(q.tiles);
+        const unsigned hit = __ballot_sync(0xffffffffu, sum > ti);
         if (hit) {
             const int l = __ffs((int)hit) - 1;
-            b = b0 + l;
-            local = ti - before - (__shfl_sync(0xffffffffu, sum, l) - __shfl_sync(0xffffffffu, n, l));
+            s = ta_tile(q, l, ti - __shfl_sync(0xffffffffu, sum - q.tiles, l), kh, mt);
+            return true;
         }
-        before += __shfl_sync(0xffffffffu, sum, 31);
+        before = __shfl_sync(0xffffffffu, sum, 31);
     }
-    if (b < 0) return false;
-    s.b = b;
-    s.first = local * mt;
-    s.r0 = a.row_start[b];
-    s.t = a.row_start[b + 1] - s.r0;
-    s.base = a.base[b];
-    s.slot = a.slots ? a.slots[b] : b;
-    if (s.r0 < 0 || s.r0 + s.t > a.rows || s.base < 0 || s.slot < 0 || s.slot >= kv.n_slots ||
-        (long long)s.base + s.t > (long long)kv.pages_per_slot * PAGE) {
-        if (threadIdx.x == 0) atomicCAS(err, 0, EC_KERR_BAD_INDEX);
+    return false;
+}
+
+// The pages of all tiles in one line (below 2^31 of them, ta_plan): sequence
+// by sequence, KV head by KV head, tile by tile.  CTA i of the first n takes
+// [start(i), start(i + 1)), at least a page each.
+struct TaLine {
+    TaSeq head;           // sequence of this lane among the first 32
+    int n, total, per, more;   // the first `more` pieces have per + 1 pages
+
+    EC_DEV static int work(const TaSeq &q, int kvh) { return q.tiles * q.pages * kvh; }
+    EC_DEV void init(const ec_kv_pages &kv, const ec_tree_attn &a, const TaGeo &g, int mt, int pieces, int *err) {
+        head = ta_seq(kv, a, g, mt, threadIdx.x & 31, err);
+        total = __reduce_add_sync(0xffffffffu, work(head, a.n_kv_head));
+        for (int b0 = 32; b0 < a.n_seq; b0 += 32)
+            total += __reduce_add_sync(0xffffffffu, work(ta_seq(kv, a, g, mt, b0 + (threadIdx.x & 31), err), a.n_kv_head));
+        n = min(pieces, total);
+        per = n ? total / n : 0;
+        more = total - per * n;
+    }
+    EC_DEV int start(int i) const { return per * i + min(i, more); }
+    EC_DEV int piece(int at) const {
+        const int wide = (per + 1) * more;
+        return at < wide ? at / (per + 1) : more + (at - wide) / per;
+    }
+    // the tile that holds place `at` (below total), and where it begins
+    EC_DEV TaTile tile(const ec_kv_pages &kv, const ec_tree_attn &a, const TaGeo &g, int mt, int at, int &begin, int *err) const {
+        int before = 0;
+        TaSeq q = head;
+        for (int b0 = 0;; b0 += 32) {
+            if (b0) q = ta_seq(kv, a, g, mt, b0 + (threadIdx.x & 31), err);
+            const int w = work(q, a.n_kv_head), sum = before + ta_scan(w);
+            const unsigned hit = __ballot_sync(0xffffffffu, sum > at);
+            if (hit || b0 + 32 >= a.n_seq) {
+                const int l = hit ? __ffs((int)hit) - 1 : 0;
+                const int from = __shfl_sync(0xffffffffu, sum - w, l);
+                const int pages = max(1, __shfl_sync(0xffffffffu, q.pages, l)), tiles = max(1, __shfl_sync(0xffffffffu, q.tiles, l));
+                const int unit = (at - from) / pages, kh = unit / tiles;
+                begin = from + unit * pages;
+                return ta_tile(q, l, unit - kh * tiles, kh, mt);
+            }
+            before = __shfl_sync(0xffffffffu, sum, 31);
+        }
+    }
+    // the tile number `index` of all, in the order of the line; false: none
+    EC_DEV bool by_index(const ec_kv_pages &kv, const ec_tree_attn &a, const TaGeo &g, int mt, int index, TaTile &s, int &begin, int *err) const {
+        int units = 0, before = 0;
+        TaSeq q = head;
+        for (int b0 = 0; b0 < a.n_seq; b0 += 32) {
+            if (b0) q = ta_seq(kv, a, g, mt, b0 + (threadIdx.x & 31), err);
+            const int w = work(q, a.n_kv_head), u = q.tiles * a.n_kv_head, ws = before + ta_scan(w), us = units + ta_scan(u);
+            const unsigned hit = __ballot_sync(0xffffffffu, us > index);
+            if (hit) {
+                const int l = __ffs((int)hit) - 1, unit = index - __shfl_sync(0xffffffffu, us - u, l);
+                const int tiles = __shfl_sync(0xffffffffu, q.tiles, l), kh = unit / tiles;
+                begin = __shfl_sync(0xffffffffu, ws - w, l) + unit * __shfl_sync(0xffffffffu, q.pages, l);
+                s = ta_tile(q, l, unit - kh * tiles, kh, mt);
+                return true;
+            }
+            before = __shfl_sync(0xffffffffu, ws, 31);
+            units = __shfl_sync(0xffffffffu, us, 31);
+        }
         return false;
     }
-    const int lo = a.window > 0 && s.base > a.window ? s.base - a.window : 0;   // no row sees a position below it
-    s.page0 = lo / PAGE;
-    s.page1 = (s.base + s.t + PAGE - 1) / PAGE;
-    return true;
-}
+};
 
 EC_DEV int ta_page(const ec_kv_pages &kv, int slot, int i, int *err) {
     int page = __ldg(kv.page_table + (size_t)slot * kv.pages_per_slot + i);
@@ -202,7 +290,9 @@ template <int HDP> EC_DEV uint32_t ta_at(int r, int c) { return (uint32_t)(r * H
 template <int QT, int KT> struct TaType {
     static constexpr bool BF = KT == EC_T_BF16, F32 = QT == EC_T_F32;
     static constexpr int NP = !F32 ? 1 : BF ? 3 : 2;
-    static constexpr float LIFT = BF ? 0.0f : 14.0f;
+    // fp32 q: p itself is exact to its last bit, and 2^14 multiplies its parts;
+    // 16-bit q: 14 is added to the exponent
+    static constexpr float LIFT = BF || F32 ? 0.0f : 14.0f, PARTS = F32 && !BF ? 16384.0f : 1.0f;
 };
 
 // WM x WN warps: WM groups of 16 rows, the 64 positions of a page shared out
@@ -214,15 +304,17 @@ template <int QT, int KT, int HDP, int WM, int WN, int STAGES> struct TaMma {
     static constexpr int TILE = PAGE * HDP * 2;                 // bytes of a K or V tile
     static constexpr int Q_BYTES = NP * MT * HDP * 2;
     static constexpr int RING = STAGES * 2 * TILE;
-    static constexpr int JOIN = WN > 1 ? WN * MT * (HDP + 2) * 4 : 0;   // overlays the ring
+    static constexpr int JOIN = WN * MT * (HDP + 2) * 4;       // overlays the ring
     static constexpr int SMEM = Q_BYTES + (RING > JOIN ? RING : JOIN) + MT * 4 + 128;
 };
 
 // Bounded by the bytes of K and V for few rows, and there by how many of them
 // are in flight: STAGES pages of K and V per CTA and two or three CTAs per SM
 // (hd 64: 16 KB a stage, hd 128: 32 KB).
-template <int QT, int KT, int HDP, int WM, int WN, int STAGES>
-__global__ void __launch_bounds__(32 * WM * WN) k_tree_mma(const ec_kv_pages kv, const ec_tree_attn a, const TaGeo g, int *err) {
+// PIECES: a CTA takes its piece of the line of pages, else (grid: tiles,
+// cluster, KV heads) its share of one tile.
+template <int QT, int KT, int HDP, int WM, int WN, int STAGES, bool PIECES>
+__global__ void __launch_bounds__(32 * WM * WN, HDP == 64 && QT != EC_T_F32 ? 3 : HDP <= 128 ? 2 : 1) k_tree_mma(const ec_kv_pages kv, const ec_tree_attn a, const TaGeo g, int *err) {
     EC_PDL_ENTER();
     typedef TaMma<QT, KT, HDP, WM, WN, STAGES> C;
     typedef typename C::Ty Ty;
@@ -232,14 +324,42 @@ __global__ void __launch_bounds__(32 * WM * WN) k_tree_mma(const ec_kv_pages kv,
     const uint32_t sq = ec_smem_u32(smem), ring = sq + C::Q_BYTES;
     float *row_scale = reinterpret_cast<float *>(smem + C::SMEM - 128 - C::MT * 4);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, wm = warp % WM, wn = warp / WM;
-    const int kh = blockIdx.z, hd = a.head_dim;
+    const int hd = a.head_dim;
     TaTile s;
-    if (!ta_find(kv, a, g, blockIdx.x, C::MT, s, err)) return;
-    int chunk;
-    const int splits = ta_splits(s, g, chunk), split = blockIdx.y;
-    if (split >= splits) return;
-    const int p_begin = s.page0 + split * chunk, p_end = min(s.page1, p_begin + chunk), end = s.base + s.t;
+    int p_begin, p_end;
+    int at = 0, stop = 0, tile_begin = 0;   // PIECES: places on the line
+    TaLine line;
+    if constexpr (PIECES) {
+        line.init(kv, a, g, C::MT, gridDim.x, err);
+        if ((int)blockIdx.x >= line.n) return;
+        at = line.start(blockIdx.x);
+        stop = line.start(blockIdx.x + 1);
+    } else {
+        if (!ta_find(kv, a, g, blockIdx.x, blockIdx.z, C::MT, s, err)) return;   // all CTAs of the cluster alike
+        const int chunk = (s.page1 - s.page0 + g.cluster - 1) / g.cluster;
+        p_begin = min(s.page1, s.page0 + (int)blockIdx.y * chunk);
+        p_end = min(s.page1, p_begin + chunk);
+    }
+    do {
+    if constexpr (PIECES) {
+        if (at >= stop) return;
+        s = line.tile(kv, a, g, C::MT, at, tile_begin, err);
+        p_begin = s.page0 + (at - tile_begin);
+        p_end = min(s.page1, p_begin + (stop - at));
+    }
+    const int kh = s.kh, end = s.base + s.t;
 
+    // the numbers of the first pages, the queries, then the pages themselves
+    int pg[STAGES];
+#pragma unroll
+    for (int i = 0; i < STAGES; ++i) pg[i] = p_begin + i < p_end ? ta_page(kv, s.slot, p_begin + i, err) : 0;
+    const bool wide = Ty::F32 ? (a.ldq & 3) == 0 && (reinterpret_cast<uintptr_t>(a.q) & 15) == 0
+                              : (a.ldq & 7) == 0 && (reinterpret_cast<uintptr_t>(a.q) & 15) == 0;   // 16-byte reads of q
+    auto q_at = [&](int r, bool &real) {   // offset in q of the tile's row r; rows behind the sequence are zero
+        const int rr = s.first + r, node = ta_node(g, rr);
+        real = node < s.t;
+        return real ? (size_t)(s.r0 + node) * a.ldq + (size_t)(kh * g.group + rr - node * g.group) * hd : 0;
+    };
     auto fetch = [&](int page, int stage, int pg) {   // page: index in the slot; pg: in the arena
         const uint32_t dk = ring + stage * 2 * C::TILE, dv = dk + C::TILE;
         const size_t off = (size_t)pg * kv.ld_page + (size_t)kh * hd;
@@ -254,61 +374,95 @@ __global__ void __launch_bounds__(32 * WM * WN) k_tree_mma(const ec_kv_pages kv,
             cp16(dv + ta_at<HDP>(r, c), v + at, real);
         }
     };
-    int next_pg = 0;
+    auto fetch_first = [&]() {
 #pragma unroll
-    for (int i = 0; i < STAGES - 1; ++i) {
-        if (p_begin + i < p_end) fetch(p_begin + i, i, ta_page(kv, s.slot, p_begin + i, err));
-        cp_commit();
-    }
-    if (p_begin + STAGES - 1 < p_end) next_pg = ta_page(kv, s.slot, p_begin + STAGES - 1, err);
-
-    // the queries of the tile, in parts; rows behind the sequence are zero
-    for (int r = warp; r < C::MT; r += WM * WN) {
-        const int rr = s.first + r, node = rr / g.group;
-        const bool real = node < s.t;
-        const size_t at = real ? (size_t)(s.r0 + node) * a.ldq + ((size_t)kh * g.group + rr % g.group) * hd : 0;
-        float x[HDP / 32], scale = 1.0f;
-        if (Ty::F32) {
-            float mx = 0.0f;
-#pragma unroll
-            for (int i = 0; i < HDP / 32; ++i) {
-                const int d = lane + 32 * i;
-                x[i] = real && d < hd ? static_cast<const float *>(a.q)[at + d] : 0.0f;
-                mx = ec_max_keep(mx, fabsf(x[i]));
-            }
-            mx = ec_warp_max(mx);
-            float back = 1.0f;
-            if (!BF && mx > 0.0f && mx < INFINITY) {
-                int e;
-                frexpf(mx, &e);
-                e = max(e, -100);   // 2^(14 - e) and its inverse stay normal
-                scale = ldexpf(1.0f, 14 - e);
-                back = ldexpf(1.0f, e - 14);
-            }
-            if (lane == 0) row_scale[r] = back;
+        for (int i = 0; i < STAGES - 1; ++i) {
+            if (p_begin + i < p_end) fetch(p_begin + i, i, pg[i]);
+            cp_commit();
         }
+    };
+    if constexpr (!Ty::F32) {
+        constexpr int CH = HDP / 8;
+        if (wide) {
+#pragma unroll 4
+            for (int i = threadIdx.x; i < C::MT * CH; i += C::THREADS) {
+                const int r = i / CH, c = i % CH;
+                bool real;
+                const size_t at = q_at(r, real);
+                real = real && c * 8 < hd;
+                cp16(sq + ta_at<HDP>(r, c), static_cast<const uint16_t *>(a.q) + (real ? at + c * 8 : 0), real);
+            }
+        } else {
+            for (int i = threadIdx.x; i < C::MT * HDP; i += C::THREADS) {
+                const int r = i / HDP, d = i % HDP;
+                bool real;
+                const size_t at = q_at(r, real);
+                *reinterpret_cast<uint16_t *>(smem + ta_at<HDP>(r, d / 8) + (d % 8) * 2) = real && d < hd ? static_cast<const uint16_t *>(a.q)[at + d] : (uint16_t)0;
+            }
+        }
+        fetch_first();   // q is part of the first group
+        cp_wait<STAGES - 2>();
+    } else {
+        // four elements a lane, BATCH rows' loads in flight
+        constexpr int LANES = HDP / 4 < 32 ? HDP / 4 : 32, EACH = HDP / 4 / LANES, ROWS = 32 / LANES, PASSES = C::MT / (WM * WN * ROWS);
+        constexpr int BATCH = PASSES < 8 / EACH ? PASSES : 8 / EACH;
+        bool fetched = false;
+        for (int b0 = 0; b0 < PASSES; b0 += BATCH) {
+            float4 x[BATCH][EACH];
 #pragma unroll
-        for (int i = 0; i < HDP / 32; ++i) {
-            const int d = lane + 32 * i;
-            unsigned char *to = smem + ta_at<HDP>(r, d / 8) + (d % 8) * 2;
-            if (Ty::F32) {
-                float left = x[i] * scale;
+            for (int i = 0; i < BATCH; ++i) {
+                bool real;
+                const size_t at = q_at(((b0 + i) * WM * WN + warp) * ROWS + lane / LANES, real);
 #pragma unroll
-                for (int p = 0; p < NP; ++p) {
-                    const uint32_t u = pack2<BF>(left, 0.0f) & 0xffffu;
-                    *reinterpret_cast<uint16_t *>(to + p * C::MT * HDP * 2) = (uint16_t)u;
-                    left -= unpack2<BF>(u).x;
+                for (int e = 0; e < EACH; ++e) {
+                    const int d = (lane % LANES + e * LANES) * 4;
+                    const float *q = static_cast<const float *>(a.q) + at + d;
+                    x[i][e] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    if (real && d < hd) x[i][e] = wide ? *reinterpret_cast<const float4 *>(q) : make_float4(q[0], q[1], q[2], q[3]);
                 }
-            } else {
-                *reinterpret_cast<uint16_t *>(to) = real && d < hd ? static_cast<const uint16_t *>(a.q)[at + d] : (uint16_t)0;
+            }
+            if (!fetched) fetch_first();
+            fetched = true;
+#pragma unroll
+            for (int i = 0; i < BATCH; ++i) {
+                const int r = ((b0 + i) * WM * WN + warp) * ROWS + lane / LANES;
+                float scale = 1.0f, back = 1.0f, mx = 0.0f;
+#pragma unroll
+                for (int e = 0; e < EACH; ++e)
+                    mx = fmaxf(fmaxf(fmaxf(mx, fabsf(x[i][e].x)), fmaxf(fabsf(x[i][e].y), fabsf(x[i][e].z))), fabsf(x[i][e].w));
+#pragma unroll
+                for (int o = LANES / 2; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+                if (!BF && mx > 0.0f && mx < INFINITY) {
+                    int e;
+                    frexpf(mx, &e);
+                    e = max(e, -100);   // 2^(14 - e) and its inverse stay normal
+                    scale = __int_as_float((127 + 14 - e) << 23);
+                    back = __int_as_float((127 + e - 14) << 23);
+                }
+                if (lane % LANES == 0) row_scale[r] = back;
+#pragma unroll
+                for (int e = 0; e < EACH; ++e) {
+                    const int d = (lane % LANES + e * LANES) * 4;
+                    float4 y = make_float4(x[i][e].x * scale, x[i][e].y * scale, x[i][e].z * scale, x[i][e].w * scale);
+                    unsigned char *to = smem + ta_at<HDP>(r, d / 8) + (d % 8) * 2;
+#pragma unroll
+                    for (int p = 0; p < NP; ++p) {
+                        const uint2 u = make_uint2(pack2<BF>(y.x, y.y), pack2<BF>(y.z, y.w));
+                        *reinterpret_cast<uint2 *>(to + p * C::MT * HDP * 2) = u;
+                        const float2 lo = unpack2<BF>(u.x), hi = unpack2<BF>(u.y);
+                        y = make_float4(y.x - lo.x, y.y - lo.y, y.z - hi.x, y.w - hi.y);
+                    }
+                }
             }
         }
     }
+    int next_pg = pg[STAGES - 1];
     __syncthreads();
 
     const int row_lo = wm * 16 + lane / 4;                 // this thread's rows: row_lo and row_lo + 8
-    const int node_lo = (s.first + row_lo) / g.group, node_hi = (s.first + row_lo + 8) / g.group;
-    const float f_lo = Ty::F32 ? g.scale2 * row_scale[row_lo] : g.scale2, f_hi = Ty::F32 ? g.scale2 * row_scale[row_lo + 8] : g.scale2;
+    const int node_lo = ta_node(g, s.first + row_lo), node_hi = ta_node(g, s.first + row_lo + 8);
+    const float f_lo = Ty::F32 ? fmaxf(g.scale2 * row_scale[row_lo], 1e-37f) : g.scale2;   // above 0: masked scores stay -inf
+    const float f_hi = Ty::F32 ? fmaxf(g.scale2 * row_scale[row_lo + 8], 1e-37f) : g.scale2;
     float o[ND][4], m_lo = -INFINITY, m_hi = -INFINITY, l_lo = 0.0f, l_hi = 0.0f;
 #pragma unroll
     for (int i = 0; i < ND; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
@@ -374,8 +528,6 @@ __global__ void __launch_bounds__(32 * WM * WN) k_tree_mma(const ec_kv_pages kv,
         for (int i = 0; i < NK; ++i) {
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                sc[i][e] *= f_lo;
-                sc[i][2 + e] *= f_hi;
                 if (part) {
                     const unsigned b_lo = i < 4 ? w_lo >> (8 * i + e) : z_lo >> (8 * (i - 4) + e), b_hi = i < 4 ? w_hi >> (8 * i + e) : z_hi >> (8 * (i - 4) + e);
                     if (!(b_lo & 1u)) sc[i][e] = -INFINITY;
@@ -390,8 +542,8 @@ __global__ void __launch_bounds__(32 * WM * WN) k_tree_mma(const ec_kv_pages kv,
             x_lo = fmaxf(x_lo, __shfl_xor_sync(0xffffffffu, x_lo, d));
             x_hi = fmaxf(x_hi, __shfl_xor_sync(0xffffffffu, x_hi, d));
         }
-        x_lo = fmaxf(x_lo, m_lo);
-        x_hi = fmaxf(x_hi, m_hi);
+        x_lo = fmaxf(x_lo * f_lo, m_lo);
+        x_hi = fmaxf(x_hi * f_hi, m_hi);
         const float u_lo = x_lo == -INFINITY ? 0.0f : x_lo, u_hi = x_hi == -INFINITY ? 0.0f : x_hi;   // nothing seen yet: weights 0
         float c_lo = ex2(m_lo - u_lo), c_hi = ex2(m_hi - u_hi);
         m_lo = x_lo;
@@ -404,11 +556,14 @@ __global__ void __launch_bounds__(32 * WM * WN) k_tree_mma(const ec_kv_pages kv,
             float p[4];
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                p[e] = ex2(sc[i][e] - u_lo + Ty::LIFT);
-                p[2 + e] = ex2(sc[i][2 + e] - u_hi + Ty::LIFT);
+                p[e] = ex2(fmaf(sc[i][e], f_lo, Ty::LIFT - u_lo));
+                p[2 + e] = ex2(fmaf(sc[i][2 + e], f_hi, Ty::LIFT - u_hi));
                 l_lo += p[e];
                 l_hi += p[2 + e];
             }
+            if (Ty::PARTS != 1.0f)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) p[e] *= Ty::PARTS;
 #pragma unroll
             for (int q = 0; q < NP; ++q) {
                 const uint32_t lo = pack2<BF>(p[0], p[1]), hi = pack2<BF>(p[2], p[3]);
@@ -495,141 +650,304 @@ __global__ void __launch_bounds__(32 * WM * WN) k_tree_mma(const ec_kv_pages kv,
         l_lo += __shfl_xor_sync(0xffffffffu, l_lo, d);
         l_hi += __shfl_xor_sync(0xffffffffu, l_hi, d);
     }
-    if (WN > 1) {   // join the warps that share the rows, in shared memory
+    // Where this CTA has all of the tile's pages it writes out, else (m, l, o).
+    const bool pair = (a.ldo & 1) == 0 && (reinterpret_cast<uintptr_t>(a.out) & (QT == EC_T_F32 ? 7 : 3)) == 0;
+    const bool whole = !PIECES || (p_begin == s.page0 && p_end == s.page1);
+    const size_t part_at = ((size_t)blockIdx.x * 2 + (p_begin == s.page0)) * C::MT;   // PIECES: a CTA has at most one tile begun before, one left open
+    float *po = g.part + part_at * HDP, *pm = g.part + (size_t)gridDim.x * 2 * C::MT * HDP + part_at * 2;
+    // Join the warps that share rows and the CTAs of the cluster: every one
+    // leaves its (m, l, o) in its shared memory, each CTA takes a share of the
+    // rows, a warp a row, and lane i the weight of source i.
+    const int ctas = PIECES ? 1 : g.cluster, me = PIECES ? 0 : (int)blockIdx.y, sources = ctas * WN;
+    if (sources > 1) {
+        cg::cluster_group cl = cg::this_cluster();
         cp_wait<0>();
         __syncthreads();
         float *jo = reinterpret_cast<float *>(smem + C::Q_BYTES), *jm = jo + WN * C::MT * HDP;   // [WN][MT][HDP], [WN][MT][2]
 #pragma unroll
         for (int n = 0; n < ND; ++n) {
-            float *p = jo + (size_t)(wn * C::MT + row_lo) * HDP + n * 8 + (lane % 4) * 2;
+            float *p = jo + (size_t)(wn * C::MT + row_lo) * HDP + ((n * 8 + (lane % 4) * 2) ^ ((row_lo & 7) * 4));   // rows shifted against bank conflicts
             *reinterpret_cast<float2 *>(p) = make_float2(o[n][0], o[n][1]);
             *reinterpret_cast<float2 *>(p + 8 * HDP) = make_float2(o[n][2], o[n][3]);
         }
         if (lane % 4 == 0) {
-            jm[(wn * C::MT + row_lo) * 2] = m_lo; jm[(wn * C::MT + row_lo) * 2 + 1] = l_lo;
-            jm[(wn * C::MT + row_lo + 8) * 2] = m_hi; jm[(wn * C::MT + row_lo + 8) * 2 + 1] = l_hi;
+            *reinterpret_cast<float2 *>(jm + (wn * C::MT + row_lo) * 2) = make_float2(m_lo, l_lo);
+            *reinterpret_cast<float2 *>(jm + (wn * C::MT + row_lo + 8) * 2) = make_float2(m_hi, l_hi);
         }
-        __syncthreads();
-        const size_t part_at = (((size_t)blockIdx.x * a.n_kv_head + kh) * g.nsplit + split) * C::MT;
-        float *po = g.part + part_at * HDP, *pm = g.part + (size_t)g.tiles * a.n_kv_head * g.nsplit * C::MT * HDP + part_at * 2;
-        for (int r = warp; r < C::MT; r += WM * WN) {
-            const int rr = s.first + r, node = rr / g.group;
+        if (ctas > 1) cl.sync();
+        else __syncthreads();
+        for (int r = me + warp * ctas; r < C::MT; r += ctas * WM * WN) {
+            const int rr = s.first + r, node = ta_node(g, rr);
             if (node >= s.t) continue;
-            float m = -INFINITY, f[WN], l = 0.0f;
-#pragma unroll
-            for (int w = 0; w < WN; ++w) m = fmaxf(m, jm[(w * C::MT + r) * 2]);
-            const float u = m == -INFINITY ? 0.0f : m;
-#pragma unroll
-            for (int w = 0; w < WN; ++w) {
-                f[w] = ex2(jm[(w * C::MT + r) * 2] - u);
-                l += jm[(w * C::MT + r) * 2 + 1] * f[w];
+            float2 ml = make_float2(-INFINITY, 0.0f);
+            if (lane < sources) {
+                const float *p = jm + ((lane / ctas) * C::MT + r) * 2;
+                ml = *reinterpret_cast<const float2 *>(ctas > 1 ? cl.map_shared_rank(p, lane % ctas) : p);
             }
-            const float inv = splits > 1 ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
-            const size_t at = (size_t)(s.r0 + node) * a.ldo + ((size_t)kh * g.group + rr % g.group) * hd;
-            if (splits > 1 && lane == 0) { pm[r * 2] = m; pm[r * 2 + 1] = l; }
-            for (int d = lane * 2; d < hd; d += 64) {
-                float x = 0.0f, y = 0.0f;
+            float m = ml.x;
 #pragma unroll
-                for (int w = 0; w < WN; ++w) {
-                    const float2 v = *reinterpret_cast<const float2 *>(jo + (size_t)(w * C::MT + r) * HDP + d);
-                    x = fmaf(v.x, f[w], x);
-                    y = fmaf(v.y, f[w], y);
+            for (int d = 16; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
+            const float f = ex2(ml.x - (m == -INFINITY ? 0.0f : m));
+            const float l = ec_warp_sum(ml.y * f);
+            constexpr int EACH = HDP >= 128 ? HDP / 128 : 1, VEC = HDP >= 128 ? 4 : 2;
+            float acc[EACH][VEC] = {};
+#pragma unroll 4
+            for (int i = 0; i < sources; ++i) {
+                const float w = __shfl_sync(0xffffffffu, f, i);
+                const float *p = jo + (size_t)((i / ctas) * C::MT + r) * HDP;
+                if (ctas > 1) p = cl.map_shared_rank(p, i % ctas);
+#pragma unroll
+                for (int e = 0; e < EACH; ++e) {
+                    const int d = (lane * VEC + e * 128) ^ ((r & 7) * 4);
+                    if constexpr (VEC == 4) {
+                        const float4 v = *reinterpret_cast<const float4 *>(p + d);
+                        acc[e][0] = fmaf(v.x, w, acc[e][0]); acc[e][1] = fmaf(v.y, w, acc[e][1]);
+                        acc[e][2] = fmaf(v.z, w, acc[e][2]); acc[e][3] = fmaf(v.w, w, acc[e][3]);
+                    } else {
+                        const float2 v = *reinterpret_cast<const float2 *>(p + d);
+                        acc[e][0] = fmaf(v.x, w, acc[e][0]); acc[e][1] = fmaf(v.y, w, acc[e][1]);
+                    }
                 }
-                if (splits > 1) *reinterpret_cast<float2 *>(po + (size_t)r * HDP + d) = make_float2(x, y);
-                else ta_store2<QT>(a.out, at + d, x * inv, y * inv, false);
+            }
+            const float inv = l == 0.0f ? 0.0f : (1.0f / Ty::PARTS) / l;
+            const size_t to = (size_t)(s.r0 + node) * a.ldo + (size_t)(kh * g.group + rr - node * g.group) * hd;
+            if (!whole && lane == 0) *reinterpret_cast<float2 *>(pm + r * 2) = make_float2(m, l);
+#pragma unroll
+            for (int e = 0; e < EACH; ++e)
+#pragma unroll
+                for (int h = 0; h < VEC; h += 2) {
+                    const int d = lane * VEC + e * 128 + h;
+                    if (d >= hd) continue;
+                    if (!whole) *reinterpret_cast<float2 *>(po + (size_t)r * HDP + d) = make_float2(acc[e][h], acc[e][h + 1]);
+                    else ta_store2<QT>(a.out, to + d, acc[e][h] * inv, acc[e][h + 1] * inv, pair);
+                }
+        }
+        if (ctas > 1) cl.sync();   // the others have read this CTA's part
+    } else {
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            const int r = row_lo + 8 * half, rr = s.first + r, node = half ? node_hi : node_lo;
+            if (node >= s.t) continue;
+            const float m = half ? m_hi : m_lo, l = half ? l_hi : l_lo, inv = l == 0.0f ? 0.0f : (1.0f / Ty::PARTS) / l;
+            const size_t to = (size_t)(s.r0 + node) * a.ldo + (size_t)(kh * g.group + rr - node * g.group) * hd;
+            if (!whole && lane % 4 == 0) *reinterpret_cast<float2 *>(pm + r * 2) = make_float2(m, l);
+#pragma unroll
+            for (int n = 0; n < ND; ++n) {
+                const int d = n * 8 + (lane % 4) * 2;
+                if (d >= hd) continue;
+                const float x = o[n][2 * half], y = o[n][2 * half + 1];
+                if (!whole) *reinterpret_cast<float2 *>(po + (size_t)r * HDP + d) = make_float2(x, y);
+                else ta_store2<QT>(a.out, to + d, x * inv, y * inv, pair);
             }
         }
-        return;
     }
-    const size_t part_at = (((size_t)blockIdx.x * a.n_kv_head + kh) * g.nsplit + split) * C::MT;
-    float *po = g.part + part_at * HDP, *pm = g.part + (size_t)g.tiles * a.n_kv_head * g.nsplit * C::MT * HDP + part_at * 2;
-    const bool pair = ((a.ldo & 1) == 0) && ((reinterpret_cast<uintptr_t>(a.out) & (QT == EC_T_F32 ? 7 : 3)) == 0);
-#pragma unroll
-    for (int half = 0; half < 2; ++half) {
-        const int r = row_lo + 8 * half, rr = s.first + r, node = half ? node_hi : node_lo;
-        if (node >= s.t) continue;
-        const float m = half ? m_hi : m_lo, l = half ? l_hi : l_lo;
-        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-        const size_t at = (size_t)(s.r0 + node) * a.ldo + ((size_t)kh * g.group + rr % g.group) * hd;
-        if (splits > 1 && lane % 4 == 0) { pm[r * 2] = m; pm[r * 2 + 1] = l; }
-#pragma unroll
-        for (int n = 0; n < ND; ++n) {
-            const int d = n * 8 + (lane % 4) * 2;
-            if (d >= hd) continue;
-            const float x = o[n][2 * half], y = o[n][2 * half + 1];
-            if (splits > 1) *reinterpret_cast<float2 *>(po + (size_t)r * HDP + d) = make_float2(x, y);
-            else ta_store2<QT>(a.out, at + d, x * inv, y * inv, pair);
-        }
+    if constexpr (PIECES) {
+        at += p_end - p_begin;
+        cp_wait<0>();
+        __syncthreads();   // shared memory is free for the next tile
     }
+    } while (PIECES);
 }
 
-// out of a row tile from its splits' (m, l, o), in their order: one warp a row
-template <int QT>
-__global__ void __launch_bounds__(128) k_tree_join(const ec_kv_pages kv, const ec_tree_attn a, const TaGeo g, int mt, int hdp, int *err) {
-    EC_PDL_ENTER();
-    TaTile s;
-    if (!ta_find(kv, a, g, blockIdx.x, mt, s, err)) return;
-    int chunk;
-    const int splits = ta_splits(s, g, chunk);
-    if (splits <= 1) return;
-    const int kh = blockIdx.z, r = blockIdx.y * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31, hd = a.head_dim;
-    const int rr = s.first + r, node = rr / g.group;
-    if (r >= mt || node >= s.t) return;
-    const size_t at = ((size_t)blockIdx.x * a.n_kv_head + kh) * g.nsplit * mt + r;
-    const float *po = g.part + at * hdp, *pm = g.part + (size_t)g.tiles * a.n_kv_head * g.nsplit * mt * hdp + at * 2;
-    float m = -INFINITY;
-    for (int i = lane; i < splits; i += 32) m = fmaxf(m, pm[(size_t)i * mt * 2]);
+// A lane's part of a row of partial sums: VEC floats, EACH times.
+template <int HDP> struct TaLane {
+    static constexpr int VEC = HDP >= 128 ? 4 : 2, EACH = HDP / 32 / VEC;
+    float v[EACH][VEC];
+    EC_DEV void zero() {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    if (m == -INFINITY) m = 0.0f;
-    float l = 0.0f, acc[8] = {};
-    for (int i = 0; i < splits; ++i) {
-        const float2 ml = *reinterpret_cast<const float2 *>(pm + (size_t)i * mt * 2);
-        const float f = ex2(ml.x - m);
-        l = fmaf(ml.y, f, l);
+        for (int e = 0; e < EACH; ++e)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int d = lane * 2 + 64 * j;
-            if (d >= hd) break;
-            const float2 v = *reinterpret_cast<const float2 *>(po + (size_t)i * mt * hdp + d);
-            acc[2 * j] = fmaf(v.x, f, acc[2 * j]);
-            acc[2 * j + 1] = fmaf(v.y, f, acc[2 * j + 1]);
+            for (int i = 0; i < VEC; ++i) v[e][i] = 0.0f;
+    }
+    EC_DEV void load(const float *row) {
+#pragma unroll
+        for (int e = 0; e < EACH; ++e) {
+            const float *p = row + (threadIdx.x & 31) * VEC + e * 128;
+            if constexpr (VEC == 4) {
+                const float4 x = *reinterpret_cast<const float4 *>(p);
+                v[e][0] = x.x; v[e][1] = x.y; v[e][2] = x.z; v[e][3] = x.w;
+            } else {
+                const float2 x = *reinterpret_cast<const float2 *>(p);
+                v[e][0] = x.x; v[e][1] = x.y;
+            }
         }
     }
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    const size_t to = (size_t)(s.r0 + node) * a.ldo + ((size_t)kh * g.group + rr % g.group) * hd;
+    EC_DEV void add(const TaLane &o, float w) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        const int d = lane * 2 + 64 * j;
-        if (d < hd) ta_store2<QT>(a.out, to + d, acc[2 * j] * inv, acc[2 * j + 1] * inv, false);
+        for (int e = 0; e < EACH; ++e)
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) v[e][i] = fmaf(o.v[e][i], w, v[e][i]);
+    }
+    template <int QT> EC_DEV void store(void *out, size_t to, int hd, float inv) const {
+#pragma unroll
+        for (int e = 0; e < EACH; ++e)
+#pragma unroll
+            for (int i = 0; i < VEC; i += 2) {
+                const int d = (threadIdx.x & 31) * VEC + e * 128 + i;
+                if (d < hd) ta_store2<QT>(out, to + d, v[e][i] * inv, v[e][i + 1] * inv, false);
+            }
+    }
+};
+
+// Joins the tiles that borders between pieces cut, in the order of their
+// pages.  SHARED (few tiles, cut into many pieces): CTA (tile, r) joins row r,
+// its warps sharing out the pieces.  Otherwise CTA (i, y) joins half of the
+// rows, up to four a warp, of the tile that the border behind piece i is the
+// first to cut.
+constexpr int TJ_THREADS = 256, TJ_WARPS = TJ_THREADS / 32, TJ_PIECES = 1024;
+
+template <int QT, int HDP, bool SHARED>
+__global__ void __launch_bounds__(TJ_THREADS) k_tree_join(const ec_kv_pages kv, const ec_tree_attn a, const TaGeo g, int mt, int pieces, float unit, int *err) {
+    EC_PDL_ENTER();
+    typedef TaLane<HDP> Lane;
+    __shared__ float weight[SHARED ? TJ_PIECES : 1], red[TJ_WARPS], acc_of[SHARED ? TJ_WARPS : 1][HDP];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, hd = a.head_dim;
+    TaLine line;
+    line.init(kv, a, g, mt, pieces, err);
+    TaTile s;
+    int begin, i0 = blockIdx.x;
+    if (SHARED) {
+        if (!line.by_index(kv, a, g, mt, blockIdx.x, s, begin, err)) return;
+        i0 = line.piece(begin);
+    } else {
+        if (i0 + 1 >= line.n) return;
+        const int border = line.start(i0 + 1);
+        s = line.tile(kv, a, g, mt, border, begin, err);
+        if (begin == border || line.start(i0) > begin) return;   // cuts nothing, or not the first
+    }
+    const int n = line.piece(begin + (s.page1 - s.page0) - 1) - i0 + 1;   // pieces of the tile
+    if (n == 1) return;
+    auto place = [&](int i, int r) { return ((size_t)(i0 + i) * 2 + (i == 0)) * mt + r; };   // begun in piece i0, goes on in the others
+    auto out_at = [&](int r) {
+        const int rr = s.first + r, node = ta_node(g, rr);
+        return (size_t)(s.r0 + node) * a.ldo + (size_t)(s.kh * g.group + rr - node * g.group) * hd;
+    };
+    const float *po = g.part, *pm = g.part + (size_t)pieces * 2 * mt * HDP;
+    if constexpr (SHARED) {
+        const int r = blockIdx.y;
+        if (ta_node(g, s.first + r) >= s.t) return;
+        auto join = [&](float v, bool max) {
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) {
+                const float u = __shfl_xor_sync(0xffffffffu, v, o);
+                v = max ? fmaxf(v, u) : v + u;
+            }
+            __syncthreads();
+            if (lane == 0) red[warp] = v;
+            __syncthreads();
+            v = red[0];
+#pragma unroll
+            for (int w = 1; w < TJ_WARPS; ++w) v = max ? fmaxf(v, red[w]) : v + red[w];
+            return v;
+        };
+        float m = -INFINITY, l = 0.0f;
+        for (int i = threadIdx.x; i < n; i += TJ_THREADS) m = fmaxf(m, pm[place(i, r) * 2]);
+        m = join(m, true);
+        if (m == -INFINITY) m = 0.0f;
+        for (int i = threadIdx.x; i < n; i += TJ_THREADS) {
+            const float2 ml = *reinterpret_cast<const float2 *>(pm + place(i, r) * 2);
+            const float f = ex2(ml.x - m);
+            l = fmaf(ml.y, f, l);
+            weight[i] = f;
+        }
+        l = join(l, false);
+        Lane acc;
+        acc.zero();
+        for (int b = warp; b < n; b += 8 * TJ_WARPS) {
+            Lane x[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[j].load(po + place(min(b + j * TJ_WARPS, n - 1), r) * HDP);
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (b + j * TJ_WARPS < n) acc.add(x[j], weight[b + j * TJ_WARPS]);
+        }
+#pragma unroll
+        for (int e = 0; e < Lane::EACH; ++e)
+#pragma unroll
+            for (int i = 0; i < Lane::VEC; ++i) acc_of[warp][lane * Lane::VEC + e * 128 + i] = acc.v[e][i];
+        __syncthreads();
+        const float inv = l == 0.0f ? 0.0f : unit / l;
+        for (int d = threadIdx.x * 2; d < hd; d += 2 * TJ_THREADS) {
+            float x = 0.0f, y = 0.0f;
+#pragma unroll
+            for (int w = 0; w < TJ_WARPS; ++w) { x += acc_of[w][d]; y += acc_of[w][d + 1]; }
+            ta_store2<QT>(a.out, out_at(r) + d, x * inv, y * inv, false);
+        }
+    } else {
+        constexpr int ROWS = HDP == 256 ? 2 : 4;
+        const int stride = gridDim.y * TJ_WARPS;
+        for (int r0 = blockIdx.y * TJ_WARPS + warp; r0 < mt; r0 += ROWS * stride) {
+            Lane acc[ROWS];
+            float m[ROWS], l[ROWS];
+#pragma unroll
+            for (int k = 0; k < ROWS; ++k) {
+                acc[k].zero();
+                m[k] = -INFINITY;
+                l[k] = 0.0f;
+            }
+            for (int i = 0; i < n; ++i) {   // one pass with a running maximum: the rows' loads go together
+                Lane x[ROWS];
+                float2 ml[ROWS];
+#pragma unroll
+                for (int k = 0; k < ROWS; ++k) {
+                    const int r = min(r0 + k * stride, mt - 1);
+                    ml[k] = *reinterpret_cast<const float2 *>(pm + place(i, r) * 2);
+                    x[k].load(po + place(i, r) * HDP);
+                }
+#pragma unroll
+                for (int k = 0; k < ROWS; ++k) {
+                    const float mn = fmaxf(m[k], ml[k].x), u = mn == -INFINITY ? 0.0f : mn;
+                    const float c = ex2(m[k] - u), f = ex2(ml[k].x - u);
+                    m[k] = mn;
+                    l[k] = fmaf(ml[k].y, f, l[k] * c);
+#pragma unroll
+                    for (int e = 0; e < Lane::EACH; ++e)
+#pragma unroll
+                        for (int j = 0; j < Lane::VEC; ++j) acc[k].v[e][j] = fmaf(x[k].v[e][j], f, acc[k].v[e][j] * c);
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < ROWS; ++k) {
+                const int r = r0 + k * stride;
+                if (r < mt && ta_node(g, s.first + r) < s.t) acc[k].template store<QT>(a.out, out_at(r), hd, l[k] == 0.0f ? 0.0f : unit / l[k]);
+            }
+        }
     }
 }
 
 // ---- launch --------------------------------------------------------------------
 
-struct TaPlan { int hdp, mt; TaGeo g; size_t bytes; };
+struct TaPlan {
+    int hdp, mt, tiles;   // tiles: upper bound over all sequences
+    int pieces;           // 0: clusters
+    TaGeo g;
+};
 
 int ta_up(int a, int b) { return (a + b - 1) / b; }
 
-// The split: enough CTAs for two per SM where the pages allow it.
-TaPlan ta_plan(int n_seq, int rows, int n_head, int n_kv_head, int hd, int max_len, int window, int sms) {
+size_t ta_piece_bytes(const TaPlan &p) { return (size_t)2 * p.mt * (p.hdp + 2) * 4; }
+
+// Clusters where they alone give every SM something to do or a tile has few
+// pages: one launch (one token over 300 positions: 7.2 us, in pieces 9.5).
+// Otherwise as many pieces as CTAs are resident.
+TaPlan ta_plan(int n_seq, int rows, int n_head, int n_kv_head, int hd, int max_len, int slot_pages, int window, bool f32, int sms) {
     TaPlan p;
     p.hdp = hd <= 64 ? 64 : hd <= 128 ? 128 : 256;
     p.g.group = n_head / n_kv_head;
+    int up = 0;
+    while ((1 << up) < p.g.group) ++up;
+    p.g.div_shift = 30 + up;   // rounded up: exact for rows below 2^30
+    p.g.div_mul = (unsigned)(((1ull << p.g.div_shift) + p.g.group - 1) / p.g.group);
     const int mean = (int)(((long long)rows * p.g.group + n_seq - 1) / n_seq);
     p.mt = mean <= 16 ? 16 : mean <= 32 ? 32 : 64;
-    const long long tiles = ((long long)rows * p.g.group) / p.mt + n_seq;   // every sequence rounds up once
-    p.g.tiles = (int)tiles;   // rows * group fits 31 bits
+    p.tiles = (int)(((long long)rows * p.g.group) / p.mt + n_seq);   // every sequence rounds up once; rows * group fits 31 bits
     int pages = ta_up(max_len > 0 ? max_len : 1, PAGE);
     if (window > 0 && pages > window / PAGE + 2) pages = window / PAGE + 2;
-    const long long real = (long long)ta_up(mean, p.mt) * n_seq * n_kv_head;
-    long long want = (2LL * sms + real - 1) / real;
-    if (want > pages) want = pages;
-    if (want > 256) want = 256;
-    if (want < 1) want = 1;
-    p.g.chunk = ta_up(pages, (int)want);
-    p.g.nsplit = ta_up(pages, p.g.chunk);
-    p.bytes = p.g.nsplit > 1 ? (size_t)p.g.tiles * n_kv_head * p.g.nsplit * p.mt * (p.hdp + 2) * 4 : 0;
+    p.g.cluster = pages >= 8 ? 8 : pages >= 4 ? 4 : pages >= 2 ? 2 : 1;
+    const long long tiles = (long long)p.tiles * n_kv_head;
+    p.pieces = 0;
+    if (!(pages <= 16 && tiles * p.g.cluster <= sms) && tiles * slot_pages <= 0x7fffffff)
+        p.pieces = (p.hdp == 64 && !f32 ? 3 : p.hdp <= 128 ? 2 : 1) * sms;
     return p;
 }
 
@@ -642,16 +960,35 @@ int ta_run(const ec_kv_pages &kv, const ec_tree_attn &a, const TaPlan &p, int id
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return (int)e;
-    auto kern = k_tree_mma<QT, KT, HDP, WM, WN, STAGES>;
+    auto pieces = k_tree_mma<QT, KT, HDP, WM, WN, STAGES, true>;
+    auto shared = k_tree_mma<QT, KT, HDP, WM, WN, STAGES, false>;
     if (!g_attr[id][dev]) {
-        e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+        e = cudaFuncSetAttribute(pieces, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+        if (e == cudaSuccess) e = cudaFuncSetAttribute(shared, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
         if (e != cudaSuccess) return (int)e;
         g_attr[id][dev] = 1;
     }
-    kern<<<dim3(p.g.tiles, p.g.nsplit, a.n_kv_head), C::THREADS, C::SMEM, stream>>>(kv, a, p.g, err);
-    e = cudaGetLastError();
-    if (e != cudaSuccess || p.g.nsplit == 1) return (int)e;
-    return (int)ec_launch_k(k_tree_join<QT>, dim3(p.g.tiles, ta_up(p.mt, 4), a.n_kv_head), dim3(128), 0, stream, kv, a, p.g, p.mt, p.hdp, err);
+    if (p.pieces) {
+        pieces<<<p.pieces, C::THREADS, C::SMEM, stream>>>(kv, a, p.g, err);
+        e = cudaGetLastError();
+        if (e != cudaSuccess || p.pieces == 1) return (int)e;
+        const long long tiles = (long long)p.tiles * a.n_kv_head;
+        if (4 * tiles <= p.pieces && p.pieces <= TJ_PIECES)
+            return (int)ec_launch_k(k_tree_join<QT, HDP, true>, dim3((unsigned)tiles, p.mt), dim3(TJ_THREADS), 0, stream, kv, a, p.g, p.mt, p.pieces, 1.0f / C::Ty::PARTS, err);
+        return (int)ec_launch_k(k_tree_join<QT, HDP, false>, dim3(p.pieces - 1, 2), dim3(TJ_THREADS), 0, stream, kv, a, p.g, p.mt, p.pieces, 1.0f / C::Ty::PARTS, err);
+    }
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(p.tiles, p.g.cluster, a.n_kv_head);
+    cfg.blockDim = dim3(C::THREADS);
+    cfg.dynamicSmemBytes = C::SMEM;
+    cfg.stream = stream;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = at[0].val.clusterDim.z = 1;
+    at[0].val.clusterDim.y = (unsigned)p.g.cluster;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    return (int)cudaLaunchKernelEx(&cfg, shared, kv, a, p.g, err);
 }
 
 template <int QT, int KT, int HDP, int STAGES>
@@ -664,25 +1001,23 @@ int ta_rows(const ec_kv_pages &kv, const ec_tree_attn &a, const TaPlan &p, int i
 template <int QT, int KT>
 int ta_dims(const ec_kv_pages &kv, const ec_tree_attn &a, const TaPlan &p, int id, int *err, cudaStream_t stream) {
     if (p.hdp == 64) return ta_rows<QT, KT, 64, 4>(kv, a, p, id, err, stream);
-    if (p.hdp == 128) return ta_rows<QT, KT, 128, 3>(kv, a, p, id + 3, err, stream);
+    if (p.hdp == 128) return ta_rows<QT, KT, 128, QT == EC_T_F32 ? 2 : 3>(kv, a, p, id + 3, err, stream);
     return ta_rows<QT, KT, 256, 2>(kv, a, p, id + 6, err, stream);
 }
 
 }  // namespace
 
 extern "C" size_t ec_tree_attention_bytes(int n_seq, int rows, int n_head, int n_kv_head, int head_dim, int max_len, int num_sms) {
-    return ta_plan(n_seq, rows, n_head, n_kv_head, head_dim, max_len, 0, num_sms).bytes;
+    const TaPlan p = ta_plan(n_seq, rows, n_head, n_kv_head, head_dim, max_len, 1, 0, false, num_sms);
+    return p.pieces * ta_piece_bytes(p);
 }
 
 extern "C" int ec_launch_tree_attention(const ec_kv_pages *kv, const ec_tree_attn *a, int num_sms, int *err, cudaStream_t stream) {
     long long len = a->max_len > 0 ? a->max_len : (long long)kv->pages_per_slot * PAGE;
-    TaPlan p = ta_plan(a->n_seq, a->rows, a->n_head, a->n_kv_head, a->head_dim, (int)(len < 0x7fffffff - PAGE ? len : 0x7fffffff - PAGE), a->window, num_sms);
-    const size_t one = (size_t)p.g.tiles * a->n_kv_head * p.mt * (p.hdp + 2) * 4;   // partial sums of one split of everything
-    if (p.g.nsplit > 1 && (!a->work || a->work_bytes < p.bytes)) {
-        const size_t fit = a->work ? a->work_bytes / one : 0;
-        const int pages = p.g.chunk * p.g.nsplit;
-        p.g.nsplit = fit > 1 ? (int)fit : 1;
-        p.g.chunk = ta_up(pages, p.g.nsplit);
+    TaPlan p = ta_plan(a->n_seq, a->rows, a->n_head, a->n_kv_head, a->head_dim, (int)(len < 0x7fffffff - PAGE ? len : 0x7fffffff - PAGE), kv->pages_per_slot, a->window, a->type == EC_T_F32, num_sms);
+    if (p.pieces) {
+        const size_t fit = a->work ? a->work_bytes / ta_piece_bytes(p) : 0;
+        if (fit < (size_t)p.pieces) p.pieces = fit > 1 ? (int)fit : 0;
     }
     p.g.scale2 = (a->scale > 0.0f ? a->scale : 1.0f / sqrtf((float)a->head_dim)) * LOG2E;
     p.g.part = static_cast<float *>(a->work);
