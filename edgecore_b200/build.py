@@ -26,10 +26,11 @@ LIB = PKG / "libedgecore_b200.so"
 CUDA = Path(os.environ.get("CUDA_HOME", "/usr/local/cuda"))
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
-CU_SOURCES = ["ec_kernels.cu", "ec_decode.cu", "ec_tc.cu", "ec_noalloc.cu", "ec_tree.cu", "ec_pages.cu",
-              "ec_sample.cu"]
+CU_SOURCES = ["ec_kernels.cu", "ec_decode.cu", "ec_tc.cu", "ec_noalloc.cu", "ec_tree.cu", "ec_tree_tc.cu",
+              "ec_pages.cu", "ec_sample.cu"]
 C_SOURCES = ["ec_host.c", "ec_abi.c", "ec_serve.c"]
-HEADERS = [CSRC / "ec_launch.h", CSRC / "ec_common.cuh", CSRC / "ec_decode.h", CSRC / "ec_serve.h", ROOT / "include" / "edgecore.h",
+HEADERS = [CSRC / "ec_launch.h", CSRC / "ec_common.cuh", CSRC / "ec_decode.h", CSRC / "ec_serve.h",
+           CSRC / "ec_tree.cuh", ROOT / "include" / "edgecore.h",
            ROOT / "include" / "edgecore_b200.h"]
 
 

@@ -13,224 +13,13 @@
 // tiles, one after the other, into equal pieces, one per resident CTA, so that
 // ragged sequences keep every SM busy to the end, and k_tree_join adds up the
 // tiles that a border cuts, in the order of their pages.
-#include "ec_common.cuh"
-#include "ec_serve.h"
+#include "ec_tree.cuh"
 
 #include <cooperative_groups.h>
 
 namespace cg = cooperative_groups;
 
 namespace {
-
-constexpr float LOG2E = 1.4426950408889634f;
-constexpr int PAGE = EC_KV_PAGE;
-
-// ---- the work of a call ------------------------------------------------------
-
-struct TaGeo {            // chosen by the launcher
-    int group;            // query heads per KV head
-    unsigned div_mul;     // row / group = (row * div_mul) >> div_shift for rows below 2^30 (group > 1)
-    int div_shift;
-    int cluster;          // CTAs of a cluster that share a tile's pages
-    float scale2;         // scale * log2 e
-    float *part;          // pieces: [CTA][2][MT][hdp] o, then [CTA][2][MT] (m, l)
-};
-
-EC_DEV int ta_node(const TaGeo &g, int row) {
-    return g.group == 1 ? row : (int)(((unsigned long long)(unsigned)row * g.div_mul) >> g.div_shift);
-}
-
-struct TaTile {           // one row tile of one KV head
-    int first;            // its first row in the sequence's (node, head) numbering
-    int kh;
-    int r0, t, base, slot;
-    int page0, page1;     // pages that hold visible positions
-};
-
-struct TaSeq {            // a sequence, in the lane that holds it
-    int r0, t, base, slot, page0, pages, tiles;   // a bad one has no tiles
-};
-
-EC_DEV TaSeq ta_seq(const ec_kv_pages &kv, const ec_tree_attn &a, const TaGeo &g, int mt, int i, int *err) {
-    TaSeq q = {};
-    if (i >= a.n_seq) return q;
-    q.r0 = a.row_start[i];
-    const long long t = (long long)a.row_start[i + 1] - q.r0;
-    q.base = a.base[i];
-    q.slot = a.slots ? a.slots[i] : i;
-    if (q.r0 < 0 || t < 0 || q.r0 + t > a.rows || q.base < 0 || q.slot < 0 || q.slot >= kv.n_slots ||
-        q.base + t > (long long)kv.pages_per_slot * PAGE) {
-        atomicCAS(err, 0, EC_KERR_BAD_INDEX);
-        return q;
-    }
-    q.t = (int)t;
-    q.tiles = (int)((t * g.group + mt - 1) / mt);
-    const int lo = a.window > 0 && q.base > a.window ? q.base - a.window : 0;   // no row sees a position below it
-    q.page0 = lo / PAGE;
-    q.pages = (q.base + q.t + PAGE - 1) / PAGE - q.page0;
-    return q;
-}
-
-EC_DEV TaTile ta_tile(const TaSeq &q, int l, int tile, int kh, int mt) {   // from the sequence that lane l holds
-    TaTile s;
-    s.first = tile * mt;
-    s.kh = kh;
-    s.r0 = __shfl_sync(0xffffffffu, q.r0, l);
-    s.t = __shfl_sync(0xffffffffu, q.t, l);
-    s.base = __shfl_sync(0xffffffffu, q.base, l);
-    s.slot = __shfl_sync(0xffffffffu, q.slot, l);
-    s.page0 = __shfl_sync(0xffffffffu, q.page0, l);
-    s.page1 = s.page0 + __shfl_sync(0xffffffffu, q.pages, l);
-    return s;
-}
-
-EC_DEV int ta_scan(int v) {   // inclusive, over the warp
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const int u = __shfl_up_sync(0xffffffffu, v, o);
-        if ((int)(threadIdx.x & 31) >= o) v += u;
-    }
-    return v;
-}
-
-// The row tile `ti` in the sequences' order; false when there is none.  Called
-// by whole warps.
-EC_DEV bool ta_find(const ec_kv_pages &kv, const ec_tree_attn &a, const TaGeo &g, int ti, int kh, int mt, TaTile &s, int *err) {
-    int before = 0;
-    for (int b0 = 0; b0 < a.n_seq; b0 += 32) {
-        const TaSeq q = ta_seq(kv, a, g, mt, b0 + (threadIdx.x & 31), err);
-        const int sum = before + ta_scan(q.tiles);
-        const unsigned hit = __ballot_sync(0xffffffffu, sum > ti);
-        if (hit) {
-            const int l = __ffs((int)hit) - 1;
-            s = ta_tile(q, l, ti - __shfl_sync(0xffffffffu, sum - q.tiles, l), kh, mt);
-            return true;
-        }
-        before = __shfl_sync(0xffffffffu, sum, 31);
-    }
-    return false;
-}
-
-// The pages of all tiles in one line (below 2^31 of them, ta_plan): sequence
-// by sequence, KV head by KV head, tile by tile.  CTA i of the first n takes
-// [start(i), start(i + 1)), at least a page each.
-struct TaLine {
-    TaSeq head;           // sequence of this lane among the first 32
-    int n, total, per, more;   // the first `more` pieces have per + 1 pages
-
-    EC_DEV static int work(const TaSeq &q, int kvh) { return q.tiles * q.pages * kvh; }
-    EC_DEV void init(const ec_kv_pages &kv, const ec_tree_attn &a, const TaGeo &g, int mt, int pieces, int *err) {
-        head = ta_seq(kv, a, g, mt, threadIdx.x & 31, err);
-        total = __reduce_add_sync(0xffffffffu, work(head, a.n_kv_head));
-        for (int b0 = 32; b0 < a.n_seq; b0 += 32)
-            total += __reduce_add_sync(0xffffffffu, work(ta_seq(kv, a, g, mt, b0 + (threadIdx.x & 31), err), a.n_kv_head));
-        n = min(pieces, total);
-        per = n ? total / n : 0;
-        more = total - per * n;
-    }
-    EC_DEV int start(int i) const { return per * i + min(i, more); }
-    EC_DEV int piece(int at) const {
-        const int wide = (per + 1) * more;
-        return at < wide ? at / (per + 1) : more + (at - wide) / per;
-    }
-    // the tile that holds place `at` (below total), and where it begins
-    EC_DEV TaTile tile(const ec_kv_pages &kv, const ec_tree_attn &a, const TaGeo &g, int mt, int at, int &begin, int *err) const {
-        int before = 0;
-        TaSeq q = head;
-        for (int b0 = 0;; b0 += 32) {
-            if (b0) q = ta_seq(kv, a, g, mt, b0 + (threadIdx.x & 31), err);
-            const int w = work(q, a.n_kv_head), sum = before + ta_scan(w);
-            const unsigned hit = __ballot_sync(0xffffffffu, sum > at);
-            if (hit || b0 + 32 >= a.n_seq) {
-                const int l = hit ? __ffs((int)hit) - 1 : 0;
-                const int from = __shfl_sync(0xffffffffu, sum - w, l);
-                const int pages = max(1, __shfl_sync(0xffffffffu, q.pages, l)), tiles = max(1, __shfl_sync(0xffffffffu, q.tiles, l));
-                const int unit = (at - from) / pages, kh = unit / tiles;
-                begin = from + unit * pages;
-                return ta_tile(q, l, unit - kh * tiles, kh, mt);
-            }
-            before = __shfl_sync(0xffffffffu, sum, 31);
-        }
-    }
-    // the tile number `index` of all, in the order of the line; false: none
-    EC_DEV bool by_index(const ec_kv_pages &kv, const ec_tree_attn &a, const TaGeo &g, int mt, int index, TaTile &s, int &begin, int *err) const {
-        int units = 0, before = 0;
-        TaSeq q = head;
-        for (int b0 = 0; b0 < a.n_seq; b0 += 32) {
-            if (b0) q = ta_seq(kv, a, g, mt, b0 + (threadIdx.x & 31), err);
-            const int w = work(q, a.n_kv_head), u = q.tiles * a.n_kv_head, ws = before + ta_scan(w), us = units + ta_scan(u);
-            const unsigned hit = __ballot_sync(0xffffffffu, us > index);
-            if (hit) {
-                const int l = __ffs((int)hit) - 1, unit = index - __shfl_sync(0xffffffffu, us - u, l);
-                const int tiles = __shfl_sync(0xffffffffu, q.tiles, l), kh = unit / tiles;
-                begin = __shfl_sync(0xffffffffu, ws - w, l) + unit * __shfl_sync(0xffffffffu, q.pages, l);
-                s = ta_tile(q, l, unit - kh * tiles, kh, mt);
-                return true;
-            }
-            before = __shfl_sync(0xffffffffu, ws, 31);
-            units = __shfl_sync(0xffffffffu, us, 31);
-        }
-        return false;
-    }
-};
-
-EC_DEV int ta_page(const ec_kv_pages &kv, int slot, int i, int *err) {
-    int page = __ldg(kv.page_table + (size_t)slot * kv.pages_per_slot + i);
-    if (page < 0 || page >= kv.n_pages) {
-        if ((threadIdx.x & 31) == 0) atomicCAS(err, 0, EC_KERR_BAD_INDEX);
-        page = 0;
-    }
-    return page;
-}
-
-EC_DEV int ta_depth(const ec_tree_attn &a, int row) {
-    int d = -1;
-    for (int w = 0; w < a.mask_words; ++w) d += __popcll(a.mask[(size_t)row * a.mask_words + w]);
-    return d;
-}
-
-EC_DEV unsigned long long ta_low(int n) { return n <= 0 ? 0ull : n >= 64 ? ~0ull : (1ull << n) - 1ull; }
-
-// Which of the 64 positions from p0 on the node `i` of the tile's sequence
-// sees, one bit each.
-EC_DEV unsigned long long ta_allow(const ec_tree_attn &a, const TaTile &s, int i, int p0) {
-    if (i >= s.t) return 0ull;
-    const int row = s.r0 + i, j0 = p0 - s.base;
-    const unsigned long long *m = a.mask + (size_t)row * a.mask_words;
-    unsigned long long tree = 0;
-    if (j0 < 0) {
-        if (j0 > -64) tree = m[0] << -j0;
-    } else {
-        const int w = j0 / 64, sh = j0 % 64;
-        if (w < a.mask_words) tree = m[w] >> sh;
-        if (sh && w + 1 < a.mask_words) tree |= m[w + 1] << (64 - sh);
-    }
-    const unsigned long long prefix = ta_low(s.base - p0);
-    tree &= ta_low(s.base + s.t - p0) & ~prefix;
-    if (a.window <= 0) return prefix | tree;
-    const int depth = ta_depth(a, row);
-    const int from = s.base + depth - a.window + 1;
-    if (a.window < 64 * a.mask_words)   // nodes of one tree are fewer levels apart than that
-        for (unsigned long long left = tree; left; left &= left - 1) {
-            const int bit = __ffsll((long long)left) - 1;
-            if (s.base + ta_depth(a, s.r0 + j0 + bit) < from) tree &= ~(1ull << bit);
-        }
-    return (prefix & ~ta_low(from - p0)) | tree;
-}
-
-template <int T> EC_DEV void ta_store2(void *p, size_t i, float x, float y, bool pair) {   // pair: i even and aligned
-    if (T == EC_T_F32) {
-        float *o = static_cast<float *>(p) + i;
-        if (pair) *reinterpret_cast<float2 *>(o) = make_float2(x, y);
-        else { o[0] = x; o[1] = y; }
-    } else {
-        uint16_t *o = static_cast<uint16_t *>(p) + i;
-        const uint16_t a = T == EC_T_F16 ? __half_as_ushort(__float2half_rn(x)) : __bfloat16_as_ushort(__float2bfloat16_rn(x));
-        const uint16_t b = T == EC_T_F16 ? __half_as_ushort(__float2half_rn(y)) : __bfloat16_as_ushort(__float2bfloat16_rn(y));
-        if (pair) *reinterpret_cast<uint32_t *>(o) = (uint32_t)a | (uint32_t)b << 16;
-        else { o[0] = a; o[1] = b; }
-    }
-}
 
 // ---- register tiles ------------------------------------------------------------
 
@@ -250,29 +39,11 @@ template <bool BF> EC_DEV void mma16816(float (&c)[4], const uint32_t (&a)[4], u
         asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-EC_DEV float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
 EC_DEV void cp16(uint32_t dst, const void *src, bool real) {   // 16 bytes, or zeros
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(real ? 16 : 0) : "memory");
 }
 EC_DEV void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> EC_DEV void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-
-template <bool BF> EC_DEV uint32_t pack2(float x, float y) {
-    if (BF) {
-        const __nv_bfloat162 v = __floats2bfloat162_rn(x, y);
-        return *reinterpret_cast<const uint32_t *>(&v);
-    }
-    const __half2 v = __floats2half2_rn(x, y);
-    return *reinterpret_cast<const uint32_t *>(&v);
-}
-template <bool BF> EC_DEV float2 unpack2(uint32_t u) {
-    if (BF) return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
-    return __half22float2(*reinterpret_cast<const __half2 *>(&u));
-}
 
 // Byte address of 16-byte chunk c of row r in a tile of rows of HDP 16-bit
 // elements: chunks are exchanged within groups of eight so that the eight
@@ -930,7 +701,7 @@ size_t ta_piece_bytes(const TaPlan &p) { return (size_t)2 * p.mt * (p.hdp + 2) *
 // Clusters where they alone give every SM something to do or a tile has few
 // pages: one launch (one token over 300 positions: 7.2 us, in pieces 9.5).
 // Otherwise as many pieces as CTAs are resident.
-TaPlan ta_plan(int n_seq, int rows, int n_head, int n_kv_head, int hd, int max_len, int slot_pages, int window, bool f32, int sms) {
+TaPlan ta_plan(int n_seq, int rows, int n_head, int n_kv_head, int hd, int max_len, int slot_pages, int window, bool f32, bool tc, int sms) {
     TaPlan p;
     p.hdp = hd <= 64 ? 64 : hd <= 128 ? 128 : 256;
     p.g.group = n_head / n_kv_head;
@@ -939,7 +710,8 @@ TaPlan ta_plan(int n_seq, int rows, int n_head, int n_kv_head, int hd, int max_l
     p.g.div_shift = 30 + up;   // rounded up: exact for rows below 2^30
     p.g.div_mul = (unsigned)(((1ull << p.g.div_shift) + p.g.group - 1) / p.g.group);
     const int mean = (int)(((long long)rows * p.g.group + n_seq - 1) / n_seq);
-    p.mt = mean <= 16 ? 16 : mean <= 32 ? 32 : 64;
+    // from 65 rows on, tiles of 128 on the tensor cores of tcgen05
+    p.mt = mean <= 16 ? 16 : mean <= 32 ? 32 : mean <= 64 || !tc ? 64 : TC_ROWS;
     p.tiles = (int)(((long long)rows * p.g.group) / p.mt + n_seq);   // every sequence rounds up once; rows * group fits 31 bits
     int pages = ta_up(max_len > 0 ? max_len : 1, PAGE);
     if (window > 0 && pages > window / PAGE + 2) pages = window / PAGE + 2;
@@ -947,11 +719,23 @@ TaPlan ta_plan(int n_seq, int rows, int n_head, int n_kv_head, int hd, int max_l
     const long long tiles = (long long)p.tiles * n_kv_head;
     p.pieces = 0;
     if (!(pages <= 16 && tiles * p.g.cluster <= sms) && tiles * slot_pages <= 0x7fffffff)
-        p.pieces = (p.hdp == 64 && !f32 ? 3 : p.hdp <= 128 ? 2 : 1) * sms;
+        p.pieces = (p.mt == TC_ROWS ? 2 : p.hdp == 64 && !f32 ? 3 : p.hdp <= 128 ? 2 : 1) * sms;
+    if (!p.pieces && p.mt == TC_ROWS) {   // clusters: the register tiles only
+        p.mt = 64;
+        p.tiles = (int)(((long long)rows * p.g.group) / p.mt + n_seq);
+    }
     return p;
 }
 
 int g_attr[64][64];
+
+template <int QT, int HDP>
+int ta_join(const ec_kv_pages &kv, const ec_tree_attn &a, const TaPlan &p, float unit, int *err, cudaStream_t stream) {
+    const long long tiles = (long long)p.tiles * a.n_kv_head;
+    if (4 * tiles <= p.pieces && p.pieces <= TJ_PIECES)
+        return (int)ec_launch_k(k_tree_join<QT, HDP, true>, dim3((unsigned)tiles, p.mt), dim3(TJ_THREADS), 0, stream, kv, a, p.g, p.mt, p.pieces, unit, err);
+    return (int)ec_launch_k(k_tree_join<QT, HDP, false>, dim3(p.pieces - 1, 2), dim3(TJ_THREADS), 0, stream, kv, a, p.g, p.mt, p.pieces, unit, err);
+}
 
 template <int QT, int KT, int HDP, int WM, int WN, int STAGES>
 int ta_run(const ec_kv_pages &kv, const ec_tree_attn &a, const TaPlan &p, int id, int *err, cudaStream_t stream) {
@@ -972,10 +756,7 @@ int ta_run(const ec_kv_pages &kv, const ec_tree_attn &a, const TaPlan &p, int id
         pieces<<<p.pieces, C::THREADS, C::SMEM, stream>>>(kv, a, p.g, err);
         e = cudaGetLastError();
         if (e != cudaSuccess || p.pieces == 1) return (int)e;
-        const long long tiles = (long long)p.tiles * a.n_kv_head;
-        if (4 * tiles <= p.pieces && p.pieces <= TJ_PIECES)
-            return (int)ec_launch_k(k_tree_join<QT, HDP, true>, dim3((unsigned)tiles, p.mt), dim3(TJ_THREADS), 0, stream, kv, a, p.g, p.mt, p.pieces, 1.0f / C::Ty::PARTS, err);
-        return (int)ec_launch_k(k_tree_join<QT, HDP, false>, dim3(p.pieces - 1, 2), dim3(TJ_THREADS), 0, stream, kv, a, p.g, p.mt, p.pieces, 1.0f / C::Ty::PARTS, err);
+        return ta_join<QT, HDP>(kv, a, p, 1.0f / C::Ty::PARTS, err, stream);
     }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(p.tiles, p.g.cluster, a.n_kv_head);
@@ -1008,20 +789,31 @@ int ta_dims(const ec_kv_pages &kv, const ec_tree_attn &a, const TaPlan &p, int i
 }  // namespace
 
 extern "C" size_t ec_tree_attention_bytes(int n_seq, int rows, int n_head, int n_kv_head, int head_dim, int max_len, int num_sms) {
-    const TaPlan p = ta_plan(n_seq, rows, n_head, n_kv_head, head_dim, max_len, 1, 0, false, num_sms);
+    const TaPlan p = ta_plan(n_seq, rows, n_head, n_kv_head, head_dim, max_len, 1, 0, false, head_dim == 64 || head_dim == 128, num_sms);
     return p.pieces * ta_piece_bytes(p);
 }
 
 extern "C" int ec_launch_tree_attention(const ec_kv_pages *kv, const ec_tree_attn *a, int num_sms, int *err, cudaStream_t stream) {
     long long len = a->max_len > 0 ? a->max_len : (long long)kv->pages_per_slot * PAGE;
-    TaPlan p = ta_plan(a->n_seq, a->rows, a->n_head, a->n_kv_head, a->head_dim, (int)(len < 0x7fffffff - PAGE ? len : 0x7fffffff - PAGE), kv->pages_per_slot, a->window, a->type == EC_T_F32, num_sms);
+    TaPlan p = ta_plan(a->n_seq, a->rows, a->n_head, a->n_kv_head, a->head_dim, (int)(len < 0x7fffffff - PAGE ? len : 0x7fffffff - PAGE), kv->pages_per_slot, a->window, a->type == EC_T_F32,
+                       ta_tc_takes(a->type, kv->type, a->head_dim), num_sms);
     if (p.pieces) {
         const size_t fit = a->work ? a->work_bytes / ta_piece_bytes(p) : 0;
         if (fit < (size_t)p.pieces) p.pieces = fit > 1 ? (int)fit : 0;
+        if (!p.pieces && p.mt == TC_ROWS) {
+            p.mt = 64;
+            p.tiles = (int)(((long long)a->rows * p.g.group) / p.mt + a->n_seq);
+        }
     }
     p.g.scale2 = (a->scale > 0.0f ? a->scale : 1.0f / sqrtf((float)a->head_dim)) * LOG2E;
     p.g.part = static_cast<float *>(a->work);
     const bool bf = kv->type == EC_T_BF16;
+    if (p.mt == TC_ROWS) {
+        const int e = ta_tc_launch(*kv, *a, p.g, p.pieces, err, stream);
+        if (e) return e;
+        if (p.hdp == 64) return bf ? ta_join<EC_T_BF16, 64>(*kv, *a, p, 1.0f, err, stream) : ta_join<EC_T_F16, 64>(*kv, *a, p, 1.0f, err, stream);
+        return bf ? ta_join<EC_T_BF16, 128>(*kv, *a, p, 1.0f, err, stream) : ta_join<EC_T_F16, 128>(*kv, *a, p, 1.0f, err, stream);
+    }
     if (a->type == EC_T_F32) return bf ? ta_dims<EC_T_F32, EC_T_BF16>(*kv, *a, p, 0, err, stream) : ta_dims<EC_T_F32, EC_T_F16>(*kv, *a, p, 9, err, stream);
     return bf ? ta_dims<EC_T_BF16, EC_T_BF16>(*kv, *a, p, 18, err, stream) : ta_dims<EC_T_F16, EC_T_F16>(*kv, *a, p, 27, err, stream);
 }

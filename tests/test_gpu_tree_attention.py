@@ -67,12 +67,12 @@ class Case:
     def dev(self, a):
         return self.torch.from_numpy(np.ascontiguousarray(a)).cuda()
 
-    def run(self, work_bytes=1 << 24, scale=0.0, **kw):
+    def run(self, work_bytes=1 << 26, scale=0.0, max_len=None, **kw):
         work = self.torch.empty(work_bytes, dtype=self.torch.uint8, device="cuda") if work_bytes else None
         ec.tree_attention(kw.pop("out", self.out), kw.pop("q", self.q), kw.pop("k", self.k), kw.pop("v", self.v), self.dev(self.table),
                           self.dev(self.start), self.dev(np.array(self.bases, np.int32)), self.dev(self.mask.view(np.int64)),
                           slots=self.dev(self.slots), window=self.window, scale=scale, workspace=work,
-                          max_len=max(b + t for b, t in zip(self.bases, self.sizes)), **kw)
+                          max_len=max_len or max(b + t for b, t in zip(self.bases, self.sizes)), **kw)
         self.torch.cuda.synchronize()
         assert ec.device_error_take() == 0
         return kw.get("out", self.out)
@@ -195,6 +195,85 @@ def test_window_hides_infinities(cuda):
     got = c.out.double().cpu().numpy()
     assert (np.abs(got - want) <= tol)[1:].all()
     assert not np.isfinite(got[0]).all()
+
+
+# max_len only steers how the work is laid out: FAR makes short caches take the path of long ones (equal pieces of the
+# pages, and tiles of 128 rows on tcgen05 from 65 rows on a KV head).
+FAR = 1 << 20
+
+
+@pytest.mark.parametrize("q,kv", [("f16", "f16"), ("bf16", "bf16"), ("f32", "f16"), ("f32", "bf16")])
+@pytest.mark.parametrize("heads,kv_heads,hd", [(14, 2, 64), (12, 2, 128), (6, 6, 64), (8, 1, 128), (3, 1, 80), (4, 2, 256)])
+@pytest.mark.parametrize("sizes,bases", [((64,), (1000,)), ((130, 70), (300, 64)), ((1, 40, 0, 9), (0, 63, 5, 128)), ((100,) * 3, (1, 0, 65))])
+def test_pieces(cuda, q, kv, heads, kv_heads, hd, sizes, bases):
+    c = Case(cuda, q, kv, heads, kv_heads, hd, sizes=sizes, bases=bases, seed=hd + len(sizes))
+    c.run(max_len=FAR)
+    c.check()
+
+
+@pytest.mark.parametrize("window", [1, 2, 7, 64, 100, 1000])
+@pytest.mark.parametrize("q,kv", [("f16", "f16"), ("bf16", "bf16"), ("f32", "f16")])
+def test_pieces_window(cuda, window, q, kv):
+    c = Case(cuda, q, kv, 8, 1, 64, sizes=(12, 1, 70), bases=(200, 5, 64), window=window, seed=window)
+    c.run(max_len=FAR)
+    c.check()
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("q,kv", [("f16", "f16"), ("bf16", "bf16"), ("f32", "f16")])
+def test_pieces_hidden_infinities(cuda, bad, q, kv, hd):
+    """A branch that holds `bad` in K and V, in the first page of its tile and in a later one."""
+    for base in (0, 70, 200):
+        parents = [-1, 0, 0, 1, 2, 3] + [3] * 20
+        c = Case(cuda, q, kv, 8, 1, hd, sizes=(26,), bases=(base,), mask=ec.tree_mask(parents).view(np.uint64), seed=6)
+        want, tol = c.expect()
+        page, off = c.table[c.slots[0], (base + 2) // 64], (base + 2) % 64
+        c.k[page, off] = bad
+        c.v[page, off] = bad
+        c.run(max_len=FAR)
+        got = c.out.double().cpu().numpy()
+        clean = [i for i in range(26) if i not in (2, 4)]
+        assert (np.abs(got - want) <= tol)[clean].all()
+        assert not np.isfinite(got[[2, 4]]).all()
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+def test_infinity_in_v_reaches_the_rows_that_see_it(cuda, hd):
+    """+inf in one element of V: that element of the rows that see it is +inf, everything else as before."""
+    for max_len in (None, FAR):
+        c = Case(cuda, "f16", "f16", 8, 1, hd, sizes=(20,), bases=(100,), mask=ec.tree_mask([-1] + [0] * 19).view(np.uint64), seed=7)
+        want, tol = c.expect()
+        c.v[c.table[c.slots[0], 107 // 64], 107 % 64, 0, 5] = math.inf      # node 7 is seen by itself alone
+        c.run(max_len=max_len)
+        got = c.out.double().cpu().numpy().reshape(20, 8, hd)
+        assert (got[7, :, 5] == math.inf).all()
+        got[7, :, 5] = want.reshape(20, 8, hd)[7, :, 5]
+        assert (np.abs(got.reshape(20, -1) - want) <= tol).all()
+
+
+def test_pieces_many_sequences_and_growing_maxima(cuda):
+    """70 ragged sequences; keys that grow along the cache, so that a row's maximum rises page by page."""
+    rs = np.random.RandomState(15)
+    sizes, bases = rs.randint(0, 25, 70), rs.randint(0, 260, 70)
+    for q, kv in (("f16", "f16"), ("bf16", "bf16"), ("f32", "f16")):
+        c = Case(cuda, q, kv, 8, 1, 64, sizes=sizes.tolist(), bases=bases.tolist(), seed=16)
+        pos = cuda.arange(64, device="cuda")[None, :, None, None]
+        c.k.mul_((1 + pos / 8).to(c.k.dtype))
+        c.run(max_len=FAR)
+        c.check()
+        c.run()
+        c.check()
+
+
+def test_pieces_little_work_and_small_workspaces(cuda):
+    for bytes_ in (1 << 17, 1 << 19, 1 << 21, 1 << 26):
+        c = Case(cuda, "bf16", "bf16", 12, 2, 128, sizes=(30, 7), bases=(700, 90), seed=17)
+        c.run(bytes_, max_len=FAR)
+        c.check()
+    c = Case(cuda, "f16", "f16", 8, 1, 64, sizes=(9,), bases=(3,), seed=18)
+    c.run(max_len=FAR)
+    c.check()
 
 
 def test_strides_three_dimensions_and_rows_behind_the_last_sequence(cuda):
