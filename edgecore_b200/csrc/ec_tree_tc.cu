@@ -35,9 +35,9 @@ template <int QT, int KT, int HD> struct TtCfg {
     static constexpr bool BF = KT == EC_T_BF16;
     static constexpr int COLS = HD / 64;               // 128-byte columns of a row
     static constexpr int TILE = 64 * HD * 2;           // K or V of a page
-    static constexpr int STAGES = HD == 64 ? 4 : 2;
+    static constexpr int KS = HD == 64 ? 5 : 3, VS = HD == 64 ? 4 : 2;   // pages of K and of V in flight: K is free once S is done
     static constexpr int Q_BYTES = TT_ROWS * HD * 2;
-    static constexpr int SMEM = Q_BYTES + STAGES * 2 * TILE + 256;
+    static constexpr int SMEM = Q_BYTES + (KS + VS) * TILE + 256;
     static constexpr int TMEM = 256;                   // S 2 x 64, O up to 128 columns: two CTAs share an SM's 512
     static constexpr float LIFT = BF ? 0.0f : 6.0f;
     static constexpr uint32_t TYPES = (1u << 4) | ((BF ? 1u : 0u) << 7) | ((BF ? 1u : 0u) << 10) | ((uint32_t)(TT_ROWS >> 4) << 24);
@@ -67,24 +67,36 @@ EC_DEV void tt_commit(uint64_t *bar) {
 EC_DEV void tt_arrive(uint64_t *bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(ec_smem_u32(bar)) : "memory"); }
 EC_DEV void tt_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 EC_DEV void tt_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-EC_DEV void tt_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 EC_DEV void tt_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 EC_DEV void tt_proxy() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
-#define TT_R32(r, b) r[b + 0], r[b + 1], r[b + 2], r[b + 3], r[b + 4], r[b + 5], r[b + 6], r[b + 7], r[b + 8], r[b + 9], r[b + 10], r[b + 11], r[b + 12], r[b + 13], r[b + 14], r[b + 15]
-// 32 columns of this thread's row
-EC_DEV void tt_ld32(uint32_t taddr, float *f) {
-    uint32_t r[32];
+// 64 or 32 columns of this thread's row, arrived (the wait is part of the
+// statement: nothing may use the registers before it)
+EC_DEV void tt_ld64(uint32_t taddr, float *f) {
     __syncwarp();   // a whole warp executes these as one
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, "
-                 "%26, %27, %28, %29, %30, %31}, [%32];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
-                   "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]),
-                   "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-                 : "r"(taddr));
-    tt_wait_ld();
-#pragma unroll
-    for (int i = 0; i < 32; ++i) f[i] = __uint_as_float(r[i]);
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x64.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, "
+                 "%30, %31, %32, %33, %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47, %48, %49, %50, %51, %52, %53, %54, %55, %56, %57, "
+                 "%58, %59, %60, %61, %62, %63}, [%64];\n\t"
+                 "tcgen05.wait::ld.sync.aligned;"
+                 : "=f"(f[0]), "=f"(f[1]), "=f"(f[2]), "=f"(f[3]), "=f"(f[4]), "=f"(f[5]), "=f"(f[6]), "=f"(f[7]), "=f"(f[8]), "=f"(f[9]), "=f"(f[10]),
+                   "=f"(f[11]), "=f"(f[12]), "=f"(f[13]), "=f"(f[14]), "=f"(f[15]), "=f"(f[16]), "=f"(f[17]), "=f"(f[18]), "=f"(f[19]), "=f"(f[20]),
+                   "=f"(f[21]), "=f"(f[22]), "=f"(f[23]), "=f"(f[24]), "=f"(f[25]), "=f"(f[26]), "=f"(f[27]), "=f"(f[28]), "=f"(f[29]), "=f"(f[30]),
+                   "=f"(f[31]), "=f"(f[32]), "=f"(f[33]), "=f"(f[34]), "=f"(f[35]), "=f"(f[36]), "=f"(f[37]), "=f"(f[38]), "=f"(f[39]), "=f"(f[40]),
+                   "=f"(f[41]), "=f"(f[42]), "=f"(f[43]), "=f"(f[44]), "=f"(f[45]), "=f"(f[46]), "=f"(f[47]), "=f"(f[48]), "=f"(f[49]), "=f"(f[50]),
+                   "=f"(f[51]), "=f"(f[52]), "=f"(f[53]), "=f"(f[54]), "=f"(f[55]), "=f"(f[56]), "=f"(f[57]), "=f"(f[58]), "=f"(f[59]), "=f"(f[60]),
+                   "=f"(f[61]), "=f"(f[62]), "=f"(f[63])
+                 : "r"(taddr) : "memory");
+}
+EC_DEV void tt_ld32(uint32_t taddr, float *f) {
+    __syncwarp();
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, "
+                 "%30, %31}, [%32];\n\t"
+                 "tcgen05.wait::ld.sync.aligned;"
+                 : "=f"(f[0]), "=f"(f[1]), "=f"(f[2]), "=f"(f[3]), "=f"(f[4]), "=f"(f[5]), "=f"(f[6]), "=f"(f[7]), "=f"(f[8]), "=f"(f[9]), "=f"(f[10]),
+                   "=f"(f[11]), "=f"(f[12]), "=f"(f[13]), "=f"(f[14]), "=f"(f[15]), "=f"(f[16]), "=f"(f[17]), "=f"(f[18]), "=f"(f[19]), "=f"(f[20]),
+                   "=f"(f[21]), "=f"(f[22]), "=f"(f[23]), "=f"(f[24]), "=f"(f[25]), "=f"(f[26]), "=f"(f[27]), "=f"(f[28]), "=f"(f[29]), "=f"(f[30]),
+                   "=f"(f[31])
+                 : "r"(taddr) : "memory");
 }
 EC_DEV void tt_st32(uint32_t taddr, const uint32_t *r) {
     __syncwarp();
@@ -137,20 +149,24 @@ template <int QT, int KT, int HD>
 __global__ void __launch_bounds__(TT_THREADS, 2)
 k_tree_tc(const __grid_constant__ TtMaps maps, const ec_kv_pages kv, const ec_tree_attn a, const TaGeo g, int *err) {
     typedef TtCfg<QT, KT, HD> C;
-    constexpr int STAGES = C::STAGES, TILE = C::TILE;
+    constexpr int KS = C::KS, VS = C::VS, TILE = C::TILE;
     extern __shared__ __align__(1024) unsigned char smem[];
     const uint32_t base = ec_smem_u32(smem);              // 1024-byte aligned: the kernel has no other shared memory
-    const uint32_t ring = base + C::Q_BYTES;
-    uint64_t *full = reinterpret_cast<uint64_t *>(smem + C::Q_BYTES + STAGES * 2 * TILE), *empty = full + STAGES;
-    uint64_t *s_full = empty + STAGES, *p_ready = s_full + 2, *o_done = p_ready + 2, *drain = o_done + 1;
+    const uint32_t k_ring = base + C::Q_BYTES, v_ring = k_ring + KS * TILE;
+    uint64_t *k_full = reinterpret_cast<uint64_t *>(smem + C::Q_BYTES + (KS + VS) * TILE), *k_empty = k_full + KS;
+    uint64_t *v_full = k_empty + KS, *v_empty = v_full + VS, *s_full = v_empty + VS, *p_ready = s_full + 2, *o_done = p_ready + 2, *drain = o_done + 1;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(drain + 1);
     volatile int *stop_word = reinterpret_cast<volatile int *>(tmem_slot + 1);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
     if (threadIdx.x == 0) {
-        for (int i = 0; i < STAGES; ++i) {
-            ec_mbar_init(&full[i], 1);
-            ec_mbar_init(&empty[i], 1);
+        for (int i = 0; i < KS; ++i) {
+            ec_mbar_init(&k_full[i], 1);
+            ec_mbar_init(&k_empty[i], 1);
+        }
+        for (int i = 0; i < VS; ++i) {
+            ec_mbar_init(&v_full[i], 1);
+            ec_mbar_init(&v_empty[i], 1);
         }
         for (int i = 0; i < 2; ++i) {
             ec_mbar_init(&s_full[i], 1);
@@ -176,35 +192,36 @@ k_tree_tc(const __grid_constant__ TtMaps maps, const ec_kv_pages kv, const ec_tr
     line.init(kv, a, g, TT_ROWS, gridDim.x, err);
     int at = (int)blockIdx.x < line.n ? line.start(blockIdx.x) : 0;
     const int stop_at = (int)blockIdx.x < line.n ? line.start(blockIdx.x + 1) : 0;
-    int count = 0;        // pages of this CTA so far: stage count % STAGES, S buffer count % 2
-    int issued = 0, next = 0;   // producer: loads issued, arena page of the next one
+    int count = 0;        // pages of this CTA so far: stages count % KS and % VS, S buffer count % 2
+    int k_issued = 0, v_issued = 0, next = 0;   // producer: loads issued, arena page of the next one
     while (at < stop_at) {
         int begin;
         const TaTile s = line.tile(kv, a, g, TT_ROWS, at, begin, err);
         const int p_begin = s.page0 + (at - begin), p_end = min(s.page1, p_begin + (stop_at - at)), pages = p_end - p_begin;
         const int kh = s.kh, end = s.base + s.t;
 
-        // The producer: the pages that the ring holds before the row warps are
-        // met below (it is empty: the last tile is done), the others after.
+        // The producer: what the rings hold before the row warps are met below
+        // (they are empty: the last tile is done), the rest after.
         auto produce = [&](int i0, int i1) {
             for (int i = i0; i < i1; ++i) {
-                const int n = count + i, st = n % STAGES, page = next;
+                const int n = count + i, ks = n % KS, vs = n % VS, page = next;
                 if (i + 1 < pages) next = ta_page(kv, s.slot, p_begin + i + 1, err);
-                if (n >= STAGES && !tt_wait(&empty[st], (uint32_t)((n / STAGES - 1) & 1), stop_word, err)) break;
-                const uint32_t k = ring + st * 2 * TILE, v = k + TILE;
-                ec_mbar_expect_tx(&full[st], 2 * TILE);
+                if (n >= KS && !tt_wait(&k_empty[ks], (uint32_t)((n / KS - 1) & 1), stop_word, err)) break;
+                ec_mbar_expect_tx(&k_full[ks], TILE);
 #pragma unroll
-                for (int c = 0; c < C::COLS; ++c) {
-                    tt_load(k + c * 8192, &maps.k, &full[st], kh * HD + c * 64, page);
-                    tt_load(v + c * 8192, &maps.v, &full[st], kh * HD + c * 64, page);
-                }
-                issued = n + 1;
+                for (int c = 0; c < C::COLS; ++c) tt_load(k_ring + ks * TILE + c * 8192, &maps.k, &k_full[ks], kh * HD + c * 64, page);
+                k_issued = n + 1;
+                if (n >= VS && !tt_wait(&v_empty[vs], (uint32_t)((n / VS - 1) & 1), stop_word, err)) break;
+                ec_mbar_expect_tx(&v_full[vs], TILE);
+#pragma unroll
+                for (int c = 0; c < C::COLS; ++c) tt_load(v_ring + vs * TILE + c * 8192, &maps.v, &v_full[vs], kh * HD + c * 64, page);
+                v_issued = n + 1;
             }
         };
         if (warp == 5) {
             if (lane == 0) {
                 next = ta_page(kv, s.slot, p_begin, err);
-                produce(0, min(pages, STAGES));
+                produce(0, min(pages, VS));
             }
         } else if (warp < 4) {
             // the queries: rows behind the sequence are zero
@@ -234,29 +251,31 @@ k_tree_tc(const __grid_constant__ TtMaps maps, const ec_kv_pages kv, const ec_tr
         tt_after();
 
         if (warp == 5) {
-            if (lane == 0) produce(min(pages, STAGES), pages);
+            if (lane == 0) produce(min(pages, VS), pages);
         } else if (warp == 4) {
             if (lane == 0) {
                 const uint64_t dq = tt_desc(base, 16);
                 for (int i = 0; i <= pages; ++i) {
                     if (i < pages) {   // S of page i
-                        const int n = count + i, st = n % STAGES;
-                        if (!tt_wait(&full[st], (uint32_t)((n / STAGES) & 1), stop_word, err)) break;
+                        const int n = count + i, ks = n % KS;
+                        if (!tt_wait(&k_full[ks], (uint32_t)((n / KS) & 1), stop_word, err)) break;
                         tt_after();
-                        const uint64_t dk = tt_desc(ring + st * 2 * TILE, 16);
+                        const uint64_t dk = tt_desc(k_ring + ks * TILE, 16);
 #pragma unroll
                         for (int k = 0; k < HD / 16; ++k)
                             tt_mma_ss(tmem + (n & 1) * 64, dq + (k / 4) * (TT_ROWS * 128 >> 4) + (k % 4) * 2, dk + (k / 4) * (8192 >> 4) + (k % 4) * 2, C::IDESC_S, k > 0);
                         tt_commit(&s_full[n & 1]);
+                        tt_commit(&k_empty[ks]);
                     }
                     if (i > 0) {       // P V of page i - 1
-                        const int n = count + i - 1, st = n % STAGES;
+                        const int n = count + i - 1, vs = n % VS;
+                        if (!tt_wait(&v_full[vs], (uint32_t)((n / VS) & 1), stop_word, err)) break;
                         if (!tt_wait(&p_ready[n & 1], (uint32_t)((n / 2) & 1), stop_word, err)) break;
                         tt_after();
-                        const uint64_t dv = tt_desc(ring + st * 2 * TILE + TILE, 8192);
+                        const uint64_t dv = tt_desc(v_ring + vs * TILE, 8192);
 #pragma unroll
                         for (int k = 0; k < 4; ++k) tt_mma_ts(tmem_o, tmem + (n & 1) * 64 + k * 8, dv + k * (2048 >> 4), C::IDESC_O, 1);
-                        tt_commit(&empty[st]);
+                        tt_commit(&v_empty[vs]);
                         tt_commit(o_done);
                     }
                 }
@@ -268,7 +287,7 @@ k_tree_tc(const __grid_constant__ TtMaps maps, const ec_kv_pages kv, const ec_tr
             float m = -INFINITY, l = 0.0f;
             bool ok = true;
             for (int i = 0; i < pages; ++i) {
-                const int n = count + i, st = n % STAGES, p0 = (p_begin + i) * PAGE;
+                const int n = count + i, vs = n % VS, p0 = (p_begin + i) * PAGE;
                 const bool part = p0 + PAGE > s.base || (a.window > 0 && p0 < (long long)s.base + 64 * a.mask_words - a.window);
                 ok = ok && tt_wait_warp(&s_full[n & 1], (uint32_t)((n / 2) & 1), stop_word, err);
                 if (!ok) {
@@ -280,8 +299,7 @@ k_tree_tc(const __grid_constant__ TtMaps maps, const ec_kv_pages kv, const ec_tr
                 }
                 tt_after();
                 float x[64];
-                tt_ld32(tmem + lane_at + (n & 1) * 64, x);
-                tt_ld32(tmem + lane_at + (n & 1) * 64 + 32, x + 32);
+                tt_ld64(tmem + lane_at + (n & 1) * 64, x);
                 unsigned long long see = ~0ull;
                 if (part) {
                     see = ta_allow(a, s, node, p0);
@@ -305,9 +323,9 @@ k_tree_tc(const __grid_constant__ TtMaps maps, const ec_kv_pages kv, const ec_tr
                     // V of positions that are not there is zero, and infinities
                     // and NaN (0 times them is NaN) are taken out and added by
                     // the rows that see them
-                    unsigned char *v = smem + (ring - base) + st * 2 * TILE + TILE;
+                    unsigned char *v = smem + (v_ring - base) + vs * TILE;
                     constexpr uint32_t E = C::BF ? 0x7f80u : 0x7c00u;
-                    ok = tt_wait_warp(&full[st], (uint32_t)((n / STAGES) & 1), stop_word, err);
+                    ok = tt_wait_warp(&v_full[vs], (uint32_t)((n / VS) & 1), stop_word, err);
                     for (int b = row; b < TILE / 16; b += 128) {
                         const int pos = (b * 16 % 8192) / 128;
                         uint4 *u = reinterpret_cast<uint4 *>(v + b * 16);
@@ -323,12 +341,9 @@ k_tree_tc(const __grid_constant__ TtMaps maps, const ec_kv_pages kv, const ec_tr
                     tt_proxy();
                     odd = tt_any(odd);
                 }
-                // All earlier products are in O.  Waited for on every page: a
-                // phase can be waited for by its parity only while it is the
-                // last or the next to complete, and S of this page says no more
-                // than that the product two pages back is done.
-                if (n > 0) ok = tt_wait_warp(o_done, (uint32_t)((n - 1) & 1), stop_word, err) && ok;
                 if (__any_sync(0xffffffffu, grow) || odd) {
+                    // all earlier products are in O
+                    if (n > 0) ok = tt_wait_warp(o_done, (uint32_t)((n - 1) & 1), stop_word, err) && ok;
                     tt_after();
 #pragma unroll
                     for (int c = 0; c < HD; c += 32) {
@@ -337,7 +352,7 @@ k_tree_tc(const __grid_constant__ TtMaps maps, const ec_kv_pages kv, const ec_tr
 #pragma unroll
                         for (int j = 0; j < 32; ++j) o[j] *= scale;
                         if (odd) {
-                            const unsigned char *v = smem + (ring - base) + st * 2 * TILE + TILE + (c / 64) * 8192;
+                            const unsigned char *v = smem + (v_ring - base) + vs * TILE + (c / 64) * 8192;
                             for (int k = 0; k < 64; ++k) {
                                 if (!(see >> k & 1)) continue;
 #pragma unroll
@@ -357,7 +372,7 @@ k_tree_tc(const __grid_constant__ TtMaps maps, const ec_kv_pages kv, const ec_tr
                     tt_wait_st();
                     if (odd) {
                         tt_any(false);   // every row has added them
-                        uint16_t *v = reinterpret_cast<uint16_t *>(smem + (ring - base) + st * 2 * TILE + TILE);
+                        uint16_t *v = reinterpret_cast<uint16_t *>(smem + (v_ring - base) + vs * TILE);
                         constexpr uint16_t E = C::BF ? 0x7f80u : 0x7c00u;
                         for (int b = row; b < TILE / 2; b += 128)
                             if ((v[b] & E) == E) v[b] = 0;
@@ -378,6 +393,11 @@ k_tree_tc(const __grid_constant__ TtMaps maps, const ec_kv_pages kv, const ec_tr
                 l += sum[0] + sum[1];
                 tt_st32(tmem + lane_at + (n & 1) * 64, p);
                 tt_wait_st();
+                // The product of the last page is done before this one may
+                // begin: a phase of o_done can be waited for by its parity only
+                // while it is the last or the next to complete, and S of a page
+                // says no more than that the product two pages back is done.
+                if (n > 0) ok = tt_wait_warp(o_done, (uint32_t)((n - 1) & 1), stop_word, err) && ok;
                 tt_before();
                 __syncwarp();
                 if (lane == 0) tt_arrive(&p_ready[n & 1]);
@@ -428,9 +448,11 @@ k_tree_tc(const __grid_constant__ TtMaps maps, const ec_kv_pages kv, const ec_tr
     // Loads that nobody waited for (after a wait that gave up) land before the
     // shared memory goes away, bounded; then the columns are freed.
     if (warp == 5 && lane == 0 && *stop_word)
-        for (int n = issued > STAGES ? issued - STAGES : 0; n < issued; ++n)
-            for (uint32_t i = 0; i < (1u << 20); ++i)
-                if (ec_mbar_try_wait(&full[n % STAGES], (uint32_t)((n / STAGES) & 1))) break;
+        for (int j = 0; j < KS + VS; ++j) {
+            const int n = j < KS ? k_issued - 1 - j : v_issued - 1 - (j - KS);
+            for (uint32_t i = 0; n >= 0 && i < (1u << 20); ++i)
+                if (j < KS ? ec_mbar_try_wait(&k_full[n % KS], (uint32_t)((n / KS) & 1)) : ec_mbar_try_wait(&v_full[n % VS], (uint32_t)((n / VS) & 1))) break;
+        }
     if (warp == 4 && lane == 0) {
         tt_commit(drain);     // every MMA that was issued is complete once this fires
         for (uint32_t i = 0; i < (1u << 24); ++i)
