@@ -586,7 +586,7 @@ __global__ void __launch_bounds__(TJ_THREADS) k_tree_join(const ec_kv_pages kv, 
         s = line.tile(kv, a, g, mt, border, begin, err);
         if (begin == border || line.start(i0) > begin) return;   // cuts nothing, or not the first
     }
-    const int n = line.piece(begin + (s.page1 - s.page0) - 1) - i0 + 1;   // pieces of the tile
+    const int n = line.piece(begin + s.len - 1) - i0 + 1;   // pieces of the tile
     if (n == 1) return;
     auto place = [&](int i, int r) { return ((size_t)(i0 + i) * 2 + (i == 0)) * mt + r; };   // begun in piece i0, goes on in the others
     auto out_at = [&](int r) {
@@ -710,7 +710,7 @@ TaPlan ta_plan(int n_seq, int rows, int n_head, int n_kv_head, int hd, int max_l
     p.g.div_shift = 30 + up;   // rounded up: exact for rows below 2^30
     p.g.div_mul = (unsigned)(((1ull << p.g.div_shift) + p.g.group - 1) / p.g.group);
     const int mean = (int)(((long long)rows * p.g.group + n_seq - 1) / n_seq);
-    // from 65 rows on, tiles of 128 on the tensor cores of tcgen05
+    // from 65 rows on, tiles of twice 128 on the tensor cores of tcgen05
     p.mt = mean <= 16 ? 16 : mean <= 32 ? 32 : mean <= 64 || !tc ? 64 : TC_ROWS;
     p.tiles = (int)(((long long)rows * p.g.group) / p.mt + n_seq);   // every sequence rounds up once; rows * group fits 31 bits
     int pages = ta_up(max_len > 0 ? max_len : 1, PAGE);
@@ -719,7 +719,7 @@ TaPlan ta_plan(int n_seq, int rows, int n_head, int n_kv_head, int hd, int max_l
     const long long tiles = (long long)p.tiles * n_kv_head;
     p.pieces = 0;
     if (!(pages <= 16 && tiles * p.g.cluster <= sms) && tiles * slot_pages <= 0x7fffffff)
-        p.pieces = (p.mt == TC_ROWS ? 2 : p.hdp == 64 && !f32 ? 3 : p.hdp <= 128 ? 2 : 1) * sms;
+        p.pieces = (p.mt == TC_ROWS ? 1 : p.hdp == 64 && !f32 ? 3 : p.hdp <= 128 ? 2 : 1) * sms;
     if (!p.pieces && p.mt == TC_ROWS) {   // clusters: the register tiles only
         p.mt = 64;
         p.tiles = (int)(((long long)rows * p.g.group) / p.mt + n_seq);

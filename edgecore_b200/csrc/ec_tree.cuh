@@ -1,5 +1,5 @@
 // ec_tree.cuh -- what the kernels of the tree attention share (ec_tree.cu: mma
-// tiles of up to 64 rows, ec_tree_tc.cu: tcgen05 tiles of 128 rows): how the
+// tiles of up to 64 rows, ec_tree_tc.cu: tcgen05 tiles of twice 128 rows): how the
 // rows and pages of a call are laid out as work, which positions a row sees,
 // and small helpers.
 #pragma once
@@ -10,6 +10,7 @@ namespace ec_tree {
 
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr int PAGE = EC_KV_PAGE;
+constexpr int TC_ROWS = 256;            // rows of a tile on tcgen05: two halves of 128
 
 // ---- the work of a call ------------------------------------------------------
 
@@ -31,10 +32,12 @@ struct TaTile {           // one row tile of one KV head
     int kh;
     int r0, t, base, slot;
     int page0, page1;     // pages that hold visible positions
+    int len, step;        // places on the line of pages (TaLine), pages of a place
 };
 
 struct TaSeq {            // a sequence, in the lane that holds it
     int r0, t, base, slot, page0, pages, tiles;   // a bad one has no tiles
+    int half;             // the last tile has no more than half of the rows (TC_ROWS tiles only)
 };
 
 EC_DEV TaSeq ta_seq(const ec_kv_pages &kv, const ec_tree_attn &a, const TaGeo &g, int mt, int i, int *err) {
@@ -51,6 +54,7 @@ EC_DEV TaSeq ta_seq(const ec_kv_pages &kv, const ec_tree_attn &a, const TaGeo &g
     }
     q.t = (int)t;
     q.tiles = (int)((t * g.group + mt - 1) / mt);
+    q.half = mt == TC_ROWS && (int)(t * g.group - (long long)(q.tiles - 1) * mt) <= mt / 2;
     const int lo = a.window > 0 && q.base > a.window ? q.base - a.window : 0;   // no row sees a position below it
     q.page0 = lo / PAGE;
     q.pages = (q.base + q.t + PAGE - 1) / PAGE - q.page0;
@@ -67,6 +71,9 @@ EC_DEV TaTile ta_tile(const TaSeq &q, int l, int tile, int kh, int mt) {   // fr
     s.slot = __shfl_sync(0xffffffffu, q.slot, l);
     s.page0 = __shfl_sync(0xffffffffu, q.page0, l);
     s.page1 = s.page0 + __shfl_sync(0xffffffffu, q.pages, l);
+    const bool half = tile == __shfl_sync(0xffffffffu, q.tiles, l) - 1 && __shfl_sync(0xffffffffu, q.half, l);
+    s.step = half ? 2 : 1;
+    s.len = half ? (s.page1 - s.page0 + 1) / 2 : s.page1 - s.page0;
     return s;
 }
 
@@ -98,13 +105,15 @@ EC_DEV bool ta_find(const ec_kv_pages &kv, const ec_tree_attn &a, const TaGeo &g
 }
 
 // The pages of all tiles in one line (below 2^31 of them, ta_plan): sequence
-// by sequence, KV head by KV head, tile by tile.  CTA i of the first n takes
-// [start(i), start(i + 1)), at least a page each.
+// by sequence, KV head by KV head, tile by tile; a place on it is a page, or
+// two of them in a tile whose rows are half as many.  CTA i of the first n
+// takes [start(i), start(i + 1)), at least one place each.
 struct TaLine {
     TaSeq head;           // sequence of this lane among the first 32
-    int n, total, per, more;   // the first `more` pieces have per + 1 pages
+    int n, total, per, more;   // the first `more` pieces have per + 1 places
 
-    EC_DEV static int work(const TaSeq &q, int kvh) { return q.tiles * q.pages * kvh; }
+    EC_DEV static int head_work(const TaSeq &q) { return q.tiles * q.pages - (q.half ? q.pages / 2 : 0); }   // of one KV head
+    EC_DEV static int work(const TaSeq &q, int kvh) { return head_work(q) * kvh; }
     EC_DEV void init(const ec_kv_pages &kv, const ec_tree_attn &a, const TaGeo &g, int mt, int pieces, int *err) {
         head = ta_seq(kv, a, g, mt, threadIdx.x & 31, err);
         total = __reduce_add_sync(0xffffffffu, work(head, a.n_kv_head));
@@ -131,9 +140,10 @@ struct TaLine {
                 const int l = hit ? __ffs((int)hit) - 1 : 0;
                 const int from = __shfl_sync(0xffffffffu, sum - w, l);
                 const int pages = max(1, __shfl_sync(0xffffffffu, q.pages, l)), tiles = max(1, __shfl_sync(0xffffffffu, q.tiles, l));
-                const int unit = (at - from) / pages, kh = unit / tiles;
-                begin = from + unit * pages;
-                return ta_tile(q, l, unit - kh * tiles, kh, mt);
+                const int each = max(1, __shfl_sync(0xffffffffu, head_work(q), l));
+                const int kh = (at - from) / each, tile = min((at - from - kh * each) / pages, tiles - 1);
+                begin = from + kh * each + tile * pages;
+                return ta_tile(q, l, tile, kh, mt);
             }
             before = __shfl_sync(0xffffffffu, sum, 31);
         }
@@ -149,7 +159,8 @@ struct TaLine {
             if (hit) {
                 const int l = __ffs((int)hit) - 1, unit = index - __shfl_sync(0xffffffffu, us - u, l);
                 const int tiles = __shfl_sync(0xffffffffu, q.tiles, l), kh = unit / tiles;
-                begin = __shfl_sync(0xffffffffu, ws - w, l) + unit * __shfl_sync(0xffffffffu, q.pages, l);
+                begin = __shfl_sync(0xffffffffu, ws - w, l) + kh * __shfl_sync(0xffffffffu, head_work(q), l) +
+                        (unit - kh * tiles) * __shfl_sync(0xffffffffu, q.pages, l);
                 s = ta_tile(q, l, unit - kh * tiles, kh, mt);
                 return true;
             }
@@ -239,7 +250,6 @@ template <bool BF> EC_DEV float2 unpack2(uint32_t u) {
 
 // tcgen05 tiles (ec_tree_tc.cu): whether they take a call of this kind, and
 // the launch of its pieces (one per resident CTA of `pieces`).
-constexpr int TC_ROWS = 128;
 bool ta_tc_takes(int q_type, int kv_type, int hd);
 int ta_tc_launch(const ec_kv_pages &kv, const ec_tree_attn &a, const TaGeo &g, int pieces, int *err, cudaStream_t stream);
 

@@ -1,24 +1,28 @@
 // ec_tree_tc.cu -- the tree attention of ec_tree.cu on the 5th-generation
-// tensor cores, for tiles of 128 rows: large drafts, or many query heads on a
-// KV head.
+// tensor cores, for tiles of two halves of 128 rows: large drafts, or many
+// query heads on a KV head.
 //
-// A CTA (two per SM) takes its piece of the line of pages, tile by tile:
-//   warp 5     TMA producer: K and V of a page, [64 positions][hd] each in
-//              columns of 128 bytes with the 128-byte swizzle, into a ring
-//   warp 4     one thread issues the MMAs: S = Q K^T (128 x 64, both operands
-//              K-major in shared memory) into one of two S buffers, and
-//              O += P V with P from tensor memory and V as it lies (rows of hd,
-//              "MN-major")
-//   warps 0-3  one row per thread: S from tensor memory, the positions that
-//              the row sees, running maximum and sum, P back over S as 16-bit
-//              pairs; O is rescaled in tensor memory only when the maximum has
-//              grown by more than 2^8 (the reference of a row is any earlier
-//              maximum, and p stays below 2^14)
-// so that the products of one page run under the exponentials of the next,
-// and one CTA's under the other's.  Per page and SM: 128 x 64 exponentials, 512
-// cycles of the special function units, and 2 x 128 x 64 x hd products, 350
-// (hd 64) to 700 (hd 128) cycles at the rate that cuBLAS reaches.  Every wait is
-// bounded; loads use no multicast.
+// A CTA (one per SM) takes its piece of the line of pages, tile by tile.  A
+// step is 128 rows against two pages (128 positions); the steps of the two
+// halves alternate, so that the products of one run under the exponentials of
+// the other.  A tile with rows for one half only gives its even steps to half 0
+// and its odd ones to half 1, whose sums are added at the end.
+//   warp 9      TMA producer: K and V of two pages, [64 positions][hd] each in
+//               columns of 128 bytes with the 128-byte swizzle, into rings
+//   warp 8      one thread issues the MMAs: S = Q K^T (128 x 128, both operands
+//               K-major in shared memory) of a step, then O += P V of the step
+//               before, a page at a time, with P from tensor memory and V as it
+//               lies (rows of hd, "MN-major")
+//   warps 0-3   half 0, warps 4-7 half 1, a row per thread: S from tensor memory,
+//               the positions that the row sees, running maximum and sum, P back
+//               over S as 16-bit pairs; O is rescaled in tensor memory only when
+//               the maximum has grown by more than 2^8 (the reference of a row is
+//               any earlier maximum, and p stays below 2^14)
+// Per step: 128 x 128 exponentials, 1024 cycles of an SM's special function
+// units, and 2 x 128 x 128 x hd products, 700 (hd 64) to 1400 (hd 128) cycles at
+// the rate that cuBLAS reaches.  Two CTAs per SM of 128 rows each, which nothing
+// kept out of step, took 3400 cycles a page instead.  Every wait is bounded;
+// loads use no multicast.
 #include "ec_tree.cuh"
 
 #include <cuda.h>
@@ -28,20 +32,21 @@
 
 namespace {
 
-constexpr int TT_THREADS = 192, TT_ROWS = 128;
+constexpr int TT_THREADS = 320, TT_ROWS = 128;
 constexpr float TT_GROWTH = 8.0f;                      // log2 growth of a maximum that is let be
 
 template <int QT, int KT, int HD> struct TtCfg {
     static constexpr bool BF = KT == EC_T_BF16;
     static constexpr int COLS = HD / 64;               // 128-byte columns of a row
     static constexpr int TILE = 64 * HD * 2;           // K or V of a page
-    static constexpr int KS = HD == 64 ? 5 : 3, VS = HD == 64 ? 4 : 2;   // pages of K and of V in flight: K is free once S is done
-    static constexpr int Q_BYTES = TT_ROWS * HD * 2;
-    static constexpr int SMEM = Q_BYTES + (KS + VS) * TILE + 256;
-    static constexpr int TMEM = 256;                   // S 2 x 64, O up to 128 columns: two CTAs share an SM's 512
+    static constexpr int ROUND = 2 * TILE;             // two pages of K or V: [column][page][64][128 bytes]
+    static constexpr int KS = HD == 64 ? 5 : 2, VS = HD == 64 ? 5 : 3;   // in flight; K is free once its S are done
+    static constexpr int Q_BYTES = TT_ROWS * HD * 2;   // of one half
+    static constexpr int SMEM = 2 * Q_BYTES + (KS + VS) * ROUND + 2048;
+    static constexpr int TMEM = 512;                   // S of the halves at 0 and 128, O at 256 and 384
     static constexpr float LIFT = BF ? 0.0f : 6.0f;
     static constexpr uint32_t TYPES = (1u << 4) | ((BF ? 1u : 0u) << 7) | ((BF ? 1u : 0u) << 10) | ((uint32_t)(TT_ROWS >> 4) << 24);
-    static constexpr uint32_t IDESC_S = TYPES | ((64u >> 3) << 17);
+    static constexpr uint32_t IDESC_S = TYPES | ((64u >> 3) << 17), IDESC_S2 = TYPES | ((128u >> 3) << 17);   // one page, two
     static constexpr uint32_t IDESC_O = TYPES | (1u << 16) | ((uint32_t)(HD >> 3) << 17);   // B is MN-major
 };
 
@@ -51,18 +56,22 @@ template <int QT, int KT, int HD> struct TtCfg {
 EC_DEV uint64_t tt_desc(uint32_t addr, uint32_t lead) {
     return (uint64_t)((addr & 0x3ffffu) >> 4) | ((uint64_t)(lead >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
 }
+// The MMA warp runs as one: every lane computes the operands, which then stay
+// in uniform registers, and an elected lane issues.  (From a branch of one lane
+// each product took 110 cycles to issue, twice what it takes to run.)
 EC_DEV void tt_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t more) {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-                 "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %5, %5, %5}, p;\n\t}"
+    asm volatile("{\n\t.reg .pred p, q;\n\telect.sync _|q, 0xffffffff;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                 "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %5, %5, %5}, p;\n\t}"
                  ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(more), "r"(0u));
 }
 EC_DEV void tt_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t more) {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %5, %5, %5}, p;\n\t}"
+    asm volatile("{\n\t.reg .pred p, q;\n\telect.sync _|q, 0xffffffff;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                 "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %5, %5, %5}, p;\n\t}"
                  ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(more), "r"(0u));
 }
-EC_DEV void tt_commit(uint64_t *bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(ec_smem_u32(bar)) : "memory");
+EC_DEV void tt_commit(uint32_t bar) {
+    asm volatile("{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\t"
+                 "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar) : "memory");
 }
 EC_DEV void tt_arrive(uint64_t *bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(ec_smem_u32(bar)) : "memory"); }
 EC_DEV void tt_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
@@ -70,13 +79,16 @@ EC_DEV void tt_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "m
 EC_DEV void tt_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 EC_DEV void tt_proxy() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
-// 64 or 32 columns of this thread's row, arrived (the wait is part of the
+// 128 or 32 columns of this thread's row, arrived (the wait is part of the
 // statement: nothing may use the registers before it)
-EC_DEV void tt_ld64(uint32_t taddr, float *f) {
+EC_DEV void tt_ld128(uint32_t taddr, float *f) {
     __syncwarp();   // a whole warp executes these as one
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x64.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, "
                  "%30, %31, %32, %33, %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47, %48, %49, %50, %51, %52, %53, %54, %55, %56, %57, "
-                 "%58, %59, %60, %61, %62, %63}, [%64];\n\t"
+                 "%58, %59, %60, %61, %62, %63}, [%128];\n\t"
+                 "tcgen05.ld.sync.aligned.32x32b.x64.b32 {%64, %65, %66, %67, %68, %69, %70, %71, %72, %73, %74, %75, %76, %77, %78, %79, %80, %81, %82, %83, %84, %85, %86, %87, %88, %89, %90, %91, "
+                 "%92, %93, %94, %95, %96, %97, %98, %99, %100, %101, %102, %103, %104, %105, %106, %107, %108, %109, %110, %111, %112, %113, %114, %115, %116, "
+                 "%117, %118, %119, %120, %121, %122, %123, %124, %125, %126, %127}, [%129];\n\t"
                  "tcgen05.wait::ld.sync.aligned;"
                  : "=f"(f[0]), "=f"(f[1]), "=f"(f[2]), "=f"(f[3]), "=f"(f[4]), "=f"(f[5]), "=f"(f[6]), "=f"(f[7]), "=f"(f[8]), "=f"(f[9]), "=f"(f[10]),
                    "=f"(f[11]), "=f"(f[12]), "=f"(f[13]), "=f"(f[14]), "=f"(f[15]), "=f"(f[16]), "=f"(f[17]), "=f"(f[18]), "=f"(f[19]), "=f"(f[20]),
@@ -84,8 +96,14 @@ EC_DEV void tt_ld64(uint32_t taddr, float *f) {
                    "=f"(f[31]), "=f"(f[32]), "=f"(f[33]), "=f"(f[34]), "=f"(f[35]), "=f"(f[36]), "=f"(f[37]), "=f"(f[38]), "=f"(f[39]), "=f"(f[40]),
                    "=f"(f[41]), "=f"(f[42]), "=f"(f[43]), "=f"(f[44]), "=f"(f[45]), "=f"(f[46]), "=f"(f[47]), "=f"(f[48]), "=f"(f[49]), "=f"(f[50]),
                    "=f"(f[51]), "=f"(f[52]), "=f"(f[53]), "=f"(f[54]), "=f"(f[55]), "=f"(f[56]), "=f"(f[57]), "=f"(f[58]), "=f"(f[59]), "=f"(f[60]),
-                   "=f"(f[61]), "=f"(f[62]), "=f"(f[63])
-                 : "r"(taddr) : "memory");
+                   "=f"(f[61]), "=f"(f[62]), "=f"(f[63]), "=f"(f[64]), "=f"(f[65]), "=f"(f[66]), "=f"(f[67]), "=f"(f[68]), "=f"(f[69]), "=f"(f[70]),
+                   "=f"(f[71]), "=f"(f[72]), "=f"(f[73]), "=f"(f[74]), "=f"(f[75]), "=f"(f[76]), "=f"(f[77]), "=f"(f[78]), "=f"(f[79]), "=f"(f[80]),
+                   "=f"(f[81]), "=f"(f[82]), "=f"(f[83]), "=f"(f[84]), "=f"(f[85]), "=f"(f[86]), "=f"(f[87]), "=f"(f[88]), "=f"(f[89]), "=f"(f[90]),
+                   "=f"(f[91]), "=f"(f[92]), "=f"(f[93]), "=f"(f[94]), "=f"(f[95]), "=f"(f[96]), "=f"(f[97]), "=f"(f[98]), "=f"(f[99]), "=f"(f[100]),
+                   "=f"(f[101]), "=f"(f[102]), "=f"(f[103]), "=f"(f[104]), "=f"(f[105]), "=f"(f[106]), "=f"(f[107]), "=f"(f[108]), "=f"(f[109]), "=f"(f[110]),
+                   "=f"(f[111]), "=f"(f[112]), "=f"(f[113]), "=f"(f[114]), "=f"(f[115]), "=f"(f[116]), "=f"(f[117]), "=f"(f[118]), "=f"(f[119]), "=f"(f[120]),
+                   "=f"(f[121]), "=f"(f[122]), "=f"(f[123]), "=f"(f[124]), "=f"(f[125]), "=f"(f[126]), "=f"(f[127])
+                 : "r"(taddr), "r"(taddr + 64) : "memory");
 }
 EC_DEV void tt_ld32(uint32_t taddr, float *f) {
     __syncwarp();
@@ -108,6 +126,21 @@ EC_DEV void tt_st32(uint32_t taddr, const uint32_t *r) {
                  : "memory");
 }
 
+// two fp32 at a time
+EC_DEV float2 tt_fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("{\n\t.reg .b64 x, y, z, w;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\t"
+        "fma.rn.f32x2 w, x, y, z;\n\tmov.b64 {%0, %1}, w;\n\t}"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
+}
+EC_DEV float2 tt_add2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n\t.reg .b64 x, y, w;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tadd.rn.f32x2 w, x, y;\n\tmov.b64 {%0, %1}, w;\n\t}"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+
 EC_DEV void tt_load(uint32_t dst, const CUtensorMap *map, uint64_t *bar, int x, int page) {   // 64 positions of 128 bytes
     asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
                  ::"r"(dst), "l"(map), "r"(ec_smem_u32(bar)), "r"(x), "r"(0), "r"(page) : "memory");
@@ -125,35 +158,62 @@ EC_DEV bool tt_wait(uint64_t *bar, uint32_t parity, volatile int *stop, int *err
     return false;
 }
 
-// The same for a whole warp, which goes on together: lane 0 waits.
+// The same for a whole warp, which goes on together.
 EC_DEV bool tt_wait_warp(uint64_t *bar, uint32_t parity, volatile int *stop, int *err) {
+    if (__all_sync(0xffffffffu, ec_mbar_try_wait(bar, parity))) return true;
     int ok = 0;
     if ((threadIdx.x & 31) == 0) ok = tt_wait(bar, parity, stop, err);
     ok = __shfl_sync(0xffffffffu, ok, 0);
-    __syncwarp();
-    return ok != 0;
+    // every lane sees the phase complete for itself: what it guards is visible to it
+    return ok && __all_sync(0xffffffffu, ec_mbar_try_wait(bar, parity));
 }
 
-// OR over the 128 threads of the row warps.  A warp whose wait gave up goes on
-// to take part in every one of these, so that no other waits for it.
-EC_DEV bool tt_any(bool v) {
+// OR over the row warps that share V: all 256 threads, or the 128 of one half.
+// A warp whose wait gave up goes on to take part in every one of these, so that
+// no other waits for it.
+EC_DEV bool tt_any(bool v, int bar, int threads) {
     int r;
     __syncwarp();
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.s32 p, %1, 0;\n\tbar.red.or.pred p, 1, 128, p;\n\tselp.s32 %0, 1, 0, p;\n\t}" : "=r"(r) : "r"((int)v) : "memory");
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.s32 p, %1, 0;\n\tbar.red.or.pred p, %2, %3, p;\n\tselp.s32 %0, 1, 0, p;\n\t}"
+                 : "=r"(r) : "r"((int)v), "r"(bar), "r"(threads) : "memory");
     return r != 0;
+}
+
+// O of this thread's row plus the infinities and NaN of the positions of a
+// round that it sees (a page's mask each).  Out of line: hardly ever called.
+template <bool BF> __noinline__ __device__ void tt_add_odd(uint32_t tmem_o, int hd, const unsigned char *v, unsigned long long see0, unsigned long long see1) {
+#pragma unroll 1
+    for (int c = 0; c < hd; c += 32) {
+        float o[32];
+        tt_ld32(tmem_o + c, o);
+#pragma unroll 1
+        for (int k = 0; k < 128; ++k) {
+            if (!((k < 64 ? see0 : see1) >> (k & 63) & 1)) continue;
+#pragma unroll
+            for (int j = 0; j < 32; j += 2) {
+                const int ch = (c % 64 + j) / 8;
+                const float2 y = unpack2<BF>(*reinterpret_cast<const uint32_t *>(v + (c / 64) * 16384 + k * 128 + ((ch ^ (k & 7)) << 4) + (j % 8) * 2));
+                if (!(fabsf(y.x) < INFINITY)) o[j] += y.x;
+                if (!(fabsf(y.y) < INFINITY)) o[j + 1] += y.y;
+            }
+        }
+        tt_st32(tmem_o + c, reinterpret_cast<const uint32_t *>(o));
+    }
+    tt_wait_st();
 }
 
 struct TtMaps { CUtensorMap k, v; };
 
 template <int QT, int KT, int HD>
-__global__ void __launch_bounds__(TT_THREADS, 2)
+__global__ void __launch_bounds__(TT_THREADS, 1)
 k_tree_tc(const __grid_constant__ TtMaps maps, const ec_kv_pages kv, const ec_tree_attn a, const TaGeo g, int *err) {
     typedef TtCfg<QT, KT, HD> C;
-    constexpr int KS = C::KS, VS = C::VS, TILE = C::TILE;
+    constexpr int KS = C::KS, VS = C::VS, ROUND = C::ROUND;
     extern __shared__ __align__(1024) unsigned char smem[];
     const uint32_t base = ec_smem_u32(smem);              // 1024-byte aligned: the kernel has no other shared memory
-    const uint32_t k_ring = base + C::Q_BYTES, v_ring = k_ring + KS * TILE;
-    uint64_t *k_full = reinterpret_cast<uint64_t *>(smem + C::Q_BYTES + (KS + VS) * TILE), *k_empty = k_full + KS;
+    const uint32_t k_ring = base + 2 * C::Q_BYTES, v_ring = k_ring + KS * ROUND;
+    float2 *other = reinterpret_cast<float2 *>(smem + 2 * C::Q_BYTES + (KS + VS) * ROUND);   // (m, l) of half 1, [128]
+    uint64_t *k_full = reinterpret_cast<uint64_t *>(other + TT_ROWS), *k_empty = k_full + KS;
     uint64_t *v_full = k_empty + KS, *v_empty = v_full + VS, *s_full = v_empty + VS, *p_ready = s_full + 2, *o_done = p_ready + 2, *drain = o_done + 1;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(drain + 1);
     volatile int *stop_word = reinterpret_cast<volatile int *>(tmem_slot + 1);
@@ -178,139 +238,175 @@ k_tree_tc(const __grid_constant__ TtMaps maps, const ec_kv_pages kv, const ec_tr
         if (base & 1023) atomicCAS(err, 0, EC_KERR_BAD_INDEX);
         ec_fence_mbar_init();
     }
-    if (warp == 4) {
+    if (warp == 8) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(ec_smem_u32(tmem_slot)), "r"(C::TMEM));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     }
     tt_before();
     __syncthreads();
     tt_after();
-    const uint32_t tmem = *tmem_slot, tmem_o = tmem + 128;
+    const uint32_t tmem = *tmem_slot;
     EC_PDL_ENTER();
 
     TaLine line;
-    line.init(kv, a, g, TT_ROWS, gridDim.x, err);
+    line.init(kv, a, g, TC_ROWS, gridDim.x, err);
     int at = (int)blockIdx.x < line.n ? line.start(blockIdx.x) : 0;
     const int stop_at = (int)blockIdx.x < line.n ? line.start(blockIdx.x + 1) : 0;
-    int count = 0;        // pages of this CTA so far: stages count % KS and % VS, S buffer count % 2
-    int k_issued = 0, v_issued = 0, next = 0;   // producer: loads issued, arena page of the next one
+    int count = 0, tiles = 0;         // loads of K (and of V) and tiles of this CTA so far
+    int steps_of[2] = {0, 0};         // steps of each half so far
+    int k_issued = 0, v_issued = 0;   // producer: loads issued
+    int k_at = 0, v_at = 0;           // MMA warp: stages of the rings, and the phases to wait for
+    uint32_t k_phase = 0, v_phase = 0, p_phase = 0;
     while (at < stop_at) {
         int begin;
-        const TaTile s = line.tile(kv, a, g, TT_ROWS, at, begin, err);
-        const int p_begin = s.page0 + (at - begin), p_end = min(s.page1, p_begin + (stop_at - at)), pages = p_end - p_begin;
+        const TaTile s = line.tile(kv, a, g, TC_ROWS, at, begin, err);
+        const int places = min(begin + s.len, stop_at) - at;
+        const int p_begin = s.page0 + (at - begin) * s.step, p_end = min(s.page1, p_begin + places * s.step), pages = p_end - p_begin, rounds = (pages + 1) / 2;
         const int kh = s.kh, end = s.base + s.t;
+        const bool split = s.step == 2;   // one half's rows, the rounds shared out over both
+        const int steps = split ? rounds : 2 * rounds;
 
         // The producer: what the rings hold before the row warps are met below
         // (they are empty: the last tile is done), the rest after.
         auto produce = [&](int i0, int i1) {
             for (int i = i0; i < i1; ++i) {
-                const int n = count + i, ks = n % KS, vs = n % VS, page = next;
-                if (i + 1 < pages) next = ta_page(kv, s.slot, p_begin + i + 1, err);
-                if (n >= KS && !tt_wait(&k_empty[ks], (uint32_t)((n / KS - 1) & 1), stop_word, err)) break;
-                ec_mbar_expect_tx(&k_full[ks], TILE);
+                const int n = count + i, ks = n % KS, vs = n % VS, two = 2 * i + 1 < pages;
+                const int pg[2] = {ta_page(kv, s.slot, p_begin + 2 * i, err), two ? ta_page(kv, s.slot, p_begin + 2 * i + 1, err) : 0};
+                auto load = [&](uint32_t to, const CUtensorMap *map, uint64_t *bar) {
+                    ec_mbar_expect_tx(bar, (1 + two) * C::TILE);
+                    for (int h = 0; h <= two; ++h)
 #pragma unroll
-                for (int c = 0; c < C::COLS; ++c) tt_load(k_ring + ks * TILE + c * 8192, &maps.k, &k_full[ks], kh * HD + c * 64, page);
+                        for (int c = 0; c < C::COLS; ++c) tt_load(to + c * 16384 + h * 8192, map, bar, kh * HD + c * 64, pg[h]);
+                };
+                if (n >= KS && !tt_wait(&k_empty[ks], (uint32_t)((n / KS - 1) & 1), stop_word, err)) break;
+                load(k_ring + ks * ROUND, &maps.k, &k_full[ks]);
                 k_issued = n + 1;
                 if (n >= VS && !tt_wait(&v_empty[vs], (uint32_t)((n / VS - 1) & 1), stop_word, err)) break;
-                ec_mbar_expect_tx(&v_full[vs], TILE);
-#pragma unroll
-                for (int c = 0; c < C::COLS; ++c) tt_load(v_ring + vs * TILE + c * 8192, &maps.v, &v_full[vs], kh * HD + c * 64, page);
+                load(v_ring + vs * ROUND, &maps.v, &v_full[vs]);
                 v_issued = n + 1;
             }
         };
-        if (warp == 5) {
-            if (lane == 0) {
-                next = ta_page(kv, s.slot, p_begin, err);
-                produce(0, min(pages, VS));
-            }
-        } else if (warp < 4) {
-            // the queries: rows behind the sequence are zero
+        constexpr int AHEAD = KS < VS ? KS : VS;
+        if (warp == 9) {
+            if (lane == 0) produce(0, min(rounds, AHEAD));
+        } else if (warp < 8) {
+            // the queries, all in flight at once; rows behind the sequence are zero
             const bool wide = (a.ldq & 7) == 0 && (reinterpret_cast<uintptr_t>(a.q) & 15) == 0;
+            constexpr int CH = HD / 8, AT_ONCE = 256 / CH;   // 16-byte chunks of a row, rows at a time
+            const int c = threadIdx.x % CH;
 #pragma unroll 4
-            for (int i = threadIdx.x; i < TT_ROWS * HD / 8; i += 128) {
-                const int r = i / (HD / 8), c = i % (HD / 8), rr = s.first + r, node = ta_node(g, rr);
-                uint4 u = make_uint4(0u, 0u, 0u, 0u);
-                if (node < s.t) {
-                    const uint16_t *q = static_cast<const uint16_t *>(a.q) + (size_t)(s.r0 + node) * a.ldq + (size_t)(kh * g.group + rr - node * g.group) * HD + c * 8;
-                    if (wide) u = *reinterpret_cast<const uint4 *>(q);
-                    else u = make_uint4(q[0] | (uint32_t)q[1] << 16, q[2] | (uint32_t)q[3] << 16, q[4] | (uint32_t)q[5] << 16, q[6] | (uint32_t)q[7] << 16);
+            for (int r = threadIdx.x / CH; r < (split ? 1 : 2) * TT_ROWS; r += AT_ONCE) {
+                const int rr = s.first + r, node = ta_node(g, rr);
+                const bool real = node < s.t;
+                const uint16_t *q = static_cast<const uint16_t *>(a.q) + (real ? (size_t)(s.r0 + node) * a.ldq + (size_t)(kh * g.group + rr - node * g.group) * HD + c * 8 : 0);
+                const uint32_t to = (r / TT_ROWS) * C::Q_BYTES + (c / 8) * (TT_ROWS * 128) + (r % TT_ROWS) * 128 + (((c % 8) ^ (r & 7)) << 4);
+                if (wide) {
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(base + to), "l"(q), "r"(real ? 16 : 0) : "memory");
+                } else {
+                    uint4 u = make_uint4(0u, 0u, 0u, 0u);
+                    if (real) u = make_uint4(q[0] | (uint32_t)q[1] << 16, q[2] | (uint32_t)q[3] << 16, q[4] | (uint32_t)q[5] << 16, q[6] | (uint32_t)q[7] << 16);
+                    *reinterpret_cast<uint4 *>(smem + to) = u;
                 }
-                *reinterpret_cast<uint4 *>(smem + (c / 8) * (TT_ROWS * 128) + r * 128 + (((c % 8) ^ (r & 7)) << 4)) = u;
             }
             // O starts from zero
             uint32_t zero[32];
 #pragma unroll
             for (int i = 0; i < 32; ++i) zero[i] = 0u;
-#pragma unroll
-            for (int c = 0; c < HD; c += 32) tt_st32(tmem_o + ((uint32_t)(warp * 32) << 16) + c, zero);
+#pragma unroll 1
+            for (int i = 0; i < HD; i += 32) tt_st32(tmem + 256 + (warp / 4) * 128 + ((uint32_t)((warp & 3) * 32) << 16) + i, zero);
             tt_wait_st();
+            asm volatile("cp.async.wait_all;" ::: "memory");
             tt_proxy();
             tt_before();
         }
         __syncthreads();
         tt_after();
 
-        if (warp == 5) {
-            if (lane == 0) produce(min(pages, VS), pages);
-        } else if (warp == 4) {
-            if (lane == 0) {
-                const uint64_t dq = tt_desc(base, 16);
-                for (int i = 0; i <= pages; ++i) {
-                    if (i < pages) {   // S of page i
-                        const int n = count + i, ks = n % KS;
-                        if (!tt_wait(&k_full[ks], (uint32_t)((n / KS) & 1), stop_word, err)) break;
-                        tt_after();
-                        const uint64_t dk = tt_desc(k_ring + ks * TILE, 16);
+        if (warp == 9) {
+            if (lane == 0) produce(min(rounds, AHEAD), rounds);
+        } else if (warp == 8) {
+            const int all = __shfl_sync(0xffffffffu, steps, 0), pages_u = __shfl_sync(0xffffffffu, pages, 0);
+            const bool split_u = __shfl_sync(0xffffffffu, split, 0);
+            int i_s = 0, i_o = 0;   // rounds of the next S and of the next product with V
+            for (int t = 0; t <= all; ++t) {
+                if (t < all) {   // S of step t, over the P of the half's last step, which its products have read
+                    const int half = t & 1;
+                    if ((split_u || !half) && !tt_wait_warp(&k_full[k_at], k_phase, stop_word, err)) break;
+                    tt_after();
+                    const uint64_t dq = tt_desc(base + (split_u ? 0 : half * C::Q_BYTES), 16), dk = tt_desc(k_ring + k_at * ROUND, 16);
+                    const uint32_t idesc = 2 * i_s + 1 < pages_u ? C::IDESC_S2 : C::IDESC_S;
 #pragma unroll
-                        for (int k = 0; k < HD / 16; ++k)
-                            tt_mma_ss(tmem + (n & 1) * 64, dq + (k / 4) * (TT_ROWS * 128 >> 4) + (k % 4) * 2, dk + (k / 4) * (8192 >> 4) + (k % 4) * 2, C::IDESC_S, k > 0);
-                        tt_commit(&s_full[n & 1]);
-                        tt_commit(&k_empty[ks]);
+                    for (int k = 0; k < HD / 16; ++k)
+                        tt_mma_ss(tmem + half * 128, dq + (k / 4) * (TT_ROWS * 128 >> 4) + (k % 4) * 2, dk + (k / 4) * (16384 >> 4) + (k % 4) * 2, idesc, k > 0);
+                    tt_commit(ec_smem_u32(&s_full[half]));
+                    if (split_u || half) {
+                        tt_commit(ec_smem_u32(&k_empty[k_at]));
+                        if (++k_at == KS) { k_at = 0; k_phase ^= 1; }
+                        ++i_s;
                     }
-                    if (i > 0) {       // P V of page i - 1
-                        const int n = count + i - 1, vs = n % VS;
-                        if (!tt_wait(&v_full[vs], (uint32_t)((n / VS) & 1), stop_word, err)) break;
-                        if (!tt_wait(&p_ready[n & 1], (uint32_t)((n / 2) & 1), stop_word, err)) break;
-                        tt_after();
-                        const uint64_t dv = tt_desc(v_ring + vs * TILE, 8192);
+                }
+                if (t > 0) {       // P V of step t - 1
+                    const int half = (t - 1) & 1;
+                    const bool two = 2 * i_o + 1 < pages_u;
+                    const uint64_t dv = tt_desc(v_ring + v_at * ROUND, 16384);
+                    const uint32_t d = tmem + 256 + half * 128, pt = tmem + half * 128;
+                    if ((split_u || !half) && !tt_wait_warp(&v_full[v_at], v_phase, stop_word, err)) break;
+                    if (!tt_wait_warp(&p_ready[half], p_phase >> half & 1, stop_word, err)) break;
+                    p_phase ^= 1u << half;
+                    tt_after();
 #pragma unroll
-                        for (int k = 0; k < 4; ++k) tt_mma_ts(tmem_o, tmem + (n & 1) * 64 + k * 8, dv + k * (2048 >> 4), C::IDESC_O, 1);
-                        tt_commit(&v_empty[vs]);
-                        tt_commit(o_done);
+                    for (int k = 0; k < 4; ++k) tt_mma_ts(d, pt + k * 8, dv + k * (2048 >> 4), C::IDESC_O, 1);
+                    if (two)
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) tt_mma_ts(d, pt + 32 + k * 8, dv + (8192 >> 4) + k * (2048 >> 4), C::IDESC_O, 1);
+                    if (split_u || half) {
+                        tt_commit(ec_smem_u32(&v_empty[v_at]));
+                        if (++v_at == VS) { v_at = 0; v_phase ^= 1; }
+                        ++i_o;
                     }
                 }
             }
-        } else if (warp < 4) {
-            const int row = threadIdx.x, rr = s.first + row, node = ta_node(g, rr);
-            const uint32_t lane_at = (uint32_t)(warp * 32) << 16;
+            tt_commit(ec_smem_u32(o_done));
+        } else {
+            const int half = warp / 4, row = threadIdx.x & 127, rr = s.first + (split ? 0 : half * TT_ROWS) + row, node = ta_node(g, rr);
+            const uint32_t lane_at = (uint32_t)((warp & 3) * 32) << 16, tmem_s = tmem + half * 128 + lane_at, tmem_o = tmem + 256 + half * 128 + lane_at;
+            const int bar = split ? 1 + half : 1, voters = split ? 128 : 256;   // who shares a round's V
             const float f = g.scale2;
             float m = -INFINITY, l = 0.0f;
             bool ok = true;
-            for (int i = 0; i < pages; ++i) {
-                const int n = count + i, vs = n % VS, p0 = (p_begin + i) * PAGE;
-                const bool part = p0 + PAGE > s.base || (a.window > 0 && p0 < (long long)s.base + 64 * a.mask_words - a.window);
-                ok = ok && tt_wait_warp(&s_full[n & 1], (uint32_t)((n / 2) & 1), stop_word, err);
+            int step = steps_of[half];
+            for (int i = split ? half : 0; i < rounds; i += split ? 2 : 1, ++step) {
+                const int n = count + i, vs = n % VS, two = 2 * i + 1 < pages, p0 = (p_begin + 2 * i) * PAGE;
+                const bool part = !two || p0 + 2 * PAGE > s.base || (a.window > 0 && p0 < (long long)s.base + 64 * a.mask_words - a.window);
+                ok = ok && tt_wait_warp(&s_full[half], (uint32_t)(step & 1), stop_word, err);
                 if (!ok) {
-                    if (part && tt_any(false)) {
-                        tt_any(false);
-                        tt_any(false);
+                    if (part && tt_any(false, bar, voters)) {
+                        tt_any(false, bar, voters);
+                        tt_any(false, bar, voters);
                     }
                     continue;
                 }
                 tt_after();
-                float x[64];
-                tt_ld64(tmem + lane_at + (n & 1) * 64, x);
-                unsigned long long see = ~0ull;
+                // S is done, and with it every product of this half before it: O may be changed
+                float x[128];
+                tt_ld128(tmem_s, x);
+                unsigned long long see[2] = {~0ull, ~0ull};
                 if (part) {
-                    see = ta_allow(a, s, node, p0);
+                    see[0] = ta_allow(a, s, node, p0);
+                    see[1] = two ? ta_allow(a, s, node, p0 + PAGE) : 0ull;
+                    const uint32_t w[4] = {(uint32_t)see[0], (uint32_t)(see[0] >> 32), (uint32_t)see[1], (uint32_t)(see[1] >> 32)};
 #pragma unroll
-                    for (int j = 0; j < 64; ++j)
-                        if (!((j < 32 ? (uint32_t)see >> j : (uint32_t)(see >> 32) >> (j - 32)) & 1u)) x[j] = -INFINITY;
+                    for (int j = 0; j < 128; ++j)
+                        if (!(w[j / 32] >> (j % 32) & 1u)) x[j] = -INFINITY;
                 }
-                float hi[4] = {x[0], x[1], x[2], x[3]};
+                float hi[8];
 #pragma unroll
-                for (int j = 4; j < 64; ++j) hi[j & 3] = fmaxf(hi[j & 3], x[j]);
-                const float top = fmaxf(fmaxf(hi[0], hi[1]), fmaxf(hi[2], hi[3])) * f;
+                for (int e = 0; e < 8; ++e) hi[e] = fmaxf(x[e], x[8 + e]);
+#pragma unroll
+                for (int j = 16; j < 128; j += 16)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) hi[e] = fmaxf(fmaxf(hi[e], x[j + e]), x[j + 8 + e]);
+                const float top = fmaxf(fmaxf(fmaxf(hi[0], hi[1]), fmaxf(hi[2], hi[3])), fmaxf(fmaxf(hi[4], hi[5]), fmaxf(hi[6], hi[7]))) * f;
                 const bool grow = top > m + TT_GROWTH || (m == -INFINITY && top > m);
                 float scale = 1.0f;
                 if (grow) {
@@ -318,149 +414,183 @@ k_tree_tc(const __grid_constant__ TtMaps maps, const ec_kv_pages kv, const ec_tr
                     m = top;
                     l *= scale;
                 }
+                unsigned char *v = smem + (v_ring - base) + vs * ROUND;   // position k of the round: page k / 64, row k % 64 of each column
+                auto v_row = [&](int c, int k) { return v + c * 16384 + k * 128; };
+                constexpr uint32_t E = C::BF ? 0x7f80u : 0x7c00u;
                 bool odd = false;
+                const bool keeper = split || half == 0;   // changes V where it has to be
                 if (part) {
                     // V of positions that are not there is zero, and infinities
                     // and NaN (0 times them is NaN) are taken out and added by
-                    // the rows that see them
-                    unsigned char *v = smem + (v_ring - base) + vs * TILE;
-                    constexpr uint32_t E = C::BF ? 0x7f80u : 0x7c00u;
+                    // the rows that see them.  The halves that share a round
+                    // meet here; the first product of the round comes after.
                     ok = tt_wait_warp(&v_full[vs], (uint32_t)((n / VS) & 1), stop_word, err);
-                    for (int b = row; b < TILE / 16; b += 128) {
-                        const int pos = (b * 16 % 8192) / 128;
-                        uint4 *u = reinterpret_cast<uint4 *>(v + b * 16);
-                        if (p0 + pos >= end) {
-                            *u = make_uint4(0u, 0u, 0u, 0u);
-                        } else {
-                            const uint4 w = *u;
-                            const uint32_t w4[4] = {w.x, w.y, w.z, w.w};
+                    const int k = row;   // a position of the round per thread
+                    if (keeper && k < (1 + two) * 64)
+                        for (int c = 0; c < C::COLS; ++c)
+                            for (int b = 0; b < 8; ++b) {
+                                uint4 *u = reinterpret_cast<uint4 *>(v_row(c, k) + ((b + k) % 8) * 16);
+                                if (p0 + k >= end) {
+                                    *u = make_uint4(0u, 0u, 0u, 0u);
+                                } else {
+                                    const uint4 w = *u;
+                                    const uint32_t w4[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-                            for (int j = 0; j < 4; ++j) odd |= (w4[j] & E) == E || (w4[j] >> 16 & E) == E;
-                        }
-                    }
-                    tt_proxy();
-                    odd = tt_any(odd);
-                }
-                if (__any_sync(0xffffffffu, grow) || odd) {
-                    // all earlier products are in O
-                    if (n > 0) ok = tt_wait_warp(o_done, (uint32_t)((n - 1) & 1), stop_word, err) && ok;
-                    tt_after();
-#pragma unroll
-                    for (int c = 0; c < HD; c += 32) {
-                        float o[32];
-                        tt_ld32(tmem_o + lane_at + c, o);
-#pragma unroll
-                        for (int j = 0; j < 32; ++j) o[j] *= scale;
-                        if (odd) {
-                            const unsigned char *v = smem + (v_ring - base) + vs * TILE + (c / 64) * 8192;
-                            for (int k = 0; k < 64; ++k) {
-                                if (!(see >> k & 1)) continue;
-#pragma unroll
-                                for (int j = 0; j < 32; j += 2) {
-                                    const int ch = (c % 64 + j) / 8;
-                                    const float2 y = unpack2<C::BF>(*reinterpret_cast<const uint32_t *>(v + k * 128 + ((ch ^ (k & 7)) << 4) + (j % 8) * 2));
-                                    if (!(fabsf(y.x) < INFINITY)) o[j] += y.x;
-                                    if (!(fabsf(y.y) < INFINITY)) o[j + 1] += y.y;
+                                    for (int j = 0; j < 4; ++j) odd |= (w4[j] & E) == E || (w4[j] >> 16 & E) == E;
                                 }
                             }
-                        }
-                        uint32_t r[32];
+                    tt_proxy();
+                    odd = tt_any(odd, bar, voters);
+                }
+                if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll 1
+                    for (int c = 0; c < HD; c += 32) {
+                        float o[32];
+                        tt_ld32(tmem_o + c, o);
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(o[j]);
-                        tt_st32(tmem_o + lane_at + c, r);
+                        for (int j = 0; j < 32; ++j) o[j] *= scale;
+                        tt_st32(tmem_o + c, reinterpret_cast<const uint32_t *>(o));
                     }
                     tt_wait_st();
-                    if (odd) {
-                        tt_any(false);   // every row has added them
-                        uint16_t *v = reinterpret_cast<uint16_t *>(smem + (v_ring - base) + vs * TILE);
-                        constexpr uint16_t E = C::BF ? 0x7f80u : 0x7c00u;
-                        for (int b = row; b < TILE / 2; b += 128)
-                            if ((v[b] & E) == E) v[b] = 0;
-                        tt_proxy();
-                        tt_any(false);
-                    }
+                }
+                if (odd) {
+                    tt_add_odd<C::BF>(tmem_o, HD, v, see[0], see[1]);
+                    tt_any(false, bar, voters);   // every row has added them
+                    const int k = row;
+                    if (keeper && k < (1 + two) * 64)
+                        for (int c = 0; c < C::COLS; ++c)
+                            for (int b = 0; b < 64; ++b) {
+                                uint16_t *u = reinterpret_cast<uint16_t *>(v_row(c, k)) + b;
+                                if ((*u & E) == E) *u = 0;
+                            }
+                    tt_proxy();
+                    tt_any(false, bar, voters);
                 }
                 const float shift = C::LIFT - (m == -INFINITY ? 0.0f : m);
-                uint32_t p[32];
-                float sum[2] = {0.0f, 0.0f};
+                const float2 f2 = make_float2(f, f), shift2 = make_float2(shift, shift);
+                float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
 #pragma unroll
-                for (int j = 0; j < 32; ++j) {
-                    const float y0 = ex2(fmaf(x[2 * j], f, shift)), y1 = ex2(fmaf(x[2 * j + 1], f, shift));
-                    sum[0] += y0;
-                    sum[1] += y1;
-                    p[j] = pack2<C::BF>(y0, y1);
+                for (int h = 0; h < 2; ++h) {
+                    if (h && !two) break;
+                    uint32_t p[32];
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) {
+                        float2 y = tt_fma2(make_float2(x[h * 64 + 2 * j], x[h * 64 + 2 * j + 1]), f2, shift2);
+                        y = make_float2(ex2(y.x), ex2(y.y));
+                        sum[j & 1] = tt_add2(sum[j & 1], y);
+                        p[j] = pack2<C::BF>(y.x, y.y);
+                    }
+                    tt_st32(tmem_s + h * 32, p);
                 }
-                l += sum[0] + sum[1];
-                tt_st32(tmem + lane_at + (n & 1) * 64, p);
                 tt_wait_st();
-                // The product of the last page is done before this one may
-                // begin: a phase of o_done can be waited for by its parity only
-                // while it is the last or the next to complete, and S of a page
-                // says no more than that the product two pages back is done.
-                if (n > 0) ok = tt_wait_warp(o_done, (uint32_t)((n - 1) & 1), stop_word, err) && ok;
                 tt_before();
                 __syncwarp();
-                if (lane == 0) tt_arrive(&p_ready[n & 1]);
+                if (lane == 0) tt_arrive(&p_ready[half]);
+                l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
             }
             // the tile's O once its last product is done
-            if (ok && tt_wait_warp(o_done, (uint32_t)((count + pages - 1) & 1), stop_word, err)) {
-                tt_after();
-                const bool whole = p_begin == s.page0 && p_end == s.page1;
-                const size_t part_at = ((size_t)blockIdx.x * 2 + (p_begin == s.page0)) * TT_ROWS + row;
-                const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-                const bool real = node < s.t;
-                uint16_t *to = static_cast<uint16_t *>(a.out) + (real ? (size_t)(s.r0 + node) * a.ldo + (size_t)(kh * g.group + rr - node * g.group) * HD : 0);
-                const bool vec = (a.ldo & 7) == 0 && (reinterpret_cast<uintptr_t>(a.out) & 15) == 0;
-                float *po = g.part + part_at * HD;
-                if (real && !whole) *reinterpret_cast<float2 *>(g.part + (size_t)gridDim.x * 2 * TT_ROWS * HD + part_at * 2) = make_float2(m, l);
-#pragma unroll
+            ok = ok && tt_wait_warp(o_done, (uint32_t)(tiles & 1), stop_word, err);
+            tt_after();
+            float mine = 1.0f, theirs = 0.0f;   // weights of the halves' sums
+            if (split) {
+                if (half == 1) other[row] = make_float2(m, l);
+                tt_any(false, 3, 256);
+                if (half == 0) {
+                    const float2 o = other[row];
+                    const float top = fmaxf(m, o.x), u = top == -INFINITY ? 0.0f : top;
+                    mine = ex2(m - u);
+                    theirs = ex2(o.x - u);
+                    m = top;
+                    l = l * mine + o.y * theirs;
+                }
+            }
+            // O as rows of shared memory (Q, K and V are done with), from where
+            // a warp writes a row at a time; a row is 16 bytes longer than hd
+            // floats, so that eight of them fall into different banks.
+            constexpr int LD = HD + 4;
+            static_assert(2 * TT_ROWS * LD * 4 <= 2 * C::Q_BYTES + (KS + VS) * ROUND, "staging of O");
+            float *stage = reinterpret_cast<float *>(smem) + (size_t)half * TT_ROWS * LD;
+            const bool whole = p_begin == s.page0 && p_end == s.page1, active = ok && (!split || half == 0);
+            if (active) {
+                const float inv = !whole ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
+                mine *= inv;
+                theirs *= inv;
+#pragma unroll 1
                 for (int c = 0; c < HD; c += 32) {
                     float o[32];
-                    tt_ld32(tmem_o + lane_at + c, o);
-                    if (!real) continue;
-                    if (!whole) {
+                    tt_ld32(tmem_o + c, o);
+                    if (split) {
+                        float y[32];
+                        tt_ld32(tmem_o + 128 + c, y);
 #pragma unroll
-                        for (int j = 0; j < 32; j += 4) *reinterpret_cast<float4 *>(po + c + j) = make_float4(o[j], o[j + 1], o[j + 2], o[j + 3]);
+                        for (int j = 0; j < 32; ++j) o[j] = o[j] * mine + y[j] * theirs;
                     } else {
 #pragma unroll
-                        for (int j = 0; j < 32; j += 8) {
-                            const uint4 u = make_uint4(pack2<C::BF>(o[j] * inv, o[j + 1] * inv), pack2<C::BF>(o[j + 2] * inv, o[j + 3] * inv),
-                                                       pack2<C::BF>(o[j + 4] * inv, o[j + 5] * inv), pack2<C::BF>(o[j + 6] * inv, o[j + 7] * inv));
-                            if (vec) {
-                                *reinterpret_cast<uint4 *>(to + c + j) = u;
-                            } else {
-                                const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+                        for (int j = 0; j < 32; ++j) o[j] *= mine;
+                    }
 #pragma unroll
-                                for (int e = 0; e < 8; ++e) to[c + j + e] = (uint16_t)(w[e / 2] >> (16 * (e % 2)));
-                            }
+                    for (int j = 0; j < 32; j += 4) *reinterpret_cast<float4 *>(stage + row * LD + c + j) = make_float4(o[j], o[j + 1], o[j + 2], o[j + 3]);
+                }
+                const size_t part_at = ((size_t)blockIdx.x * 2 + (p_begin == s.page0)) * TC_ROWS + half * TT_ROWS;
+                if (!whole && node < s.t) *reinterpret_cast<float2 *>(g.part + (size_t)gridDim.x * 2 * TC_ROWS * HD + (part_at + row) * 2) = make_float2(m, l);
+                __syncwarp();
+                const int r0 = (warp & 3) * 32;   // the warp's own rows
+                if (!whole) {
+                    constexpr int LANES = HD / 4, ROWS = 32 / LANES;   // lanes of a row, rows at a time
+#pragma unroll 4
+                    for (int i = 0; i < 32; i += ROWS) {
+                        const int r = r0 + i + lane / LANES, d = lane % LANES * 4;
+                        *reinterpret_cast<float4 *>(g.part + (part_at + r) * HD + d) = *reinterpret_cast<const float4 *>(stage + r * LD + d);
+                    }
+                } else {
+                    constexpr int LANES = HD / 4, ROWS = 32 / LANES;
+                    const bool vec = (a.ldo & 3) == 0 && (reinterpret_cast<uintptr_t>(a.out) & 7) == 0;
+#pragma unroll 4
+                    for (int i = 0; i < 32; i += ROWS) {
+                        const int r = r0 + i + lane / LANES, d = lane % LANES * 4, to_rr = s.first + (split ? 0 : half * TT_ROWS) + r, to_node = ta_node(g, to_rr);
+                        if (to_node >= s.t) continue;
+                        const float4 o = *reinterpret_cast<const float4 *>(stage + r * LD + d);
+                        uint16_t *to = static_cast<uint16_t *>(a.out) + (size_t)(s.r0 + to_node) * a.ldo + (size_t)(kh * g.group + to_rr - to_node * g.group) * HD + d;
+                        const uint2 u = make_uint2(pack2<C::BF>(o.x, o.y), pack2<C::BF>(o.z, o.w));
+                        if (vec) {
+                            *reinterpret_cast<uint2 *>(to) = u;
+                        } else {
+                            to[0] = (uint16_t)u.x;
+                            to[1] = (uint16_t)(u.x >> 16);
+                            to[2] = (uint16_t)u.y;
+                            to[3] = (uint16_t)(u.y >> 16);
                         }
                     }
                 }
             }
+            tt_proxy();   // before the next tile's loads into the same memory
             tt_before();
         }
-        count += pages;
-        at += pages;
-        // Q, O and the line are free for the next tile, or a role gave up
+        count += rounds;
+        steps_of[0] += split ? (steps + 1) / 2 : rounds;
+        steps_of[1] += split ? steps / 2 : rounds;
+        ++tiles;
+        at += places;
+        // Q, O and the rings are free for the next tile, or a role gave up
         if (__syncthreads_or(*stop_word)) break;
         tt_after();
     }
     // Loads that nobody waited for (after a wait that gave up) land before the
     // shared memory goes away, bounded; then the columns are freed.
-    if (warp == 5 && lane == 0 && *stop_word)
+    if (warp == 9 && lane == 0 && *stop_word)
         for (int j = 0; j < KS + VS; ++j) {
             const int n = j < KS ? k_issued - 1 - j : v_issued - 1 - (j - KS);
             for (uint32_t i = 0; n >= 0 && i < (1u << 20); ++i)
                 if (j < KS ? ec_mbar_try_wait(&k_full[n % KS], (uint32_t)((n / KS) & 1)) : ec_mbar_try_wait(&v_full[n % VS], (uint32_t)((n / VS) & 1))) break;
         }
-    if (warp == 4 && lane == 0) {
-        tt_commit(drain);     // every MMA that was issued is complete once this fires
+    if (warp == 8) {
+        tt_commit(ec_smem_u32(drain));   // every MMA that was issued is complete once this fires
         for (uint32_t i = 0; i < (1u << 24); ++i)
             if (ec_mbar_try_wait(drain, 0)) break;
     }
     tt_before();
     __syncthreads();
-    if (warp == 4) {
+    if (warp == 8) {
         __syncwarp();
         tt_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(C::TMEM));
@@ -491,7 +621,7 @@ int map_of(CUtensorMap *map, const void *p, const ec_kv_pages &kv) {
 template <int QT, int KT, int HD>
 int launch(const ec_kv_pages &kv, const ec_tree_attn &a, const TaGeo &g, int pieces, int id, int *err, cudaStream_t stream) {
     typedef TtCfg<QT, KT, HD> C;
-    static_assert(C::SMEM <= 114 * 1024 - 1024, "two CTAs per SM");
+    static_assert(C::SMEM <= 232448, "shared memory per CTA");
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return (int)e;
