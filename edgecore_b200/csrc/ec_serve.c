@@ -142,7 +142,7 @@ EC_EXPORT int ec_tree_commit(const ec_kv_pages *kv, const ec_tree_path *a, void 
     static const char fn[] = "ec_tree_commit";
     if (check_pages(fn, kv)) return -1;
     if (!a) return refuse("%s: no arguments", fn);
-    if (a->n_seq < 0 || a->rows < 0) return refuse("%s: n_seq %d, rows %d", fn, a->n_seq, a->rows);
+    if (a->n_seq < 0 || a->n_seq > 0x0fffffff || a->rows < 0) return refuse("%s: n_seq %d, rows %d", fn, a->n_seq, a->rows);
     if (a->mask_words < 1 || a->max_path < 1) return refuse("%s: mask_words %d, max_path %d", fn, a->mask_words, a->max_path);
     if (a->n_seq == 0) return 0;
     int dev, sms;
@@ -163,7 +163,7 @@ EC_EXPORT int ec_kv_copy(const ec_kv_pages *kv, int n_copies, const int *src, co
 {
     static const char fn[] = "ec_kv_copy";
     if (check_pages(fn, kv)) return -1;
-    if (n_copies < 0 || n_copies > 65535) return refuse("%s: %d copies", fn, n_copies);
+    if (n_copies < 0 || n_copies > EC_KV_COPY_MAX) return refuse("%s: %d copies (at most %d)", fn, n_copies, EC_KV_COPY_MAX);
     if (n_copies == 0) return 0;
     int dev, sms;
     if (current_device(fn, &dev, &sms)) return -1;

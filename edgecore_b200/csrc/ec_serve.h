@@ -21,6 +21,8 @@ int ec_launch_tree_commit(const ec_kv_pages *kv, const ec_tree_path *a, int *err
 int ec_launch_kv_copy(const ec_kv_pages *kv, int n, const int *src, const int *dst, const int *start, const int *end,
                       int num_sms, int *err, cudaStream_t stream);
 
+#define EC_KV_COPY_MAX 4096          /* jobs of a call: every CTA keeps a flag of each */
+
 typedef struct {
     int *ids;
     float *prob;

@@ -715,10 +715,16 @@ TaPlan ta_plan(int n_seq, int rows, int n_head, int n_kv_head, int hd, int max_l
     p.tiles = (int)(((long long)rows * p.g.group) / p.mt + n_seq);   // every sequence rounds up once; rows * group fits 31 bits
     int pages = ta_up(max_len > 0 ? max_len : 1, PAGE);
     if (window > 0 && pages > window / PAGE + 2) pages = window / PAGE + 2;
-    p.g.cluster = pages >= 8 ? 8 : pages >= 4 ? 4 : pages >= 2 ? 2 : 1;
+    // Up to 16 pages a tile is one cluster's, of as many CTAs as two rounds of
+    // the SMs hold: 24 windowed sequences of 10 pages, 12 heads, take 20 us so
+    // and 31 us as equal pieces with a second launch.  Beyond, ragged lengths
+    // leave clusters waiting: 32 sequences of 65 to 1900 positions take 33 us
+    // as pieces, 34 to 39 us as clusters.
     const long long tiles = (long long)p.tiles * n_kv_head;
+    p.g.cluster = pages >= 8 ? 8 : pages >= 4 ? 4 : pages >= 2 ? 2 : 1;
+    while (p.g.cluster > 1 && tiles * p.g.cluster > 2 * sms) p.g.cluster /= 2;
     p.pieces = 0;
-    if (!(pages <= 16 && tiles * p.g.cluster <= sms) && tiles * slot_pages <= 0x7fffffff)
+    if (pages > 16 && tiles * slot_pages <= 0x7fffffff)
         p.pieces = (p.mt == TC_ROWS ? 1 : p.hdp == 64 && !f32 ? 3 : p.hdp <= 128 ? 2 : 1) * sms;
     if (!p.pieces && p.mt == TC_ROWS) {   // clusters: the register tiles only
         p.mt = 64;

@@ -346,7 +346,7 @@ typedef struct {
 int ec_tree_commit(const ec_kv_pages *kv, const ec_tree_path *a, void *stream);
 
 /* Copy the K and V of positions [start[j], end[j]) in every layer from slot
- * src[j] to slot dst[j], for n_copies jobs (DEVICE int arrays).  A job whose
+ * src[j] to slot dst[j], for n_copies jobs (DEVICE int arrays; at most 4096).  A job whose
  * target is written or read by another job at a common position, or is its
  * own source, is skipped and reported (code 2), and so is one with a bad
  * slot or range; an empty range copies nothing. */

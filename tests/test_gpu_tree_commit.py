@@ -194,3 +194,40 @@ def test_copy_with_an_unmapped_page(cuda):
     assert ec.device_error_take() == 2
     for x, y in zip(a.host(), want):
         assert (x == y).all()
+
+
+@pytest.mark.parametrize("back,step", [(3, 2), (700, 1), (1500, 150)])
+def test_trees_of_many_nodes(cuda, back, step):
+    """Paths that go on after gaps of one node, of some hundred, and of more than the nodes a block holds."""
+    a = Arena(cuda, 2, 72, 2, 30, seed=11)
+    trees = []
+    for _ in range(2):
+        parents, tokens, picked = random_tree(a.rs, 1700, 50, back)
+        node = 0
+        while True:                      # a path that reaches the last nodes
+            to = [c for c in range(node + 1, min(1700, node + 2 * step + 1)) if c - node >= min(step, 1699 - node)]
+            if not to:
+                break
+            child = to[int(a.rs.randint(len(to)))]
+            parents[child], tokens[child] = node, picked[node]
+            node = child
+        trees.append((parents, tokens, picked))
+    assert min(commit(a, trees, [0, 99], 900, slots=[1, 0])) > 1
+
+
+def test_copies_of_many_jobs(cuda):
+    """More jobs than a block judges at a time: forks of two sources in groups, ranges of their own, bad ones among them."""
+    a = Arena(cuda, 2, 24, 310, 2, seed=12)
+    jobs = [(0, d, 3, 100) for d in range(2, 150)] + [(1, d, 0, 64) for d in range(150, 280)] + [(1, d, d - 280, 90) for d in range(280, 305)]
+    jobs = [jobs[i] for i in a.rs.permutation(len(jobs))]
+    bad = [(0, 400, 3, 100), (0, 0, 3, 100), (-1, 305, 0, 9)]
+    want = a.host()
+    for s, d, lo, hi in jobs:
+        for p in range(lo, hi):
+            for x in want:
+                x[:, a.at(d, p)] = x[:, a.at(s, p)]
+    for extra in ([], bad):
+        ec.kv_copy(a.k, a.v, a.dev(a.table), *(a.dev(c) for c in zip(*(extra + jobs))))
+        assert ec.device_error_take() == (2 if extra else 0)
+    for x, y in zip(a.host(), want):
+        assert (x == y).all()
