@@ -9,8 +9,8 @@ namespace {
 constexpr int PG_THREADS = 256;
 constexpr int PG_NODES = 512;               // nodes of a tree that a block walks at a time
 constexpr int PG_BATCH = 8;                 // rows of a column in flight
-constexpr int PG_SHARES = 8;                // CTAs of a sequence, at most
-constexpr int PC_VECTORS = 4;               // 16-byte vectors of a thread in flight
+constexpr int PG_SHARES = 4;                // CTAs of a sequence, at most
+constexpr int PC_VECTORS = 8;               // 16-byte vectors of a thread in flight
 constexpr int PC_JOBS = EC_KV_COPY_MAX;
 
 // Element offset of position p of `slot` in a layer; -1 (and the error word)
@@ -57,7 +57,11 @@ EC_DEV uint16_t *pg_column(const ec_kv_pages &kv, int i, int cols) {   // the i-
 // batch nor a later block reads a row that was overwritten before.  Only the
 // cluster's first CTA writes the results, after all have read base, which
 // new_base may be.
-__global__ void __launch_bounds__(PG_THREADS) k_tree_commit(const ec_kv_pages kv, const ec_tree_path a, int shares, int *err) {
+// One stream (17 nodes, 24 layers of 128): 4.0 us, the latency of launch and
+// three reads.  128 sequences of 41 nodes that accept 0 to 8, 28 layers of
+// 256 (29 MB): 8.9 us, 3.3 TB/s, with 4 CTAs a sequence, which all fit at
+// once; 18 us with 8, which do not, 10 us with 2; 9.4 us with 4 rows in flight.
+__global__ void __launch_bounds__(PG_THREADS, 4) k_tree_commit(const ec_kv_pages kv, const ec_tree_path a, int shares, int *err) {
     EC_PDL_ENTER();
     __shared__ int s_child[PG_NODES], s_token[PG_NODES], s_picked[PG_NODES], s_path[PG_NODES];
     __shared__ long long s_row[PG_NODES], s_from[PG_NODES], s_to[PG_NODES];
@@ -145,26 +149,31 @@ __global__ void __launch_bounds__(PG_THREADS) k_tree_commit(const ec_kv_pages kv
 // once and written to every member: n forks of a prompt cost one read and n
 // writes.  Every CTA judges all jobs (flags in shared memory), counts the
 // groups' units -- PC_VECTORS x PG_THREADS vectors of 16 bytes, of one layer's
-// K or V and within one page -- and takes every gridDim-th.
+// K or V and within one page -- and takes every gridDim-th.  16 forks of 1733
+// positions, 28 layers of 256 (845 MB): 153 us, 5.5 TB/s, bound by the writes
+// (264 us when every job read for itself; 155 us with 4 vectors and twice the
+// CTAs).  One fork of 45 positions, 12 layers of 768: 5.7 us, half of it the
+// judging; 8 CTAs an SM take 6.4 us, 2 take 5.0 us but 158 us for the 16.
 __global__ void __launch_bounds__(PG_THREADS) k_kv_copy(const ec_kv_pages kv, int n, const int *src, const int *dst,
                                                         const int *start, const int *end, int *err) {
     EC_PDL_ENTER();
     __shared__ int4 s_job[PG_THREADS];
     __shared__ unsigned char s_flag[PC_JOBS];         // 1: skipped, 2: not its group's first
     __shared__ unsigned short s_member[PC_JOBS];      // the group's jobs that are not skipped
-    __shared__ long long s_sum[PG_THREADS], s_to[PG_THREADS];
+    __shared__ long long s_warp[PG_THREADS / 32], s_sum[PG_THREADS], s_to[PG_THREADS];
     __shared__ int s_members;
     const int tid = threadIdx.x;
-    const auto job = [&](int j) { return make_int4(src[j], dst[j], start[j], end[j]); };
+    // up to PG_THREADS jobs s_job keeps all of them
+    const auto job = [&](int j) { return n <= PG_THREADS ? s_job[j] : make_int4(src[j], dst[j], start[j], end[j]); };
     for (int j0 = 0; j0 < n; j0 += PG_THREADS) {
         const int j = j0 + tid;
         int4 me = make_int4(0, 0, 0, 0);
-        if (j < n) me = job(j);
+        if (j < n) me = make_int4(src[j], dst[j], start[j], end[j]);
         bool bad = me.x < 0 || me.x >= kv.n_slots || me.y < 0 || me.y >= kv.n_slots || me.z < 0 ||
                    (long long)me.w > (long long)kv.pages_per_slot * EC_KV_PAGE || (me.x == me.y && me.z < me.w), later = false;
         for (int i0 = 0; i0 < n; i0 += PG_THREADS) {
             __syncthreads();
-            if (i0 + tid < n) s_job[tid] = i0 == j0 ? me : job(i0 + tid);
+            if (i0 + tid < n) s_job[tid] = i0 == j0 ? me : make_int4(src[i0 + tid], dst[i0 + tid], start[i0 + tid], end[i0 + tid]);
             __syncthreads();
             const int m = min(PG_THREADS, n - i0);
             for (int i = 0; i < m; ++i) {
@@ -188,17 +197,19 @@ __global__ void __launch_bounds__(PG_THREADS) k_kv_copy(const ec_kv_pages kv, in
         long long units = 0;
         __syncthreads();
         if (j < n && !(s_flag[j] & 2)) {
-            const int p0 = start[j], p1 = end[j];
+            const int4 me = job(j);
+            const int p0 = me.z, p1 = me.w;
             if (p0 >= 0 && p0 < p1 && (long long)p1 <= (long long)kv.pages_per_slot * EC_KV_PAGE)
                 units = (long long)((p1 - 1) / rows - p0 / rows + 1) * 2 * kv.n_layers;
         }
-        s_sum[tid] = units;
-        for (int step = 1; step < PG_THREADS; step *= 2) {
-            __syncthreads();
-            const long long before = tid >= step ? s_sum[tid - step] : 0;
-            __syncthreads();
-            s_sum[tid] += before;
+        for (int step = 1; step < 32; step *= 2) {
+            const long long before = __shfl_up_sync(~0u, units, step);
+            if (tid % 32 >= step) units += before;
         }
+        if (tid % 32 == 31) s_warp[tid / 32] = units;
+        __syncthreads();
+        for (int w = 0; w < tid / 32; ++w) units += s_warp[w];
+        s_sum[tid] = units;
         __syncthreads();
         const long long total = s_sum[PG_THREADS - 1];
         int at = -1;
@@ -216,9 +227,11 @@ __global__ void __launch_bounds__(PG_THREADS) k_kv_copy(const ec_kv_pages kv, in
                 __syncthreads();
                 if (tid == 0) s_members = 0;
                 __syncthreads();
-                for (int i = tid; i < n; i += PG_THREADS)
-                    if (!(s_flag[i] & 1) && src[i] == lead.x && start[i] == lead.z && end[i] == lead.w)
+                for (int i = tid; i < n; i += PG_THREADS) {
+                    const int4 me = job(i);
+                    if (!(s_flag[i] & 1) && me.x == lead.x && me.z == lead.z && me.w == lead.w)
                         s_member[atomicAdd(&s_members, 1)] = (unsigned short)i;   // any order: targets are apart
+                }
                 __syncthreads();
             }
             const int members = s_members;
@@ -232,7 +245,7 @@ __global__ void __launch_bounds__(PG_THREADS) k_kv_copy(const ec_kv_pages kv, in
             for (int m0 = 0; m0 < members; m0 += PG_THREADS) {
                 const int m1 = min(PG_THREADS, members - m0);
                 __syncthreads();
-                if (tid < m1) s_to[tid] = pg_row(kv, dst[s_member[m0 + tid]], p0, err);
+                if (tid < m1) s_to[tid] = pg_row(kv, job(s_member[m0 + tid]).y, p0, err);
                 __syncthreads();
                 if (from < 0) continue;
                 for (int i0 = tid; i0 < count; i0 += PC_VECTORS * PG_THREADS) {
@@ -279,6 +292,6 @@ extern "C" int ec_launch_tree_commit(const ec_kv_pages *kv, const ec_tree_path *
 
 extern "C" int ec_launch_kv_copy(const ec_kv_pages *kv, int n, const int *src, const int *dst, const int *start,
                                  const int *end, int num_sms, int *err, cudaStream_t stream) {
-    k_kv_copy<<<8 * num_sms, PG_THREADS, 0, stream>>>(*kv, n, src, dst, start, end, err);
+    k_kv_copy<<<4 * num_sms, PG_THREADS, 0, stream>>>(*kv, n, src, dst, start, end, err);
     return (int)cudaGetLastError();
 }

@@ -99,6 +99,7 @@ def test_tree_commit(built, kw, error, says):
     (dict(dst=torch.zeros(3, dtype=torch.int32)), ValueError, "dst"),
     (dict(start=torch.zeros(2)), ValueError, "start"),
     (dict(end=torch.zeros(4, dtype=torch.int32)[::2]), ValueError, "end"),
+    (dict(zip(("src", "dst", "start", "end"), [torch.zeros(4097, dtype=torch.int32)] * 4)), RuntimeError, "4096"),
     (dict(), RuntimeError, "device"),
 ])
 def test_kv_copy(built, kw, error, says):
@@ -153,3 +154,8 @@ def test_tree_mask():
     for bad in ([0], [-2], [-1, 1], [-1, 0, 5]):
         with pytest.raises(ValueError):
             ec.tree_mask(bad)
+
+
+def test_sample_refuses_a_vocabulary_beyond_shared_memory(built):
+    with pytest.raises(RuntimeError, match="750000"):
+        ec.sample(torch.zeros(1, dtype=torch.int32), torch.zeros(1, 750001), torch.zeros(1))
