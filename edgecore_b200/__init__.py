@@ -61,6 +61,9 @@ def _declare(lib: C.CDLL) -> None:
         "ec_tree_commit": (_i, [_vp, _vp, _vp]),
         "ec_kv_copy": (_i, [_vp, _i, _vp, _vp, _vp, _vp, _vp]),
         "ec_sample": (_i, [_vp, _vp, _vp, _i, C.c_longlong, _i, _i, _vp, _vp, _vp, _vp, _vp, _vp]),
+        "ec_forward_tree": (_i, [_vp, _vp, _vp, _vp, _vp, _vp]),
+        "ec_kv_fork": (_i, [_vp, _i, _vp, _i, _i]),
+        "ec_decode_sample": (_i, [_vp, _vp, _vp, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
         "ec_model_set_taps": (_i, [_vp, _i]),
         "ec_model_get_taps": (_i, [_vp, _vp, _i]),
         "ec_model_set_vocab_shard": (_i, [_vp, _i, _i]),
@@ -264,6 +267,12 @@ class _TreePath(C.Structure):
     _fields_ = [("n_seq", _i), ("rows", _i), ("mask_words", _i), ("max_path", _i), ("slots", _vp), ("row_start", _vp),
                 ("base", _vp), ("mask", _vp), ("tokens", _vp), ("picked", _vp), ("accepted", _vp), ("n_accepted", _vp),
                 ("new_base", _vp)]
+
+
+class _TreeStep(C.Structure):
+    """ec_tree_step"""
+    _fields_ = [("n_seq", _i), ("max_path", _i), ("slots", _vp), ("row_start", _vp), ("base", _vp), ("tokens", _vp),
+                ("parents", _vp), ("u", _vp), ("temperature", _vp), ("top_p", _vp), ("min_p", _vp), ("top_k", _vp)]
 
 
 _TYPES = {"torch.float32": 0, "torch.float16": 1, "torch.bfloat16": 2, "torch.int32": 3, "torch.int64": 4}
@@ -509,6 +518,62 @@ class Model:
         self._check(self.lib.ec_decode_batch(self.h, _ptr(d_tokens), _ptr(d_positions), int(n_steps),
                                              _ptr(d_out_ids)))
 
+    def decode_sample(self, d_tokens, d_positions, n_steps: int, d_u, temperature=None, top_k=None, top_p=None, min_p=None,
+                      d_out_ids=None, d_out_prob=None) -> None:
+        """decode_batch with every token drawn by sample(): step s of slot m uses d_u[s][m] (device fp32
+        [n_steps][batch_cap]) and the slot's settings (device arrays [batch_cap]; top_k int32, the others fp32; None: off);
+        ids and, fp32, their probabilities into d_out_ids and d_out_prob [n_steps][batch_cap] when given."""
+        self._check(self.lib.ec_decode_sample(self.h, _ptr(d_tokens), _ptr(d_positions), int(n_steps), _ptr(d_u), _ptr(temperature),
+                                              _ptr(top_k), _ptr(top_p), _ptr(min_p), _ptr(d_out_ids), _ptr(d_out_prob)))
+
+    def forward_tree(self, trees, base, slots=None, max_path: int | None = None, u=None, temperature=None, top_k=None, top_p=None,
+                     min_p=None) -> dict:
+        """One step of drafted trees (ec_forward_tree).  trees: (tokens, parents) of each sequence, the root first with parent
+        -1: the last token that is not in the cache yet.  base: committed positions of each.  With u (one number in [0, 1) per
+        node of all trees in order) the choices are drawn as by sample(), with settings per node (or one number for all);
+        without, they are the argmax.  The accepted rows are committed.  Returns accepted (a list of tokens per sequence, the
+        last of them the next root), picked (the choice after every node) and, with u, prob."""
+        trees = [(_np(t, np.int32).reshape(-1), _np(p, np.int32).reshape(-1)) for t, p in trees]
+        n = len(trees)
+        for t, p in trees:
+            if len(t) != len(p):
+                raise ValueError(f"a tree has {len(t)} tokens and {len(p)} parents")
+        base = _np(base, np.int32).reshape(-1)
+        slots = None if slots is None else _np(slots, np.int32).reshape(-1)
+        if len(base) != n or (slots is not None and len(slots) != n):
+            raise ValueError(f"{n} trees need {n} bases and slots")
+        start = np.zeros(n + 1, np.int32)
+        start[1:] = np.cumsum([len(t) for t, _ in trees])
+        rows = int(start[n])
+        tokens, parents = (np.concatenate([t[i] for t in trees] + [np.zeros(0, np.int32)]) for i in range(2))
+        if max_path is None:
+            max_path = max([1] + [len(t) for t, _ in trees])
+
+        def each(v, dtype, name):
+            if v is None:
+                return None
+            v = np.ascontiguousarray(np.broadcast_to(np.asarray(v, dtype), (rows,)) if np.ndim(v) == 0 else np.asarray(v, dtype))
+            if v.shape != (rows,):
+                raise ValueError(f"{name} must be one number or {rows}, one for each node")
+            return v
+
+        if u is not None and np.ndim(u) == 0 and rows != 1:
+            raise ValueError("u must have one number for each node")
+        vals = [each(v, t, k) for v, t, k in ((u, np.float32, "u"), (temperature, np.float32, "temperature"), (top_p, np.float32, "top_p"),
+                                              (min_p, np.float32, "min_p"), (top_k, np.int32, "top_k"))]
+        step = _TreeStep(n, int(max_path), _ptr(slots), _ptr(start), _ptr(base), _ptr(tokens), _ptr(parents), *(_ptr(v) for v in vals))
+        picked, prob = np.empty(rows, np.int32), np.empty(rows, np.float32)
+        accepted, count = np.empty((n, max(1, int(max_path))), np.int32), np.empty(n, np.int32)
+        self._check(self.lib.ec_forward_tree(self.h, C.addressof(step), _ptr(picked), _ptr(prob) if u is not None else None, _ptr(accepted),
+                                             _ptr(count)))
+        out = {"accepted": [accepted[b, :count[b]].tolist() for b in range(n)], "picked": picked}
+        return out | {"prob": prob} if u is not None else out
+
+    def kv_fork(self, src: int, dst, length: int) -> None:
+        """Slots dst take over positions [0, length) of slot src, copied into pages of their own (ec_kv_fork)."""
+        dst = _np(dst, np.int32).reshape(-1)
+        self._check(self.lib.ec_kv_fork(self.h, int(src), _ptr(dst), len(dst), int(length)))
+
     def batch_hidden(self, d_tokens, d_positions, M: int, max_pos_end: int, d_hidden) -> None:
         """Rows m < M (slot m) through every layer and the final norm into
         d_hidden [M][n_embd] fp32 (device); every position < max_pos_end."""
@@ -551,7 +616,7 @@ class Model:
         return out.reshape(N, ldw * elt), {"N": N, "K": K, "Kp": Kp, "ldw": ldw, "elt": elt}
 
     def batch_graph_kernels(self, kind: int) -> int:
-        """Kernel launches in the captured step graph (0: decode_batch, 1: batch_hidden)."""
+        """Kernel launches in the captured step graph (0: decode_batch, 1: batch_hidden, 2: decode_sample)."""
         n = self.lib.ec_batch_graph_kernels(self.h, int(kind))
         if n < 0:
             raise RuntimeError(last_error())

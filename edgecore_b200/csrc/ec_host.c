@@ -23,6 +23,7 @@
 #include "edgecore.h"
 #include "edgecore_b200.h"
 #include "ec_launch.h"
+#include "ec_serve.h"
 #include "ec_decode.h"
 
 #include <cuda_runtime_api.h>
@@ -273,11 +274,18 @@ typedef struct ec_dev {
     float *h_logits;
     size_t h_logits_cap;
     /* batched decode: one captured CUDA graph per step shape (0: full greedy
-     * step, 1: hidden rows only); ws_gen counts workspace reallocations and
+     * step, 1: hidden rows only, 2: sampled step); ws_gen counts workspace reallocations and
      * vocab-shard changes, which invalidate the graphs */
-    struct { cudaGraphExec_t exec; int M, maxlen, chunk, hist, kernels; unsigned gen; } bg[2];
+    struct { cudaGraphExec_t exec; int M, maxlen, chunk, hist, kernels; unsigned gen; } bg[3];
     unsigned ws_gen;
     int *d_counter;
+    /* operands of tree steps, forks and sampled steps: pinned staging and its
+     * device copy, and the tree attention's partial sums */
+    char *h_ops, *d_ops;
+    size_t ops_cap;
+    void *tree_work;
+    size_t tree_work_bytes;
+    float *d_samp;             /* sampled decode: u | temperature | top_p | min_p | prob | top_k, each [B] */
     /* taps */
     int taps_on;
     float *taps;
@@ -733,7 +741,8 @@ static void ec_dev_free(ec_dev *d)
     cudaFree(d->attn_part); cudaFree(d->logits); cudaFree(d->amax_part); cudaFree(d->lm_part);
     cudaFree(d->d_hist); cudaFree(d->taps); cudaFree(d->d_counter);
     cudaFree(d->acc32); cudaFree(d->tile_cnt);
-    for (int k = 0; k < 2; k++)
+    cudaFreeHost(d->h_ops); cudaFree(d->d_ops); cudaFree(d->tree_work); cudaFree(d->d_samp);
+    for (int k = 0; k < 3; k++)
         if (d->bg[k].exec) cudaGraphExecDestroy(d->bg[k].exec);
     cudaFreeHost(d->h_logits);
     if (d->prof_ready)
@@ -1159,9 +1168,18 @@ static int ec_linear(ec_dev *d, const ec_lin *l, const float *X, int ldx, int M,
     return 0;
 }
 
+/* Rows that are nodes of drafted trees: their positions in the cache, which
+ * differ from those in the text, and the attention over them. */
+typedef struct {
+    ec_tree_attn at;
+    ec_kv_pages kv;            /* layer 0 */
+    const int *row;            /* device [M] */
+} ec_tree_rows;
+
 /* Per-layer kernels for rows already staged in d_tok/d_pos/d_slot: the
- * prefill path.  Leaves the normed final hidden state in d->h. */
-static int ec_enqueue_body(ec_dev *d, int M, int maxlen)
+ * prefill path, or with `tree` the nodes of drafted trees.  Leaves the normed
+ * final hidden state in d->h. */
+static int ec_enqueue_body(ec_dev *d, int M, int maxlen, const ec_tree_rows *tree)
 {
     cudaStream_t st = d->stream;
     const int E = d->E, ldqkv = E + 2 * d->kv;
@@ -1189,11 +1207,19 @@ static int ec_enqueue_body(ec_dev *d, int M, int maxlen)
         ec_prof_end(d, pi);
         if (ec_linear(d, &W->qkv, fuse_norm ? NULL : d->h, E, M, d->qkv, ldqkv, EC_EPI_STORE)) return -1;
         pi = ec_prof_begin(d, EC_PC_OTHER, 0.0);
-        CK(ec_launch_qkv_split(d->q, d->qkv, ldqkv, ec_tk(d), ec_geo(d, l), d->H, d->KVH, d->arch == ARCH_QWEN2, M, st));
+        CK(ec_launch_qkv_split(d->q, d->qkv, ldqkv, ec_tk(d), tree ? tree->row : NULL, ec_geo(d, l), d->H, d->KVH,
+                               d->arch == ARCH_QWEN2, M, st));
         ec_prof_end(d, pi);
         at.geo = ec_geo(d, l);
         pi = ec_prof_begin(d, EC_PC_ATTN, 0.0);
-        CK(ec_launch_attention(&at, st));
+        if (tree) {
+            ec_kv_pages kv = tree->kv;
+            kv.k = d->kc + d->layer_kv * l;
+            kv.v = d->vc + d->layer_kv * l;
+            CK(ec_launch_tree_attention(&kv, &tree->at, d->num_sms, ec_error_word(), st));
+        } else {
+            CK(ec_launch_attention(&at, st));
+        }
         ec_prof_end(d, pi);
         if (ec_linear(d, &W->o, d->att, E, M, d->x, E, EC_EPI_RESID)) return -1;
         pi = ec_prof_begin(d, EC_PC_NORM, 8.0 * M * E);
@@ -1564,7 +1590,7 @@ static int ec_forward_impl(GPT2 *g, const int *tokens, const int *positions, con
         CK(cudaMemcpyAsync(d->d_blk, d->h_blk, (size_t)nb * 8, cudaMemcpyHostToDevice, d->stream));
         d->nblk = nb;
     }
-    const int body = ec_enqueue_body(d, M, maxlen);
+    const int body = ec_enqueue_body(d, M, maxlen, NULL);
     d->nblk = 0;
     if (body) return -1;
     int chunk = (int)((256u << 20) / ((size_t)Vs * 4));
@@ -1773,6 +1799,43 @@ static int ec_enqueue_lm_argmax(ec_dev *d, int M, int chunk)
     return 0;
 }
 
+/* Per-row sampling settings, device arrays (ec_sample). */
+typedef struct {
+    const float *u, *temperature, *top_p, *min_p;
+    const int *top_k;
+    float *prob;
+} ec_sampling;
+
+/* lm_head over rows [0, M) of d->h and a token drawn for each into d_ids,
+ * chunk rows at a time. */
+static int ec_enqueue_lm_sample(ec_dev *d, int M, int chunk, ec_sampling sp)
+{
+    for (int r0 = 0; r0 < M; r0 += chunk) {
+        const int rows = M - r0 < chunk ? M - r0 : chunk;
+        if (ec_enqueue_lm(d, r0, rows)) return -1;
+        const ec_sample_args a = {d->d_ids + r0, sp.prob ? sp.prob + r0 : NULL, d->logits, d->V, EC_T_F32, rows, d->V,
+                                  sp.temperature + r0, sp.top_k + r0, sp.top_p + r0, sp.min_p + r0, sp.u + r0};
+        CK(ec_launch_sample(&a, d->num_sms, ec_error_word(), d->stream));
+    }
+    return 0;
+}
+
+static ec_sampling ec_batch_sampling(const ec_dev *d)
+{
+    float *f = d->d_samp;
+    const size_t B = (size_t)d->B;
+    const ec_sampling sp = {f, f + B, f + 2 * B, f + 3 * B, (const int *)(f + 5 * B), f + 4 * B};
+    return sp;
+}
+
+/* Sampling draws over the whole vocabulary. */
+static int ec_check_sampling(const char *fn, const ec_dev *d)
+{
+    if (d->v0 != 0 || d->v1 != d->V) { ec_seterr("%s: the model holds a vocabulary shard, sampling needs all of it", fn); return -1; }
+    if (d->V > EC_SAMPLE_MAX_VOCAB) { ec_seterr("%s: vocabulary %d (at most %d)", fn, d->V, EC_SAMPLE_MAX_VOCAB); return -1; }
+    return 0;
+}
+
 /* Workspaces of a batched call of M rows (slot m = row m) attending at most
  * maxlen positions, with lm_head chunks of `chunk` rows; kernel set-up done
  * here so that nothing allocates or sets attributes during graph capture. */
@@ -1791,7 +1854,8 @@ static int ec_batch_prepare(ec_dev *d, int M, int maxlen, int chunk)
 }
 
 /* The captured graph of kind k (0: body + lm_head argmax + token/position
- * advance; 1: body only, normed rows left in d->h), rebuilt when the shape or
+ * advance; 1: body only, normed rows left in d->h; 2: as 0 with the token
+ * sampled by the settings in d_samp), rebuilt when the shape or
  * a workspace changed. */
 static int ec_bgraph(ec_dev *d, int kind, int M, int maxlen, int chunk, int hist, cudaGraphExec_t *out)
 {
@@ -1807,9 +1871,10 @@ static int ec_bgraph(ec_dev *d, int kind, int M, int maxlen, int chunk, int hist
     cudaGraph_t gr = NULL;
     CK(cudaStreamBeginCapture(d->stream, cudaStreamCaptureModeThreadLocal));
     int rc = 0;
-    rc = ec_enqueue_body(d, M, maxlen);
+    rc = ec_enqueue_body(d, M, maxlen, NULL);
     if (!rc && kind == 0) rc = ec_enqueue_lm_argmax(d, M, chunk);
-    if (!rc && kind == 0 &&
+    if (!rc && kind == 2) rc = ec_enqueue_lm_sample(d, M, chunk, ec_batch_sampling(d));
+    if (!rc && kind != 1 &&
         ec_launch_step_advance(d->d_tok, d->d_pos, d->d_ids, M, hist ? d->d_hist : NULL, hist ? d->d_counter : NULL,
                                0, 0, d->stream))
         rc = -1;
@@ -1856,12 +1921,10 @@ static int ec_batch_len(const ec_dev *d, int max_pos_end)
     return ec_len_bucket(d, len);
 }
 
-EC_EXPORT int ec_decode_batch(GPT2 *g, int *d_tokens, int *d_positions, int n_steps, int *d_out_ids)
+/* The slots' positions read back and their pages mapped for n_steps more;
+ * returns the end of the furthest, or -1. */
+static int ec_batch_positions(ec_dev *d, const int *d_positions, int n_steps)
 {
-    ec_dev *d = ec_lookup(g);
-    if (!d) { ec_seterr("model not loaded"); return -1; }
-    if (n_steps < 0) { ec_seterr("n_steps must be >= 0"); return -1; }
-    if (n_steps == 0) return 0;
     const int M = d->B;
     if (ec_ensure(d, M)) return -1;
     CK(cudaStreamSynchronize(d->stream));
@@ -1878,7 +1941,18 @@ EC_EXPORT int ec_decode_batch(GPT2 *g, int *d_tokens, int *d_positions, int n_st
         if (p + n_steps > maxp) maxp = p + n_steps;
         if (ec_kv_map(d, m, p + n_steps)) return -1;
     }
-    if (ec_kv_flush(d)) return -1;
+    return ec_kv_flush(d) ? -1 : maxp;
+}
+
+EC_EXPORT int ec_decode_batch(GPT2 *g, int *d_tokens, int *d_positions, int n_steps, int *d_out_ids)
+{
+    ec_dev *d = ec_lookup(g);
+    if (!d) { ec_seterr("model not loaded"); return -1; }
+    if (n_steps < 0) { ec_seterr("n_steps must be >= 0"); return -1; }
+    if (n_steps == 0) return 0;
+    const int M = d->B;
+    const int maxp = ec_batch_positions(d, d_positions, n_steps);
+    if (maxp < 0) return -1;
     if (M < EC_TC_MIN_M) {   /* up to 7 streams: the persistent decode kernel, one launch for all steps;
                                from 8 the per-layer graph with tensor-core GEMMs is faster */
         int max_len = maxp;
@@ -1927,6 +2001,274 @@ EC_EXPORT int ec_decode_batch(GPT2 *g, int *d_tokens, int *d_positions, int n_st
     CK(cudaMemcpyAsync(d_positions, d->d_pos, (size_t)M * 4, cudaMemcpyDeviceToDevice, d->stream));
     if (d_out_ids)
         CK(cudaMemcpyAsync(d_out_ids, d->d_hist, (size_t)n_steps * M * 4, cudaMemcpyDeviceToDevice, d->stream));
+    return 0;
+}
+
+/* Pinned staging and device operands of at least `bytes`; the stream is idle
+ * afterwards, so that the staging can be written. */
+static int ec_ops(ec_dev *d, size_t bytes)
+{
+    CK(cudaStreamSynchronize(d->stream));
+    if (bytes <= d->ops_cap) return 0;
+    cudaFreeHost(d->h_ops);
+    cudaFree(d->d_ops);
+    d->h_ops = d->d_ops = NULL;
+    d->ops_cap = 0;
+    bytes = (bytes + 4095) & ~(size_t)4095;
+    CK(cudaMallocHost((void **)&d->h_ops, bytes));
+    CK(cudaMalloc((void **)&d->d_ops, bytes));
+    d->ops_cap = bytes;
+    return 0;
+}
+
+/* The model of a call, its device current; NULL with a message. */
+static ec_dev *ec_enter(const GPT2 *g)
+{
+    ec_dev *d = ec_lookup(g);
+    if (!d) { ec_seterr("model not loaded"); return NULL; }
+    int cur = 0;
+    cudaGetDevice(&cur);
+    if (cur != d->device && cudaSetDevice(d->device) != cudaSuccess) {
+        cudaGetLastError();
+        ec_seterr("cannot use the model's device %d", d->device);
+        return NULL;
+    }
+    return d;
+}
+
+EC_EXPORT int ec_decode_sample(GPT2 *g, int *d_tokens, int *d_positions, int n_steps, const float *d_u,
+                               const float *d_temperature, const int *d_top_k, const float *d_top_p,
+                               const float *d_min_p, int *d_out_ids, float *d_out_prob)
+{
+    ec_dev *d = ec_enter(g);
+    if (!d) return -1;
+    if (n_steps < 0) { ec_seterr("n_steps must be >= 0"); return -1; }
+    if (!d_tokens || !d_positions || !d_u) { ec_seterr("ec_decode_sample: tokens, positions and u must not be NULL"); return -1; }
+    if (ec_check_sampling("ec_decode_sample", d)) return -1;
+    if (n_steps == 0) return 0;
+    const int M = d->B;
+    const int maxp = ec_batch_positions(d, d_positions, n_steps);
+    if (maxp < 0) return -1;
+    const int maxlen = ec_batch_len(d, maxp), chunk = ec_lm_chunk(d, M);
+    if (ec_batch_prepare(d, M, maxlen, chunk)) return -1;
+    if (!d->d_samp) CK(cudaMalloc((void **)&d->d_samp, (size_t)M * 6 * 4));
+    if (ec_ops(d, (size_t)M * 6 * 4)) return -1;
+    const size_t B = (size_t)M;
+    float *h = (float *)d->h_ops, *f = d->d_samp;
+    for (size_t m = 0; m < B; m++) {   /* what a NULL array stands for */
+        h[m] = h[4 * B + m] = h[3 * B + m] = 0.0f;
+        h[B + m] = h[2 * B + m] = 1.0f;
+        ((int *)h)[5 * B + m] = 0;
+    }
+    cudaStream_t st = d->stream;
+    CK(cudaMemcpyAsync(f, h, B * 6 * 4, cudaMemcpyHostToDevice, st));
+    if (d_temperature) CK(cudaMemcpyAsync(f + B, d_temperature, B * 4, cudaMemcpyDeviceToDevice, st));
+    if (d_top_p) CK(cudaMemcpyAsync(f + 2 * B, d_top_p, B * 4, cudaMemcpyDeviceToDevice, st));
+    if (d_min_p) CK(cudaMemcpyAsync(f + 3 * B, d_min_p, B * 4, cudaMemcpyDeviceToDevice, st));
+    if (d_top_k) CK(cudaMemcpyAsync(f + 5 * B, d_top_k, B * 4, cudaMemcpyDeviceToDevice, st));
+    CK(cudaMemcpyAsync(d->d_tok, d_tokens, B * 4, cudaMemcpyDeviceToDevice, st));
+    CK(cudaMemcpyAsync(d->d_pos, d_positions, B * 4, cudaMemcpyDeviceToDevice, st));
+    cudaGraphExec_t ex;
+    if (!ec_error_word()) { ec_seterr("ec_decode_sample: no device error word"); return -1; }
+    if (ec_bgraph(d, 2, M, maxlen, chunk, 0, &ex)) return -1;
+    for (int s = 0; s < n_steps; s++) {
+        CK(cudaMemcpyAsync(f, d_u + (size_t)s * B, B * 4, cudaMemcpyDeviceToDevice, st));
+        CK(cudaGraphLaunch(ex, st));
+        if (d_out_ids) CK(cudaMemcpyAsync(d_out_ids + (size_t)s * B, d->d_ids, B * 4, cudaMemcpyDeviceToDevice, st));
+        if (d_out_prob) CK(cudaMemcpyAsync(d_out_prob + (size_t)s * B, f + 4 * B, B * 4, cudaMemcpyDeviceToDevice, st));
+    }
+    CK(cudaMemcpyAsync(d_tokens, d->d_tok, B * 4, cudaMemcpyDeviceToDevice, st));
+    CK(cudaMemcpyAsync(d_positions, d->d_pos, B * 4, cudaMemcpyDeviceToDevice, st));
+    return 0;
+}
+
+static size_t ec_section(size_t *at, size_t bytes)
+{
+    const size_t here = *at;
+    *at = (here + bytes + 255) & ~(size_t)255;
+    return here;
+}
+
+EC_EXPORT int ec_forward_tree(GPT2 *g, const ec_tree_step *t, int *picked, float *prob, int *accepted, int *n_accepted)
+{
+    static const char fn[] = "ec_forward_tree";
+    ec_dev *d = ec_enter(g);
+    if (!d) return -1;
+    if (!t || !t->row_start || !t->base || !t->tokens || !t->parents || !accepted || !n_accepted) {
+        ec_seterr("%s: row_start, base, tokens, parents, accepted and n_accepted must not be NULL", fn);
+        return -1;
+    }
+    const int n = t->n_seq;
+    if (n < 1 || n > d->B) { ec_seterr("%s: n_seq %d outside [1, %d]", fn, n, d->B); return -1; }
+    if (t->max_path < 1 || t->max_path > d->C) { ec_seterr("%s: max_path %d outside [1, %d]", fn, t->max_path, d->C); return -1; }
+    if (d->hd % 8 || d->hd > 256 || d->kv % 8) { ec_seterr("%s: head_dim %d (a multiple of 8 up to 256)", fn, d->hd); return -1; }
+    if (t->u ? ec_check_sampling(fn, d) : d->v0 != 0 || d->v1 != d->V) {
+        if (!t->u) ec_seterr("%s: the model holds a vocabulary shard, a tree step needs all of it", fn);
+        return -1;
+    }
+    if (!t->u && (prob || t->temperature || t->top_k || t->top_p || t->min_p)) {
+        ec_seterr("%s: sampling settings and prob need u", fn);
+        return -1;
+    }
+    /* every index before anything changes */
+    if (t->row_start[0] != 0) { ec_seterr("%s: row_start[0] is %d", fn, t->row_start[0]); return -1; }
+    int most = 0, longest = 1;
+    for (int b = 0; b < n; b++) {
+        const int r0 = t->row_start[b], nodes = t->row_start[b + 1] - r0, s = t->slots ? t->slots[b] : b;
+        if (t->row_start[b + 1] < r0) { ec_seterr("%s: row_start falls at sequence %d", fn, b); return -1; }
+        if (s < 0 || s >= d->B) { ec_seterr("%s: slot %d outside [0, %d)", fn, s, d->B); return -1; }
+        for (int e = 0; e < b; e++)
+            if ((t->slots ? t->slots[e] : e) == s) { ec_seterr("%s: slot %d has two trees", fn, s); return -1; }
+        if (t->base[b] < 0 || t->base[b] > d->C - nodes) {
+            ec_seterr("%s: slot %d: positions [%d, %d + %d) exceed eff_ctx %d", fn, s, t->base[b], t->base[b], nodes, d->C);
+            return -1;
+        }
+        for (int j = 0; j < (t->base[b] + EC_KV_PAGE - 1) / EC_KV_PAGE; j++)
+            if (d->h_pt[(size_t)s * d->mp + j] < 0) { ec_seterr("%s: slot %d holds fewer than %d positions", fn, s, t->base[b]); return -1; }
+        for (int i = 0; i < nodes; i++) {
+            const int tok = t->tokens[r0 + i], up = t->parents[r0 + i];
+            if (tok < 0 || tok >= d->V) { ec_seterr("token id %d out of range [0,%d)", tok, d->V); return -1; }
+            if (i == 0 ? up != -1 : up < 0 || up >= i) { ec_seterr("%s: slot %d: parent %d of node %d (node 0 is the root, -1)", fn, s, up, i); return -1; }
+        }
+        if (nodes > most) most = nodes;
+        if (t->base[b] + nodes > longest) longest = t->base[b] + nodes;
+    }
+    const int M = t->row_start[n];
+    if (M == 0) {
+        for (int b = 0; b < n; b++) n_accepted[b] = 0;
+        for (size_t i = 0; i < (size_t)n * t->max_path; i++) accepted[i] = -1;
+        return 0;
+    }
+    if (ec_ensure(d, M)) return -1;
+    const int words = (most + 63) / 64;
+    size_t bytes = 0;
+    const size_t o_mask = ec_section(&bytes, (size_t)M * words * 8), o_row = ec_section(&bytes, (size_t)M * 4);
+    const size_t o_start = ec_section(&bytes, (size_t)(n + 1) * 4), o_base = ec_section(&bytes, (size_t)n * 4);
+    const size_t o_slot = ec_section(&bytes, (size_t)n * 4);
+    const size_t o_samp = ec_section(&bytes, t->u ? (size_t)M * 5 * 4 : 0);
+    const size_t in_bytes = bytes;
+    const size_t o_prob = ec_section(&bytes, (size_t)M * 4), o_acc = ec_section(&bytes, (size_t)n * t->max_path * 4);
+    const size_t o_num = ec_section(&bytes, (size_t)n * 4);
+    if (ec_ops(d, bytes)) return -1;
+    const size_t work = ec_tree_attention_bytes(n, M, d->H, d->KVH, d->hd, longest, d->num_sms);
+    if (work > d->tree_work_bytes) {
+        cudaFree(d->tree_work);
+        d->tree_work = NULL;
+        d->tree_work_bytes = 0;
+        CK(cudaMalloc(&d->tree_work, work));
+        d->tree_work_bytes = work;
+    }
+    const int Vs = d->v1 - d->v0;
+    int chunk = (int)((256u << 20) / ((size_t)Vs * 4));
+    if (chunk < 8) chunk = 8;
+    if (chunk > M) chunk = M;
+    if (ec_ensure_logits(d, chunk) || ec_ensure_amax(d, chunk)) return -1;
+    unsigned long long *mask = (unsigned long long *)(d->h_ops + o_mask);
+    int *row = (int *)(d->h_ops + o_row), *ht = d->h_in, *hp = d->h_in + M, *hs = d->h_in + 2 * M;
+    memset(mask, 0, (size_t)M * words * 8);
+    ec_kv_begin(d);
+    for (int b = 0; b < n; b++) {
+        const int r0 = t->row_start[b], nodes = t->row_start[b + 1] - r0, s = t->slots ? t->slots[b] : b;
+        if (ec_kv_map(d, s, t->base[b] + nodes)) return -1;
+        ((int *)(d->h_ops + o_slot))[b] = s;
+        for (int i = 0; i < nodes; i++) {
+            const int r = r0 + i, up = t->parents[r];
+            if (up >= 0) memcpy(mask + (size_t)r * words, mask + (size_t)(r0 + up) * words, (size_t)words * 8);
+            mask[(size_t)r * words + i / 64] |= 1ull << (i % 64);
+            ht[r] = t->tokens[r];
+            hp[r] = up >= 0 ? hp[r0 + up] + 1 : t->base[b];
+            hs[r] = s;
+            row[r] = t->base[b] + i;
+        }
+    }
+    if (ec_kv_flush(d)) return -1;
+    memcpy(d->h_ops + o_start, t->row_start, (size_t)(n + 1) * 4);
+    memcpy(d->h_ops + o_base, t->base, (size_t)n * 4);
+    ec_sampling sp = {NULL, NULL, NULL, NULL, NULL, NULL};
+    if (t->u) {
+        float *h = (float *)(d->h_ops + o_samp), *f = (float *)(d->d_ops + o_samp);
+        const size_t m = (size_t)M;
+        memcpy(h, t->u, m * 4);
+        for (size_t r = 0; r < m; r++) {
+            h[m + r] = t->temperature ? t->temperature[r] : 1.0f;
+            h[2 * m + r] = t->top_p ? t->top_p[r] : 1.0f;
+            h[3 * m + r] = t->min_p ? t->min_p[r] : 0.0f;
+            ((int *)h)[4 * m + r] = t->top_k ? t->top_k[r] : 0;
+        }
+        sp.u = f; sp.temperature = f + m; sp.top_p = f + 2 * m; sp.min_p = f + 3 * m; sp.top_k = (const int *)(f + 4 * m);
+        sp.prob = (float *)(d->d_ops + o_prob);
+    }
+    cudaStream_t st = d->stream;
+    CK(cudaMemcpyAsync(d->d_ops, d->h_ops, in_bytes, cudaMemcpyHostToDevice, st));
+    if (ec_copy_inputs(d, M)) return -1;
+    ec_tree_rows tree;
+    memset(&tree, 0, sizeof tree);
+    if (ec_model_kv(g, &tree.kv)) return -1;
+    const ec_kv_pages all = tree.kv;
+    tree.kv.n_layers = 1;
+    tree.row = (const int *)(d->d_ops + o_row);
+    ec_tree_attn *a = &tree.at;
+    a->q = d->q; a->out = d->att; a->ldq = a->ldo = d->E; a->type = EC_T_F32;
+    a->n_seq = n; a->rows = M; a->n_head = d->H; a->n_kv_head = d->KVH; a->head_dim = d->hd;
+    a->window = d->window; a->max_len = longest; a->mask_words = words;
+    a->slots = (const int *)(d->d_ops + o_slot); a->row_start = (const int *)(d->d_ops + o_start);
+    a->base = (const int *)(d->d_ops + o_base); a->mask = (const unsigned long long *)(d->d_ops + o_mask);
+    a->work = d->tree_work; a->work_bytes = d->tree_work_bytes;
+    if (ec_enqueue_body(d, M, longest, &tree)) return -1;
+    if (t->u ? ec_enqueue_lm_sample(d, M, chunk, sp) : ec_enqueue_lm_argmax(d, M, chunk)) return -1;
+    ec_tree_path path;
+    memset(&path, 0, sizeof path);
+    path.n_seq = n; path.rows = M; path.mask_words = words; path.max_path = t->max_path;
+    path.slots = a->slots; path.row_start = a->row_start; path.base = a->base; path.mask = a->mask;
+    path.tokens = d->d_tok; path.picked = d->d_ids;
+    path.accepted = (int *)(d->d_ops + o_acc); path.n_accepted = (int *)(d->d_ops + o_num);
+    path.new_base = (int *)(d->d_ops + o_base);
+    CK(ec_launch_tree_commit(&all, &path, ec_error_word(), st));
+    CK(cudaMemcpyAsync(d->h_ops + in_bytes, d->d_ops + in_bytes, bytes - in_bytes, cudaMemcpyDeviceToHost, st));
+    if (picked) CK(cudaMemcpyAsync(d->h_ids, d->d_ids, (size_t)M * 4, cudaMemcpyDeviceToHost, st));
+    CK(cudaStreamSynchronize(st));
+    if (ec_check_kernel_error(d)) return -1;
+    if (picked) memcpy(picked, d->h_ids, (size_t)M * 4);
+    if (prob) memcpy(prob, d->h_ops + o_prob, (size_t)M * 4);
+    memcpy(accepted, d->h_ops + o_acc, (size_t)n * t->max_path * 4);
+    memcpy(n_accepted, d->h_ops + o_num, (size_t)n * 4);
+    return 0;
+}
+
+EC_EXPORT int ec_kv_fork(GPT2 *g, int src, const int *dst, int n_dst, int len)
+{
+    static const char fn[] = "ec_kv_fork";
+    ec_dev *d = ec_enter(g);
+    if (!d) return -1;
+    if (n_dst < 0 || n_dst > d->B || n_dst > EC_KV_COPY_MAX || (n_dst && !dst)) { ec_seterr("%s: %d slots", fn, n_dst); return -1; }
+    if (d->kv % 8) { ec_seterr("%s: %d elements a position (a multiple of 8)", fn, d->kv); return -1; }
+    if (src < 0 || src >= d->B) { ec_seterr("%s: slot %d outside [0, %d)", fn, src, d->B); return -1; }
+    if (len < 0 || len > d->C) { ec_seterr("%s: length %d outside [0, %d]", fn, len, d->C); return -1; }
+    for (int i = 0; i < n_dst; i++) {
+        if (dst[i] < 0 || dst[i] >= d->B) { ec_seterr("%s: slot %d outside [0, %d)", fn, dst[i], d->B); return -1; }
+        if (dst[i] == src) { ec_seterr("%s: slot %d is its own target", fn, src); return -1; }
+        for (int j = 0; j < i; j++)
+            if (dst[j] == dst[i]) { ec_seterr("%s: slot %d is a target twice", fn, dst[i]); return -1; }
+    }
+    for (int j = 0; j < (len + EC_KV_PAGE - 1) / EC_KV_PAGE; j++)
+        if (d->h_pt[(size_t)src * d->mp + j] < 0) { ec_seterr("%s: slot %d holds fewer than %d positions", fn, src, len); return -1; }
+    if (n_dst == 0 || len == 0) return 0;
+    if (ec_ops(d, (size_t)n_dst * 16)) return -1;
+    ec_kv_begin(d);
+    int *h = (int *)d->h_ops;
+    const int *o = (const int *)d->d_ops;
+    for (int i = 0; i < n_dst; i++) {
+        if (ec_kv_map(d, dst[i], len)) return -1;
+        h[i] = src;
+        h[n_dst + i] = dst[i];
+        h[2 * n_dst + i] = 0;
+        h[3 * n_dst + i] = len;
+    }
+    if (ec_kv_flush(d)) return -1;
+    CK(cudaMemcpyAsync(d->d_ops, h, (size_t)n_dst * 16, cudaMemcpyHostToDevice, d->stream));
+    ec_kv_pages kv;
+    if (ec_model_kv(g, &kv)) return -1;
+    CK(ec_launch_kv_copy(&kv, n_dst, o, o + n_dst, o + 2 * n_dst, o + 3 * n_dst, d->num_sms, ec_error_word(), d->stream));
     return 0;
 }
 
@@ -2043,7 +2385,7 @@ EC_EXPORT long long ec_model_packed(const GPT2 *g, int layer, int which, void *o
 EC_EXPORT int ec_batch_graph_kernels(GPT2 *g, int kind)
 {
     ec_dev *d = ec_lookup(g);
-    if (!d || kind < 0 || kind > 1) { ec_seterr("ec_batch_graph_kernels: no model or bad kind"); return -1; }
+    if (!d || kind < 0 || kind > 2) { ec_seterr("ec_batch_graph_kernels: no model or bad kind"); return -1; }
     return d->bg[kind].exec ? d->bg[kind].kernels : 0;
 }
 
@@ -2099,7 +2441,7 @@ EC_EXPORT int ec_decode_profile(GPT2 *g, int *d_tokens, int start_pos, int n_ste
         for (int st = 0; st < n_steps; st++) {
             d->prof_on = 1;
             d->prof_n = 0;
-            int rc = ec_enqueue_body(d, M, maxlen);
+            int rc = ec_enqueue_body(d, M, maxlen, NULL);
             for (int r0 = 0; !rc && r0 < M; r0 += chunk) {   /* lm_head (GEMM class) + argmax (other) */
                 const int rows = M - r0 < chunk ? M - r0 : chunk;
                 rc = ec_enqueue_lm(d, r0, rows);

@@ -629,17 +629,18 @@ extern "C" int ec_launch_norm_quant(int8_t *q, float *scale, int Kp, const float
 // q and k (fp64, reference src/gpt2.c:656-665), q -> q_out [M][E] in head
 // order, k and v -> fp16 KV cache at (slot, pos).
 __global__ void __launch_bounds__(256) k_qkv_split(float *q_out, const float *qkv, int ldq, ec_tokens tk,
-                                                   ec_kvgeo g, int H, int KVH, int packed) {
+                                                   const int *cache_row, ec_kvgeo g, int H, int KVH, int packed) {
     EC_PDL_ENTER();
     const int m = blockIdx.x;
     const int pos = tk.pos[m], slot = tk.slot[m];
-    if (pos < 0 || pos >= g.C || slot < 0 || slot >= g.B) {
+    const int at = cache_row ? cache_row[m] : pos;   // nodes of a drafted tree lie apart from their position
+    if (pos < 0 || pos >= g.C || at < 0 || at >= g.C || slot < 0 || slot >= g.B) {
         if (threadIdx.x == 0) atomicCAS(&g_ec_err, 0, EC_KERR_BAD_INDEX);
         return;
     }
     const float *row = qkv + (size_t)m * ldq;
     float *qo = q_out + (size_t)m * g.E;
-    const size_t kvo = ec_kv_row(g.pt, g.mp, slot, pos) * g.kv;
+    const size_t kvo = ec_kv_row(g.pt, g.mp, slot, at) * g.kv;
     uint16_t *kr = g.kc + kvo;
     uint16_t *vr = g.vc + kvo;
     if (packed) {
@@ -670,10 +671,10 @@ __global__ void __launch_bounds__(256) k_qkv_split(float *q_out, const float *qk
     }
 }
 
-extern "C" int ec_launch_qkv_split(float *q_out, const float *qkv, int ldq, ec_tokens tk, ec_kvgeo geo, int H,
-                                   int KVH, int packed, int M, cudaStream_t stream) {
+extern "C" int ec_launch_qkv_split(float *q_out, const float *qkv, int ldq, ec_tokens tk, const int *cache_row,
+                                   ec_kvgeo geo, int H, int KVH, int packed, int M, cudaStream_t stream) {
     if (M <= 0) return 0;
-    k_qkv_split<<<M, 256, 0, stream>>>(q_out, qkv, ldq, tk, geo, H, KVH, packed);
+    k_qkv_split<<<M, 256, 0, stream>>>(q_out, qkv, ldq, tk, cache_row, geo, H, KVH, packed);
     return (int)cudaGetLastError();
 }
 

@@ -152,8 +152,9 @@ int ec_launch_norm(float *out, const float *x, const float *gamma, const float *
                    int M, int E, double eps, cudaStream_t stream);
 
 /* Split the q|k|v rows of a GEMM output [M][ldq] (Qwen2 packed layout when
- * packed != 0): RoPE, q -> q_out [M][E] in head order, k/v -> fp16 cache. */
-int ec_launch_qkv_split(float *q_out, const float *qkv, int ldq, ec_tokens tk, ec_kvgeo geo, int H,
+ * packed != 0): RoPE, q -> q_out [M][E] in head order, k/v -> fp16 cache, at
+ * position cache_row[m] of the slot (NULL: at the row's position). */
+int ec_launch_qkv_split(float *q_out, const float *qkv, int ldq, ec_tokens tk, const int *cache_row, ec_kvgeo geo, int H,
                         int KVH, int packed, int M, cudaStream_t stream);
 
 /* out[m][j] = silu(gu[m][2j]) * gu[m][2j+1] (gate|up interleaved). */

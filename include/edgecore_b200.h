@@ -110,7 +110,7 @@ int ec_lm_shard_keys(GPT2 *g, const float *d_hidden, int rows, long long *d_keys
 int ec_keys_advance(GPT2 *g, const long long *d_keys, int M, int *d_tokens, int *d_positions);
 
 /* Kernel launches in the last captured step graph of ec_decode_batch
- * (kind 0) or ec_batch_hidden (kind 1); 0 if none was captured. */
+ * (kind 0), ec_batch_hidden (kind 1) or ec_decode_sample (kind 2); 0 if none was captured. */
 int ec_batch_graph_kernels(GPT2 *g, int kind);
 
 /* Paged KV arena.  Each layer's K and V caches are pools of pages of 64
@@ -373,6 +373,45 @@ int ec_kv_copy(const ec_kv_pages *kv, int n_copies, const int *src, const int *d
 int ec_sample(int *ids, float *prob, const void *logits, int type, long long ld, int rows, int vocab,
               const float *temperature, const int *top_k, const float *top_p, const float *min_p,
               const float *u, void *stream);
+
+/* The operators on a loaded model's own arena.  Host arrays are read during
+ * the call. */
+
+/* One verified step of drafted trees: n_seq sequences, tree b's nodes in rows
+ * [row_start[b], row_start[b+1]) (row_start[0] = 0) with their tokens and
+ * parents, which come before their nodes: parents[first row] = -1, node 0 is
+ * the root and stands for the last token that is not in the cache yet.  Slot
+ * slots[b] (NULL: b) holds base[b] committed positions. */
+typedef struct {
+    int n_seq, max_path;
+    const int *slots, *row_start, *base;
+    const int *tokens, *parents;
+    /* settings per node as for ec_sample; u NULL: the greedy choice */
+    const float *u, *temperature, *top_p, *min_p;
+    const int *top_k;
+} ec_tree_step;
+
+/* All nodes through the model at once (ec_tree_attention in every layer), a
+ * choice after each (the argmax, or ec_sample), then ec_tree_commit: the
+ * accepted path's rows move to positions base[b] on, accepted
+ * [n_seq][max_path] holds the choices along it (-1 behind) and n_accepted its
+ * length, so the slot holds base[b] + n_accepted[b] positions and the last of
+ * accepted is the next root.  picked and prob ([rows], may be NULL): the
+ * choice after every node and its probability (prob only with u).  A call
+ * that is refused changes nothing.  Returns after the step. */
+int ec_forward_tree(GPT2 *g, const ec_tree_step *t, int *picked, float *prob, int *accepted, int *n_accepted);
+
+/* Slots dst[0..n_dst) take over positions [0, len) of slot src, copied into
+ * pages of their own (ec_kv_copy); enqueued on the model stream. */
+int ec_kv_fork(GPT2 *g, int src, const int *dst, int n_dst, int len);
+
+/* ec_decode_batch with the token of every step drawn by ec_sample: step s of
+ * slot m uses d_u[s * batch_cap + m] and the slot's settings (device arrays
+ * [batch_cap], NULL: off).  d_out_ids, d_out_prob: [n_steps][batch_cap], may
+ * be NULL. */
+int ec_decode_sample(GPT2 *g, int *d_tokens, int *d_positions, int n_steps, const float *d_u,
+                     const float *d_temperature, const int *d_top_k, const float *d_top_p, const float *d_min_p,
+                     int *d_out_ids, float *d_out_prob);
 
 #ifdef __cplusplus
 }

@@ -159,3 +159,10 @@ def test_tree_mask():
 def test_sample_refuses_a_vocabulary_beyond_shared_memory(built):
     with pytest.raises(RuntimeError, match="750000"):
         ec.sample(torch.zeros(1, dtype=torch.int32), torch.zeros(1, 750001), torch.zeros(1))
+
+
+def test_model_entries_refuse_a_model_that_is_not_loaded(built):
+    lib = ec.load_library()
+    assert lib.ec_forward_tree(None, None, None, None, None, None) == -1 and "not loaded" in ec.last_error()
+    assert lib.ec_kv_fork(None, 0, None, 0, 0) == -1 and "not loaded" in ec.last_error()
+    assert lib.ec_decode_sample(None, None, None, 1, None, None, None, None, None, None, None) == -1 and "not loaded" in ec.last_error()
