@@ -261,7 +261,7 @@ typedef struct ec_dev {
     float *logits;
     int logit_rows;
     void *amax_part;
-    int amax_chunks;
+    int amax_chunks, amax_rows;
     void *lm_part;             /* argmax partials of the fused lm_head (EC_EPI_ARGMAX) */
     size_t lm_part_bytes;
     int *d_tok, *d_pos, *d_slot, *d_ids;
@@ -700,10 +700,11 @@ static int ec_ensure_amax(ec_dev *d, int M)
 {
     const int chunks = 2 * d->num_sms;
     const int rows = d->cap > M ? d->cap : M;
-    if (d->amax_part && d->amax_chunks >= chunks && d->cap >= M) return 0;
+    if (d->amax_part && d->amax_chunks >= chunks && d->amax_rows >= rows) return 0;
     CK(cudaStreamSynchronize(d->stream));
     cudaFree(d->amax_part);
     d->amax_part = NULL;
+    d->amax_rows = 0;
     CK(cudaMalloc(&d->amax_part, (size_t)rows * chunks * 8));
     d->amax_chunks = chunks;
     /* fused lm_head argmax: two partials per column tile of 64 or more */
@@ -711,6 +712,7 @@ static int ec_ensure_amax(ec_dev *d, int M)
     d->lm_part = NULL;
     d->lm_part_bytes = (size_t)rows * 2 * ((d->V + 63) / 64) * 8;
     CK(cudaMalloc(&d->lm_part, d->lm_part_bytes));
+    d->amax_rows = rows;
     d->ws_gen++;
     return 0;
 }

@@ -292,3 +292,19 @@ def test_refusals_change_nothing(tiny_models, cuda):
             feed(other, prompt, 0, 1)
             want = feed(other, [5], 8, 1)
         assert np.abs(feed(m, [5], 8, 1) - want).max() <= TOL * np.abs(want).max()
+
+
+@pytest.mark.parametrize("first,then", [(9, 30), (13, 20), (20, 200)])
+def test_rows_that_grow_between_calls(tiny_models, cuda, first, then):
+    """The argmax workspaces follow a later call of more rows: nothing behind them is written."""
+    spec, path = tiny_models["qwen2_fp16"]
+    with ec.Model(path, batch_cap=8) as m:
+        for rows in (first, then):
+            tokens = synth.prompt_ids(spec.vocab, rows, seed=rows)
+            args = tokens, np.arange(rows, dtype=np.int32) % 25, np.arange(rows, dtype=np.int32) // 25
+            assert np.array_equal(m.forward_argmax(*args)[0], np.argmax(m.forward(*args), axis=1))
+        root, flat = (np.array([5]), np.array([-1])), (np.arange(then), np.maximum(np.arange(then) - 1 - np.arange(then) % 3, 0) - (np.arange(then) == 0))
+        if then < spec.n_ctx - 25:
+            out = m.forward_tree([flat], [min(25, then)], [0])
+            assert out["accepted"] == [walk(flat[0], flat[1], out["picked"])]
+        assert len(m.forward_tree([root], [min(25, then)], [0])["accepted"][0]) == 1
