@@ -135,10 +135,10 @@ __global__ void __launch_bounds__(PG_THREADS, 4) k_tree_commit(const ec_kv_pages
         len += found;
         __syncthreads();
     }
-    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.arrive.release;" ::: "memory");
     if (share == 0)
         for (int i = len + tid; i < a.max_path; i += PG_THREADS) a.accepted[(size_t)b * a.max_path + i] = -1;
-    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
     if (share == 0 && tid == 0) {
         a.n_accepted[b] = len;
         a.new_base[b] = base + len;
