@@ -775,6 +775,183 @@ __global__ void __launch_bounds__(SA_THREADS, 2) k_sample(const ec_sample_args a
     }
 }
 
+constexpr int DR_THREADS = 512, DR_WARPS = DR_THREADS / 32, DR_VOCAB = 16384;
+constexpr int DR_BATCH = 4;                       // 16-byte loads of a thread in flight
+
+// A row in global memory, in aligned 16-byte blocks; its first and last may
+// reach beyond it and are then read element by element.
+template <int T> struct DrRow {
+    typedef typename SaElt<T>::V V;
+    static constexpr int ELT = sizeof(V), PER = 16 / ELT;
+    const V *src;
+    int skew, vocab, blocks;   // place p is element p - skew
+    bool infinite;             // +inf weighs one, all else nothing
+    SaWeight weight;
+
+    EC_DEV float value(float v) const { return !infinite ? v : v == INFINITY ? 0.0f : -INFINITY; }
+    EC_DEV float at(int p) const { return p >= skew && p - skew < vocab ? value(sa_value<T>(src[p - skew])) : -INFINITY; }
+    EC_DEV uint4 block(int b) const {
+        const int e = b * PER - skew;
+        if (e >= 0 && e + PER <= vocab) return *reinterpret_cast<const uint4 *>(src + e);
+        uint32_t w[4];
+        for (int i = 0; i < 4; ++i) {
+            w[i] = T == EC_T_F32 ? 0xff800000u : T == EC_T_F16 ? 0xfc00fc00u : 0xff80ff80u;
+            for (int j = 0; j < PER / 4; ++j) {
+                const int n = e + i * (PER / 4) + j;
+                if (n < 0 || n >= vocab) continue;
+                if constexpr (T == EC_T_F32) w[i] = __float_as_uint(src[n]);
+                else w[i] = (w[i] & (j ? 0xffffu : 0xffff0000u)) | (uint32_t)src[n] << (16 * j);
+            }
+        }
+        return make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    // f(value, place) for blocks [b0, b1), taken by threads t of `threads`
+    template <typename F> EC_DEV void each(int b0, int b1, int t, int threads, F f) const {
+#pragma unroll 1
+        for (int b = b0 + t; b < b1; b += DR_BATCH * threads) {
+            uint4 u[DR_BATCH];
+#pragma unroll
+            for (int i = 0; i < DR_BATCH; ++i)
+                if (b + i * threads < b1) u[i] = block(b + i * threads);
+#pragma unroll
+            for (int i = 0; i < DR_BATCH; ++i) {
+                if (b + i * threads >= b1) break;
+                const uint32_t w[4] = {u[i].x, u[i].y, u[i].z, u[i].w};
+#pragma unroll
+                for (int j = 0; j < PER; ++j) {
+                    V x;
+                    if constexpr (T == EC_T_F32) x = __uint_as_float(w[j]);
+                    else x = (uint16_t)(w[j / 2] >> (16 * (j % 2)));
+                    f(sa_value<T>(x), (b + i * threads) * PER + j);
+                }
+            }
+        }
+    }
+    // A warp's sum of the weights of blocks [b0, b1)
+    template <bool RARE> EC_DEV u64 sum(int b0, int b1, int lane, double least) const {
+        u64 raw = 0;
+        each(b0, b1, lane, 32, [&](float v, int) {
+            const double w = weight(RARE ? value(v) : v);
+            raw += RARE && !(w >= least) ? SaWeight::RAW : SaWeight::raw(w);
+        });
+        const int terms = b1 - b0 > lane ? ((b1 - b0 - lane - 1) / 32 + 1) * PER : 0;
+        return sa_warp_sum(raw - (u64)terms * SaWeight::RAW);
+    }
+    EC_DEV u64 sum(int b0, int b1, int lane, double least) const {
+        return infinite || least > 0.0 ? sum<true>(b0, b1, lane, least) : sum<false>(b0, b1, lane, least);
+    }
+};
+
+// The warp of whose sum, in `part`, the point is part; `before` gains the
+// sums ahead of it.
+EC_DEV int dr_find(const u64 *part, u64 target, u64 &before) {
+    int w = 0;
+    while (w < DR_WARPS - 1 && before + part[w] <= target) before += part[w++];
+    return w;
+}
+
+// Many rows without top-k and top-p: a CTA per row, which reads it twice, for
+// the largest logit and for the sum, and then a 256th of it to find the point.
+// The second reading comes from L2: 1000 rows of 50257 fp32 logits (201 MB)
+// read 266 MB of DRAM.  They take 111 us, 1.8 TB/s, bound by the instructions
+// of the weights (about 30 for an element) and their dependence; k_sample,
+// whose SMs hold one row at a time and work on it or wait for it, takes 158.
+// Smaller CTAs (4 of 256 threads: 130 us) leave a longer tail and more rows
+// in flight than L2 holds; more than 2 CTAs of 512 have to spill.
+// The sums are the integers of k_sample, so the draws are the same.
+template <int T> __global__ void __launch_bounds__(DR_THREADS, 2) k_sample_rows(const ec_sample_args a, int shift) {
+    EC_PDL_ENTER();
+    typedef DrRow<T> Row;
+    constexpr int PER = Row::PER;
+    __shared__ double tab[SA_TAB], part2[48];
+    __shared__ float high[DR_WARPS];
+    __shared__ int firsts[DR_WARPS];
+    __shared__ u64 part[2][DR_WARPS];
+    const int r = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const float temperature = a.temperature ? a.temperature[r] : 1.0f, min_p = a.min_p ? a.min_p[r] : 0.0f;
+    Row row;
+    row.src = static_cast<const typename Row::V *>(a.logits) + (size_t)r * a.ld;
+    row.skew = (int)((reinterpret_cast<uintptr_t>(row.src) & 15) / Row::ELT);
+    row.vocab = a.vocab;
+    row.blocks = (row.skew + a.vocab + PER - 1) / PER;
+    row.infinite = false;
+    if (tid < 48) part2[tid] = exp2(tid < 16 ? (double)tid / 16 + shift : (double)(tid - 16) / SA_TAB);
+    float mx = -INFINITY;
+    row.each(0, row.blocks, tid, DR_THREADS, [&](float v, int) { mx = fmaxf(mx, v); });
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+    if (lane == 0) high[warp] = mx;
+    __syncthreads();
+    for (int j = tid; j < SA_TAB; j += DR_THREADS) tab[j] = part2[j / 32] * part2[16 + j % 32];
+    for (int w = 0; w < DR_WARPS; ++w) mx = fmaxf(mx, high[w]);
+    __syncthreads();
+    if (mx == -INFINITY) {
+        if (tid == 0) {
+            a.ids[r] = -1;
+            if (a.prob) a.prob[r] = 0.0f;
+        }
+        return;
+    }
+    if (!(temperature > 0.0f) || min_p > 1.0f) {   // the first of the largest
+        int first = 0x7fffffff;
+        row.each(0, row.blocks, tid, DR_THREADS, [&](float v, int p) {
+            if (v == mx) first = min(first, p - row.skew);
+        });
+        first = __reduce_min_sync(0xffffffffu, first);
+        if (lane == 0) firsts[warp] = first;
+        __syncthreads();
+        if (tid == 0) {
+            for (int w = 0; w < DR_WARPS; ++w) first = min(first, firsts[w]);
+            a.ids[r] = first;
+            if (a.prob) a.prob[r] = 1.0f;
+        }
+        return;
+    }
+    row.infinite = mx == INFINITY;
+    if (row.infinite) mx = 0.0f;
+    // as in k_sample
+    const double vanish = (double)temperature * 0.6931471805599453 * (shift + 3), per_nat = 512.0 * 1.4426950408889634 / (double)temperature;
+    row.weight = {(double)mx, per_nat, fmaxf(__double2float_ru((double)mx - vanish), -FLT_MAX), tab};
+    const double least = min_p > 0.0f ? (double)min_p * (double)(1ull << shift) : 0.0;
+    // each warp's piece of the row, then the pieces of the one with the point
+    int b0 = 0, b1 = row.blocks;
+    u64 before = 0, target = 0, total = 0;
+    for (int level = 0; level < 2; ++level) {
+        const int piece = (b1 - b0 + DR_WARPS - 1) / DR_WARPS;
+        const u64 mine = row.sum(min(b1, b0 + warp * piece), min(b1, b0 + (warp + 1) * piece), lane, least);
+        if (lane == 0) part[level][warp] = mine;
+        __syncthreads();
+        if (level == 0) {
+            for (int w = 0; w < DR_WARPS; ++w) total += part[0][w];
+            target = sa_point(a.u[r], total);
+        }
+        const int w = dr_find(part[level], target, before);
+        const int from = min(b1, b0 + w * piece);
+        b1 = min(b1, b0 + (w + 1) * piece);
+        b0 = from;
+    }
+    // the piece's elements in order, a warp at a time
+    if (warp != 0) return;
+    for (int p0 = b0 * PER; p0 < b1 * PER; p0 += 32) {
+        const float v = row.at(p0 + lane);
+        const double x = row.weight(v);
+        const u64 mine = p0 + lane < b1 * PER && x >= least ? SaWeight::whole(x) : 0ull;
+        u64 upto = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const u64 t = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += t;
+        }
+        upto += before;
+        if (upto > target && upto - mine <= target) {
+            a.ids[r] = p0 + lane - row.skew;
+            if (a.prob) a.prob[r] = (float)(x / (double)total);
+        }
+        before = __shfl_sync(0xffffffffu, upto, 31);
+        if (before > target) return;
+    }
+}
+
 int g_sample_attr[3][64];
 
 template <int T>
@@ -792,6 +969,12 @@ int sa_launch(const ec_sample_args &a, int num_sms, int *err, cudaStream_t strea
     int bits = 0;
     while ((1ll << bits) < a.vocab) ++bits;
     const int shift = 62 - bits < 50 ? 62 - bits : 50;
+    // 148 rows of 50257: 22 us, 28 as clusters; 400 rows of 1000: 15 and 13 us,
+    // 4000 of 10000: 144 and 145 us
+    if (!a.top_k && !a.top_p && a.rows >= num_sms && a.vocab >= DR_VOCAB) {
+        k_sample_rows<T><<<a.rows, DR_THREADS, 0, stream>>>(a, shift);
+        return (int)cudaGetLastError();
+    }
     const size_t fixed = (sizeof(SaShared) + 127) / 128 * 128;
     int ctas = 1;
     auto share_of = [&](int c) { return (int)(((long long)a.vocab + 2 * PER16 + c - 1) / c + PER16 - 1) / PER16 * PER16; };

@@ -196,3 +196,24 @@ def test_frequencies(cuda):
     count = np.bincount(ids, minlength=6)
     assert count[3] == 0
     assert (np.abs(count - n * w) <= 6 * np.sqrt(n * w * (1 - w)) + 1e-9).all()
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("vocab,pad", [(1001, 6), (16384, 0), (16391, 6), (20011, 3), (50257, 1)])
+def test_many_rows(cuda, kind, vocab, pad):
+    """Enough rows for one CTA each, without top-k and top-p: the definition's tokens, and bit for bit those of the kernel that
+    a call with (idle) top-k takes; rows of every alignment, with infinities and NaN among them."""
+    rows = 180
+    rs = np.random.RandomState(vocab)
+    x = _logits(cuda, rows, vocab + pad, kind, vocab)[:, pad // 2: pad // 2 + vocab]
+    if vocab > 2:
+        for r, v in ((5, math.inf), (6, math.nan), (7, -math.inf)):
+            x[r::40, :: 2 + r % 2] = v
+        x[8] = -math.inf
+        x[9] = math.nan
+    u = rs.rand(rows).astype(np.float32)
+    temperature, min_p = rs.choice([0.0, -1.0, math.nan, 0.02, 0.7, 1.0, 3.0], rows), rs.choice([0.0, 0.0, 0.003, 0.4, 1.0, 1.5], rows)
+    check(cuda, x, u, temperature=temperature, min_p=min_p)
+    for kw in (dict(), dict(temperature=temperature), dict(min_p=min_p), dict(temperature=temperature, min_p=min_p)):
+        a, b = run(cuda, x, u, **kw), run(cuda, x, u, top_k=np.zeros(rows), **kw)
+        assert np.array_equal(a[0], b[0]) and np.array_equal(a[1].view(np.int32), b[1].view(np.int32))
