@@ -17,6 +17,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
 from pathlib import Path
 from typing import Any
 
@@ -247,26 +248,11 @@ def argmax_key_decode(key: int) -> tuple[float, int]:
 
 # ---- serving operators on device tensors --------------------------------------
 
-class _KvPages(C.Structure):
-    """ec_kv_pages"""
-    _fields_ = [("k", _vp), ("v", _vp), ("ld_layer", C.c_longlong), ("ld_page", C.c_longlong), ("ld_pos", C.c_longlong),
-                ("page_table", _vp), ("type", _i), ("n_layers", _i), ("n_pages", _i), ("n_slots", _i),
-                ("pages_per_slot", _i), ("dim", _i)]
-
-
-class _TreeAttn(C.Structure):
-    """ec_tree_attn"""
-    _fields_ = [("q", _vp), ("out", _vp), ("ldq", C.c_longlong), ("ldo", C.c_longlong), ("type", _i), ("n_seq", _i),
-                ("rows", _i), ("n_head", _i), ("n_kv_head", _i), ("head_dim", _i), ("window", _i), ("max_len", _i),
-                ("mask_words", _i), ("scale", _f), ("slots", _vp), ("row_start", _vp), ("base", _vp), ("mask", _vp),
-                ("work", _vp), ("work_bytes", C.c_size_t)]
-
-
-class _TreePath(C.Structure):
-    """ec_tree_path"""
-    _fields_ = [("n_seq", _i), ("rows", _i), ("mask_words", _i), ("max_path", _i), ("slots", _vp), ("row_start", _vp),
-                ("base", _vp), ("mask", _vp), ("tokens", _vp), ("picked", _vp), ("accepted", _vp), ("n_accepted", _vp),
-                ("new_base", _vp)]
+# ec_kv_pages, ec_tree_attn and ec_tree_path, field by field: packed bytes cost
+# a quarter of a ctypes structure, on calls of a few microseconds
+_KV_PAGES = struct.Struct("PPqqqP6i")
+_TREE_ATTN = struct.Struct("PPqq9ifPPPPPN")
+_TREE_PATH = struct.Struct("4i9P")
 
 
 class _TreeStep(C.Structure):
@@ -279,23 +265,26 @@ _TYPES = {"torch.float32": 0, "torch.float16": 1, "torch.bfloat16": 2, "torch.in
 _TYPE_OF: dict = {}
 
 
-def _type(t) -> int:
-    """Code of a tensor's element type (0..2 as the C ABI's EC_T_*, 3 int32, 4 int64; -1: any other)."""
-    d = t.dtype
-    code = _TYPE_OF.get(d)
-    if code is None:
-        code = _TYPE_OF[d] = _TYPES.get(str(d), -1)
+def _new_type(d) -> int:
+    code = _TYPE_OF[d] = _TYPES.get(str(d), -1)
     return code
 
 
-def _vec(t, name: str, code: int, n: int | None = None):
-    """Address of a contiguous vector of the given type and, if given, length."""
+def _type(t) -> int:
+    """Code of a tensor's element type (0..2 as the C ABI's EC_T_*, 3 int32, 4 int64; -1: any other)."""
+    d = t.dtype
+    return _TYPE_OF[d] if d in _TYPE_OF else _new_type(d)
+
+
+def _vec(t, name: str, code: int, n: int | None = None) -> int:
+    """Address of a contiguous vector of the given type and, if given, length (0 for None)."""
     if t is None:
-        return None
-    if _type(t) != code or t.dim() != 1 or not t.is_contiguous():
+        return 0
+    shape = t.shape
+    if len(shape) != 1 or _type(t) != code or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous 1-D tensor of {list(_TYPES)[code]}")
-    if n is not None and t.shape[0] != n:
-        raise ValueError(f"{name} has {t.shape[0]} elements, {n} are needed")
+    if n is not None and shape[0] != n:
+        raise ValueError(f"{name} has {shape[0]} elements, {n} are needed")
     return t.data_ptr()
 
 
@@ -311,14 +300,14 @@ def _table(page_table):
     return page_table.shape
 
 
-def _layers(k, v, page_table) -> _KvPages:
+def _layers(k, v, page_table) -> bytes:
     """The arena of all layers: k and v [layers][pages][64][dim] (dim contiguous, any other strides)."""
     shape, st = k.shape, k.stride()
     if len(shape) != 4 or shape[1] < 1 or shape[2] != 64 or st[3] != 1 or v.shape != shape or v.stride() != st or v.dtype != k.dtype:
         raise ValueError("k and v must be alike: [layers][pages][64][dim] with contiguous positions")
     slots, per_slot = _table(page_table)
-    return _KvPages(k.data_ptr(), v.data_ptr(), st[0], st[1], st[2], page_table.data_ptr(), _type(k), shape[0], shape[1], slots,
-                    per_slot, shape[3])
+    return _KV_PAGES.pack(k.data_ptr(), v.data_ptr(), st[0], st[1], st[2], page_table.data_ptr(), _type(k), shape[0], shape[1], slots,
+                          per_slot, shape[3])
 
 
 def tree_mask(parents) -> np.ndarray:
@@ -363,18 +352,17 @@ def tree_attention(out, q, k, v, page_table, row_start, base, mask, *, slots=Non
             raise ValueError("the rows of q and out must be contiguous")
     rows, n_seq = qs[0], base.shape[0]
     slots_n, per_slot = _table(page_table)
-    kv = _KvPages(k.data_ptr(), v.data_ptr(), 0, kst[0], kst[1], page_table.data_ptr(), _type(k), 1, ks[0], slots_n, per_slot,
-                  ks[2] * hd)
-    work = None
-    nbytes = 0
+    kv = _KV_PAGES.pack(k.data_ptr(), v.data_ptr(), 0, kst[0], kst[1], page_table.data_ptr(), _type(k), 1, ks[0], slots_n, per_slot,
+                        ks[2] * hd)
+    work = nbytes = 0
     if workspace is not None:
         if not workspace.is_contiguous():
             raise ValueError("workspace must be contiguous")
         work, nbytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
-    a = _TreeAttn(q.data_ptr(), out.data_ptr(), qst[0], ost[0], _type(q), n_seq, rows, wide // hd, ks[2], hd, window, max_len,
+    a = _TREE_ATTN.pack(q.data_ptr(), out.data_ptr(), qst[0], ost[0], _type(q), n_seq, rows, wide // hd, ks[2], hd, window, max_len,
                   _words(mask, rows), scale, _vec(slots, "slots", 3, n_seq), _vec(row_start, "row_start", 3, n_seq + 1),
                   _vec(base, "base", 3), mask.data_ptr(), work, nbytes)
-    if load_library().ec_tree_attention(C.addressof(kv), C.addressof(a), stream):
+    if load_library().ec_tree_attention(kv, a, stream):
         raise RuntimeError(last_error())
     return out
 
@@ -390,11 +378,11 @@ def tree_commit(k, v, page_table, row_start, base, mask, tokens, picked, accepte
     rows = tokens.shape[0]
     if _type(accepted) != 3 or accepted.dim() != 2 or accepted.shape[0] != n_seq or not accepted.is_contiguous():
         raise ValueError(f"accepted must be a contiguous int32 tensor [{n_seq}][nodes]")
-    a = _TreePath(n_seq, rows, _words(mask, rows), accepted.shape[1], _vec(slots, "slots", 3, n_seq),
+    a = _TREE_PATH.pack(n_seq, rows, _words(mask, rows), accepted.shape[1], _vec(slots, "slots", 3, n_seq),
                   _vec(row_start, "row_start", 3, n_seq + 1), _vec(base, "base", 3), mask.data_ptr(), _vec(tokens, "tokens", 3),
                   _vec(picked, "picked", 3, rows), accepted.data_ptr(), _vec(n_accepted, "n_accepted", 3, n_seq),
                   _vec(new_base, "new_base", 3, n_seq))
-    if load_library().ec_tree_commit(C.addressof(kv), C.addressof(a), stream):
+    if load_library().ec_tree_commit(kv, a, stream):
         raise RuntimeError(last_error())
 
 
@@ -403,7 +391,7 @@ def kv_copy(k, v, page_table, src, dst, start, end, *, stream=None) -> None:
     [layers][pages][64][dim], the others int32 vectors of one length."""
     kv = _layers(k, v, page_table)
     n = src.shape[0]
-    if load_library().ec_kv_copy(C.addressof(kv), n, _vec(src, "src", 3), _vec(dst, "dst", 3, n), _vec(start, "start", 3, n),
+    if load_library().ec_kv_copy(kv, n, _vec(src, "src", 3), _vec(dst, "dst", 3, n), _vec(start, "start", 3, n),
                                  _vec(end, "end", 3, n), stream):
         raise RuntimeError(last_error())
 

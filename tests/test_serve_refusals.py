@@ -3,7 +3,10 @@ No GPU is needed: the checks of arguments come before the first CUDA call, and a
 (or with host memory on one with a device) is refused too."""
 from __future__ import annotations
 
-import ctypes as C
+import re
+import struct
+import subprocess
+from pathlib import Path
 
 import numpy as np
 import pytest
@@ -137,12 +140,34 @@ def test_c_entries_refuse_null(built):
     assert lib.ec_sample(None, None, None, 0, 1, 1, 1, None, None, None, None, None, None) == -1
     assert lib.ec_model_kv(None, None) == -1
     k = torch.zeros(1, 5, 64, 128, dtype=torch.float16)
-    kv = ec._layers(k, k.clone(), torch.zeros(1, 2, dtype=torch.int32))
-    assert lib.ec_tree_attention(C.addressof(kv), None, None) == -1 and "no arguments" in ec.last_error()
-    for field, value in (("n_pages", 0), ("pages_per_slot", 1 << 26), ("ld_pos", 120), ("ld_pos", 132), ("k", kv.k + 2), ("type", 0)):
-        bad = ec._layers(k, k.clone(), torch.zeros(1, 2, dtype=torch.int32))
-        setattr(bad, field, value)
-        assert lib.ec_tree_commit(C.addressof(bad), C.addressof(ec._TreePath(1, 0, 1, 1)), None) == -1, field
+    v, table = k.clone(), torch.zeros(1, 2, dtype=torch.int32)
+    kv = ec._layers(k, v, table)
+    assert lib.ec_tree_attention(kv, None, None) == -1 and "no arguments" in ec.last_error()
+    names = ("k", "v", "ld_layer", "ld_page", "ld_pos", "page_table", "type", "n_layers", "n_pages", "n_slots", "pages_per_slot", "dim")
+    path = ec._TREE_PATH.pack(1, 0, 1, 1, *[0] * 9)
+    for field, value in (("n_pages", 0), ("pages_per_slot", 1 << 26), ("ld_pos", 120), ("ld_pos", 132), ("k", k.data_ptr() + 2), ("type", 0)):
+        bad = list(ec._KV_PAGES.unpack(kv))
+        bad[names.index(field)] = value
+        assert lib.ec_tree_commit(ec._KV_PAGES.pack(*bad), path, None) == -1, field
+
+
+def test_packed_structs_are_the_headers(built, tmp_path):
+    """The struct formats of the binding against the compiler's layout of the header."""
+    fields = {"ec_kv_pages": (ec._KV_PAGES, "k v ld_layer ld_page ld_pos page_table type n_layers n_pages n_slots pages_per_slot dim"),
+              "ec_tree_attn": (ec._TREE_ATTN, "q out ldq ldo type n_seq rows n_head n_kv_head head_dim window max_len mask_words scale slots row_start base mask work work_bytes"),
+              "ec_tree_path": (ec._TREE_PATH, "n_seq rows mask_words max_path slots row_start base mask tokens picked accepted n_accepted new_base")}
+    src = ["#include <stddef.h>", "#include <stdio.h>", '#include "edgecore_b200.h"', "int main(void) {"]
+    for name, (_, f) in fields.items():
+        src += [f'printf("{name} {k} %zu\\n", offsetof({name}, {k}));' for k in f.split()] + [f'printf("{name} . %zu\\n", sizeof({name}));']
+    (tmp_path / "p.c").write_text("\n".join(src + ["return 0; }"]))
+    include = Path(ec.__file__).resolve().parents[1] / "include"
+    subprocess.run(["gcc", "-I", str(include), "-o", str(tmp_path / "p"), str(tmp_path / "p.c")], check=True)
+    said = [line.split() for line in subprocess.run([str(tmp_path / "p")], check=True, capture_output=True, text=True).stdout.splitlines()]
+    for name, (fmt, f) in fields.items():
+        codes = re.sub(r"(\d+)(.)", lambda m: m[2] * int(m[1]), fmt.format)
+        at = {k: struct.calcsize(codes[:i] + "0" + c) for i, (k, c) in enumerate(zip(f.split(), codes))}
+        assert len(codes) == len(f.split())
+        assert {k: int(v) for n, k, v in said if n == name} == at | {".": fmt.size}
 
 
 def test_tree_mask():
