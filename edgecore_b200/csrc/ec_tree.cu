@@ -7,12 +7,19 @@
 // One pass over the pages with a running maximum m and sum l per row:
 //   s = scale * q.k (masked: -inf), m' = max(m, s), p = 2^((s - m') log2 e),
 //   l = l 2^((m - m') log2 e) + sum p,  o = o 2^((m - m') log2 e) + p V
-// and out = o / l (0 where nothing was seen).  The pages are the work: small
-// calls give every row tile to the CTAs of a cluster, which join their (m, l,
-// o) through each other's shared memory; larger ones cut the pages of all
+// and out = o / l (0 where nothing was seen).  The pages are the work: short
+// contexts give every row tile to the CTAs of a cluster, which join their (m,
+// l, o) through each other's shared memory; longer ones cut the pages of all
 // tiles, one after the other, into equal pieces, one per resident CTA, so that
 // ragged sequences keep every SM busy to the end, and k_tree_join adds up the
 // tiles that a border cuts, in the order of their pages.
+// Measured: one token of one stream, 7 us; a tree of 9 nodes at 30011 positions,
+// 12 heads of 128 on 2 (31 MB, 1.7 GFLOP), 26 us or 1.2 TB/s, 7 us of it the
+// second launch with its wait for the first; 32 sequences of 1
+// to 17 nodes with fp32 q at 65 to 1900 positions 33 us; 24 windowed ones 20 us
+// or 1.6 TB/s.  All are bound by latency: a page is a chain of load, product,
+// maximum, exponentials and product of about a microsecond in a warp, and
+// little more than one chain of a few pages fits a call of this length.
 #include "ec_tree.cuh"
 
 #include <cooperative_groups.h>
@@ -716,15 +723,20 @@ TaPlan ta_plan(int n_seq, int rows, int n_head, int n_kv_head, int hd, int max_l
     int pages = ta_up(max_len > 0 ? max_len : 1, PAGE);
     if (window > 0 && pages > window / PAGE + 2) pages = window / PAGE + 2;
     // Up to 16 pages a tile is one cluster's, of as many CTAs as two rounds of
-    // the SMs hold: 24 windowed sequences of 10 pages, 12 heads, take 20 us so
-    // and 31 us as equal pieces with a second launch.  Beyond, ragged lengths
-    // leave clusters waiting: 32 sequences of 65 to 1900 positions take 33 us
-    // as pieces, 34 to 39 us as clusters.
+    // the SMs hold: 24 windowed sequences of 10 pages, 12 heads of 64, take 20
+    // us so and 31 us as equal pieces with a second launch; 64 sequences of one
+    // token up to 900 positions, 14 heads of 64 on 2, 16 and 22 us.  Beyond,
+    // ragged lengths leave clusters waiting: 32 sequences of 65 to 1900
+    // positions take 33 us as pieces, 34 to 39 us as clusters.  fp32 rows wider
+    // than 64, with two or three products for each of the others', are better
+    // cut from 9 pages on unless the clusters leave SMs idle: 32 trees of 24
+    // nodes at 450 to 900 positions 44 us, 57 as clusters.
     const long long tiles = (long long)p.tiles * n_kv_head;
     p.g.cluster = pages >= 8 ? 8 : pages >= 4 ? 4 : pages >= 2 ? 2 : 1;
     while (p.g.cluster > 1 && tiles * p.g.cluster > 2 * sms) p.g.cluster /= 2;
     p.pieces = 0;
-    if (pages > 16 && tiles * slot_pages <= 0x7fffffff)
+    const bool cut = pages > 16 || (pages > 8 && f32 && p.hdp > 64 && tiles * p.g.cluster > sms);
+    if (cut && tiles * slot_pages <= 0x7fffffff)
         p.pieces = (p.mt == TC_ROWS ? 1 : p.hdp == 64 && !f32 ? 3 : p.hdp <= 128 ? 2 : 1) * sms;
     if (!p.pieces && p.mt == TC_ROWS) {   // clusters: the register tiles only
         p.mt = 64;

@@ -23,6 +23,12 @@
 // the rate that cuBLAS reaches.  Two CTAs per SM of 128 rows each, which nothing
 // kept out of step, took 3400 cycles a page instead.  Every wait is bounded;
 // loads use no multicast.
+// Measured: 16 trees of 48 to 64 nodes at 6000 to 10000 positions, 12 heads of
+// 128 on 2 (43.7 GFLOP), 99 us or 440 TFLOP/s, join included; the register
+// tiles of ec_tree.cu take 192.  A round of two steps takes 2.3 to 2.9 us where its exponentials and
+// products need 1.5: the rows' own instructions (scale, mask, maximum, pack)
+// are the longest link.  The join and its launch are 20 us, the ends of two
+// tiles in a piece 10.
 #include "ec_tree.cuh"
 
 #include <cuda.h>

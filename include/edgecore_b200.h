@@ -116,9 +116,9 @@ int ec_batch_graph_kernels(GPT2 *g, int kind);
 /* Paged KV arena.  Each layer's K and V caches are pools of pages of 64
  * positions; slot s keeps positions [64 j, 64 j + 64) in the page its table
  * entry j names.  Pages are mapped as calls reach new positions of a slot
- * (host-visible positions: the rows of gpt2_forward / ec_forward_argmax,
- * start_pos + n_steps of the decode loops, max_pos_end of
- * ec_batch_hidden; ec_forward_device maps every slot fully) and stay mapped
+ * (host-visible positions: the rows of gpt2_forward / ec_forward_argmax and
+ * the nodes of ec_forward_tree, start_pos + n_steps of the decode loops,
+ * max_pos_end of ec_batch_hidden, the targets of ec_kv_fork; ec_forward_device maps every slot fully) and stay mapped
  * until ec_kv_release(slot) (slot < 0: every slot) returns them.  The pool
  * holds batch_cap * ceil(eff_ctx / 64) pages by default, so no call can run
  * out; the environment variable EDGECORE_KV_PAGES at gpt2_load sets a

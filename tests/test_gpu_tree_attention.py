@@ -266,6 +266,18 @@ def test_pieces_many_sequences_and_growing_maxima(cuda):
         c.check()
 
 
+@pytest.mark.parametrize("q,kv,hd", [("f16", "f16", 64), ("bf16", "bf16", 128), ("f32", "f16", 64), ("f32", "bf16", 128), ("f16", "f16", 256)])
+@pytest.mark.parametrize("seqs", [1, 4, 12, 30, 50])
+def test_short_contexts_of_every_cluster_size(cuda, seqs, q, kv, hd):
+    """6 KV heads and up to 5 pages: tiles for clusters of 4 CTAs, of 2 and of one, and for more of them than fit at once."""
+    rs = np.random.RandomState(seqs)
+    sizes, bases = rs.randint(1, 40, seqs), rs.randint(0, 270, seqs)
+    for window in (0, 90):
+        c = Case(cuda, q, kv, 6, 6, hd, sizes=sizes.tolist(), bases=bases.tolist(), window=window, seed=hd + seqs)
+        c.run(max_len=310)
+        c.check()
+
+
 def test_pieces_little_work_and_small_workspaces(cuda):
     for bytes_ in (1 << 17, 1 << 19, 1 << 21, 1 << 26):
         c = Case(cuda, "bf16", "bf16", 12, 2, 128, sizes=(30, 7), bases=(700, 90), seed=17)
