@@ -23,6 +23,7 @@
 #include "ec_tree.cuh"
 
 #include <cooperative_groups.h>
+#include <limits.h>
 
 namespace cg = cooperative_groups;
 
@@ -241,6 +242,8 @@ __global__ void __launch_bounds__(32 * WM * WN, HDP == 64 && QT != EC_T_F32 ? 3 
     const int node_lo = ta_node(g, s.first + row_lo), node_hi = ta_node(g, s.first + row_lo + 8);
     const float f_lo = Ty::F32 ? fmaxf(g.scale2 * row_scale[row_lo], 1e-37f) : g.scale2;   // above 0: masked scores stay -inf
     const float f_hi = Ty::F32 ? fmaxf(g.scale2 * row_scale[row_lo + 8], 1e-37f) : g.scale2;
+    const int depth_lo = a.window > 0 && node_lo < s.t ? ta_depth(a, s.r0 + node_lo) : 0;
+    const int depth_hi = a.window > 0 && node_hi < s.t ? ta_depth(a, s.r0 + node_hi) : 0;
     float o[ND][4], m_lo = -INFINITY, m_hi = -INFINITY, l_lo = 0.0f, l_hi = 0.0f;
 #pragma unroll
     for (int i = 0; i < ND; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
@@ -296,8 +299,27 @@ __global__ void __launch_bounds__(32 * WM * WN, HDP == 64 && QT != EC_T_F32 ? 3 
         const bool part = p0 + PAGE > s.base || (a.window > 0 && p0 < (long long)s.base + 64 * a.mask_words - a.window);
         unsigned long long see_lo = ~0ull, see_hi = ~0ull;
         if (part) {
-            see_lo = ta_allow(a, s, node_lo, p0);
-            see_hi = ta_allow(a, s, node_hi, p0);
+            see_lo = ta_see(a, s, node_lo, p0, depth_lo);
+            see_hi = ta_see(a, s, node_hi, p0, depth_hi);
+            if (ta_short_window(a) && p0 + PAGE > s.base) {
+                // the depths of the page's nodes, two a lane, against each of
+                // the warp's rows in turn (reading them per ancestor of a row:
+                // 53 trees of 130 nodes, window 4, 12 heads of 64, fp32: 176 us
+                // instead of 105)
+                const int j = p0 - s.base + lane;
+                const int d0 = j >= 0 && j < s.t ? ta_depth(a, s.r0 + j) : INT_MAX, d1 = j + 32 >= 0 && j + 32 < s.t ? ta_depth(a, s.r0 + j + 32) : INT_MAX;
+                const int least_lo = depth_lo - a.window + 1, least_hi = depth_hi - a.window + 1;
+                unsigned long long keep_lo = 0, keep_hi = 0;
+#pragma unroll
+                for (int r = 0; r < 8; ++r) {
+                    const int t_lo = __shfl_sync(0xffffffffu, least_lo, 4 * r), t_hi = __shfl_sync(0xffffffffu, least_hi, 4 * r);
+                    const unsigned long long b_lo = __ballot_sync(0xffffffffu, d0 >= t_lo) | (unsigned long long)__ballot_sync(0xffffffffu, d1 >= t_lo) << 32;
+                    const unsigned long long b_hi = __ballot_sync(0xffffffffu, d0 >= t_hi) | (unsigned long long)__ballot_sync(0xffffffffu, d1 >= t_hi) << 32;
+                    if (lane / 4 == r) { keep_lo = b_lo; keep_hi = b_hi; }
+                }
+                see_lo &= keep_lo;   // committed positions: INT_MAX above, kept
+                see_hi &= keep_hi;
+            }
         }
         float x_lo = -INFINITY, x_hi = -INFINITY;
         const unsigned w_lo = (unsigned)(see_lo >> (wn * KN + (lane % 4) * 2)), w_hi = (unsigned)(see_hi >> (wn * KN + (lane % 4) * 2));

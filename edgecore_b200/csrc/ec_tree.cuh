@@ -189,11 +189,11 @@ EC_DEV int ta_depth(const ec_tree_attn &a, int row) {
 EC_DEV unsigned long long ta_low(int n) { return n <= 0 ? 0ull : n >= 64 ? ~0ull : (1ull << n) - 1ull; }
 
 // Which of the 64 positions from p0 on the node `i` of the tile's sequence
-// sees, one bit each.
-EC_DEV unsigned long long ta_allow(const ec_tree_attn &a, const TaTile &s, int i, int p0) {
+// sees, one bit each, but for what a window hides of the tree itself.
+EC_DEV unsigned long long ta_see(const ec_tree_attn &a, const TaTile &s, int i, int p0, int depth) {
     if (i >= s.t) return 0ull;
-    const int row = s.r0 + i, j0 = p0 - s.base;
-    const unsigned long long *m = a.mask + (size_t)row * a.mask_words;
+    const int j0 = p0 - s.base;
+    const unsigned long long *m = a.mask + (size_t)(s.r0 + i) * a.mask_words;
     unsigned long long tree = 0;
     if (j0 < 0) {
         if (j0 > -64) tree = m[0] << -j0;
@@ -204,15 +204,24 @@ EC_DEV unsigned long long ta_allow(const ec_tree_attn &a, const TaTile &s, int i
     }
     const unsigned long long prefix = ta_low(s.base - p0);
     tree &= ta_low(s.base + s.t - p0) & ~prefix;
-    if (a.window <= 0) return prefix | tree;
-    const int depth = ta_depth(a, row);
-    const int from = s.base + depth - a.window + 1;
-    if (a.window < 64 * a.mask_words)   // nodes of one tree are fewer levels apart than that
-        for (unsigned long long left = tree; left; left &= left - 1) {
+    return (a.window > 0 ? prefix & ~ta_low(s.base + depth - a.window + 1 - p0) : prefix) | tree;
+}
+
+// A window hides nodes from their descendants only if it is shorter than the
+// levels that a tree can have.
+EC_DEV bool ta_short_window(const ec_tree_attn &a) { return a.window > 0 && a.window < 64 * a.mask_words; }
+
+// The same with the window applied to the tree too.
+EC_DEV unsigned long long ta_allow(const ec_tree_attn &a, const TaTile &s, int i, int p0) {
+    if (i >= s.t) return 0ull;
+    const int depth = a.window > 0 ? ta_depth(a, s.r0 + i) : 0;
+    unsigned long long see = ta_see(a, s, i, p0, depth);
+    if (ta_short_window(a))
+        for (unsigned long long left = see & ~ta_low(s.base - p0); left; left &= left - 1) {
             const int bit = __ffsll((long long)left) - 1;
-            if (s.base + ta_depth(a, s.r0 + j0 + bit) < from) tree &= ~(1ull << bit);
+            if (ta_depth(a, s.r0 + p0 - s.base + bit) < depth - a.window + 1) see &= ~(1ull << bit);
         }
-    return (prefix & ~ta_low(from - p0)) | tree;
+    return see;
 }
 
 template <int T> EC_DEV void ta_store2(void *p, size_t i, float x, float y, bool pair) {   // pair: i even and aligned

@@ -267,15 +267,28 @@ def test_pieces_many_sequences_and_growing_maxima(cuda):
 
 
 @pytest.mark.parametrize("q,kv,hd", [("f16", "f16", 64), ("bf16", "bf16", 128), ("f32", "f16", 64), ("f32", "bf16", 128), ("f16", "f16", 256)])
-@pytest.mark.parametrize("seqs", [1, 4, 12, 30, 50])
-def test_short_contexts_of_every_cluster_size(cuda, seqs, q, kv, hd):
+@pytest.mark.parametrize("seqs,window", [(4, 0), (12, 90), (40, 0)])
+def test_short_contexts_of_every_cluster_size(cuda, seqs, window, q, kv, hd):
     """6 KV heads and up to 5 pages: tiles for clusters of 4 CTAs, of 2 and of one, and for more of them than fit at once."""
     rs = np.random.RandomState(seqs)
     sizes, bases = rs.randint(1, 40, seqs), rs.randint(0, 270, seqs)
-    for window in (0, 90):
-        c = Case(cuda, q, kv, 6, 6, hd, sizes=sizes.tolist(), bases=bases.tolist(), window=window, seed=hd + seqs)
-        c.run(max_len=310)
-        c.check()
+    c = Case(cuda, q, kv, 6, 6, hd, sizes=sizes.tolist(), bases=bases.tolist(), window=window, seed=hd + seqs)
+    c.run(max_len=310)
+    c.check()
+
+
+@pytest.mark.parametrize("window", [1, 3, 20, 128])
+@pytest.mark.parametrize("q,kv", [("f32", "bf16"), ("f16", "f16")])
+def test_window_within_large_trees(cuda, window, q, kv):
+    """Trees of more levels than the window: it hides nodes from their descendants, across pages and mask words."""
+    chain = np.maximum(np.arange(150) - 1 - np.arange(150) % 3 % 2, -1)
+    chain[1:] = np.maximum(chain[1:], 0)
+    mask = ec.tree_mask(chain).view(np.uint64)
+    for base in (0, 40, 130):
+        c = Case(cuda, q, kv, 6, 3, 64, sizes=(150,), bases=(base,), window=window, mask=mask, seed=window)
+        for far in (None, FAR):
+            c.run(**({} if far is None else {"max_len": far}))
+            c.check()
 
 
 def test_pieces_little_work_and_small_workspaces(cuda):
