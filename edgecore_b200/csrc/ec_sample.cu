@@ -447,7 +447,7 @@ EC_DEV void sa_select(cg::cluster_group &cl, SaRow<T> &row, u64 want, float top_
 
 // The other half of the arrival at the kernel's start: no CTA of the cluster
 // is still to come.
-EC_DEV void sa_cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+EC_DEV void sa_cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
 
 // The point u of a sum of whole weights: the running sum has to exceed it.
 EC_DEV u64 sa_point(float u, u64 total) {
@@ -569,7 +569,7 @@ __global__ void __launch_bounds__(SA_THREADS, 2) k_sample(const ec_sample_args a
         s.low[threadIdx.x] = INFINITY;
     }
     // this CTA has started, and what others write first is set (sa_cluster_wait)
-    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.arrive.release;" ::: "memory");
     EC_PDL_ENTER();
     V *vals = reinterpret_cast<V *>(smem + (sizeof(SaShared) + 127) / 128 * 128);
     cg::cluster_group cl = cg::this_cluster();
