@@ -207,9 +207,9 @@ EC_DEV unsigned long long ta_see(const ec_tree_attn &a, const TaTile &s, int i, 
     return (a.window > 0 ? prefix & ~ta_low(s.base + depth - a.window + 1 - p0) : prefix) | tree;
 }
 
-// A window hides nodes from their descendants only if it is shorter than the
-// levels that a tree can have.
-EC_DEV bool ta_short_window(const ec_tree_attn &a) { return a.window > 0 && a.window < 64 * a.mask_words; }
+// A window hides nodes from each other only if it is no longer than two depths
+// can be apart: a row of all bits has 64 words - 1, one of none has -1.
+EC_DEV bool ta_short_window(const ec_tree_attn &a) { return a.window > 0 && a.window <= 64ll * a.mask_words; }
 
 // The same with the window applied to the tree too.
 EC_DEV unsigned long long ta_allow(const ec_tree_attn &a, const TaTile &s, int i, int p0) {

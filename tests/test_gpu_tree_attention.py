@@ -384,3 +384,21 @@ def test_captured_graph_replays_on_new_data_and_other_stream(cuda):
     ec.tree_attention(c.out, c.q, c.k, c.v, *args, slots=slots, workspace=work, max_len=2004, stream=s.cuda_stream)
     s.synchronize()
     assert cuda.equal(c.out, first)      # the same result, bit for bit
+
+
+@pytest.mark.parametrize("window", [63, 64, 65, 127, 128, 129])
+@pytest.mark.parametrize("far", [None, FAR])
+@pytest.mark.parametrize("q,kv", [("f16", "f16"), ("bf16", "bf16"), ("f32", "f16")])
+def test_window_as_long_as_a_mask_has_bits(cuda, window, far, q, kv):
+    """Rows of all bits (depth 64 words - 1) and of none (depth -1): the furthest apart that two nodes of a mask can stand.
+    A window of 64 words still hides the one from the other, one more no longer does."""
+    words = 1 if window < 100 else 2
+    mask = np.random.RandomState(5).randint(0, 1 << 62, (20, words)).astype(np.uint64)
+    mask[[0, 7]] = 2 ** 64 - 1
+    mask[[1, 9]] = 0
+    mask[2] = 1
+    mask[3] = 2 ** 64 - 2
+    for base in (0, 70):
+        c = Case(cuda, q, kv, 8, 1, 64, sizes=(20,), bases=(base,), window=window, mask=mask, words=words, seed=window)
+        c.run(max_len=far)
+        c.check()
