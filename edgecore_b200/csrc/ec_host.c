@@ -2215,7 +2215,7 @@ EC_EXPORT int ec_forward_tree(GPT2 *g, const ec_tree_step *t, int *picked, float
     a->window = d->window; a->max_len = longest; a->mask_words = words;
     a->slots = (const int *)(d->d_ops + o_slot); a->row_start = (const int *)(d->d_ops + o_start);
     a->base = (const int *)(d->d_ops + o_base); a->mask = (const unsigned long long *)(d->d_ops + o_mask);
-    a->work = d->tree_work; a->work_bytes = d->tree_work_bytes;
+    a->work = d->tree_work; a->work_bytes = work;   /* what a longer step left is not used: a result depends on its call alone */
     if (ec_enqueue_body(d, M, longest, &tree)) return -1;
     if (t->u ? ec_enqueue_lm_sample(d, M, chunk, sp) : ec_enqueue_lm_argmax(d, M, chunk)) return -1;
     ec_tree_path path;

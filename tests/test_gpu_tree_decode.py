@@ -308,3 +308,25 @@ def test_rows_that_grow_between_calls(tiny_models, cuda, first, then):
             out = m.forward_tree([flat], [min(25, then)], [0])
             assert out["accepted"] == [walk(flat[0], flat[1], out["picked"])]
         assert len(m.forward_tree([root], [min(25, then)], [0])["accepted"][0]) == 1
+
+
+def test_a_step_does_not_depend_on_earlier_ones(cuda, tmp_path):
+    """The same trees on the same caches before and after a step at a longer context: the same choices and probabilities, bit
+    for bit, whatever workspace the longer step left behind."""
+    spec = synth.TINY_QWEN2.with_(n_embd=512, n_head=4, n_kv_head=2, n_ctx=2048)
+    path = synth.ensure_model(spec, tmp_path)
+    rs = np.random.RandomState(9)
+    B = 17
+    with ec.Model(path, batch_cap=B) as m:
+        base = [600 + int(rs.randint(0, 250)) for _ in range(B - 1)]
+        for s in range(B - 1):
+            feed(m, synth.prompt_ids(spec.vocab, base[s], seed=s), 0, s)
+        feed(m, synth.prompt_ids(spec.vocab, 1500, seed=99), 0, B - 1)
+        trees = [draft(rs, 3 + s, [], 4, 24, spec.vocab) for s in range(B - 1)]
+        u, temp = rs.rand(24 * (B - 1)).astype(np.float32), np.full(24 * (B - 1), 0.7, np.float32)
+        step = lambda: m.forward_tree(trees, base, u=u, temperature=temp)  # noqa: E731
+        first = step()
+        m.forward_tree([(np.array([5]), np.array([-1]))], [1500], [B - 1])
+        again = step()
+        assert np.array_equal(first["picked"], again["picked"]) and first["accepted"] == again["accepted"]
+        assert np.array_equal(first["prob"].view(np.int32), again["prob"].view(np.int32))
