@@ -327,7 +327,8 @@ def tree_mask(parents) -> np.ndarray:
 
 
 def tree_attention_work(n_seq: int, rows: int, n_head: int, n_kv_head: int, head_dim: int, max_len: int) -> int:
-    """Bytes of workspace with which tree_attention splits long caches as far as it pays."""
+    """Bytes of workspace with which tree_attention splits long caches as far as it pays, for any type of q and window;
+    max_len as in the call (0: any length)."""
     return int(load_library().ec_tree_attention_work(n_seq, rows, n_head, n_kv_head, head_dim, max_len))
 
 

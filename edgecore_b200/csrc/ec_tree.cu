@@ -723,6 +723,8 @@ struct TaPlan {
     TaGeo g;
 };
 
+constexpr int TA_MOST = 0x7fffffff - PAGE;   // positions that a plan counts with, at most
+
 int ta_up(int a, int b) { return (a + b - 1) / b; }
 
 size_t ta_piece_bytes(const TaPlan &p) { return (size_t)2 * p.mt * (p.hdp + 2) * 4; }
@@ -828,14 +830,21 @@ int ta_dims(const ec_kv_pages &kv, const ec_tree_attn &a, const TaPlan &p, int i
 
 }  // namespace
 
+// The larger of what 16-bit and fp32 queries take; a window only ever takes less.
 extern "C" size_t ec_tree_attention_bytes(int n_seq, int rows, int n_head, int n_kv_head, int head_dim, int max_len, int num_sms) {
-    const TaPlan p = ta_plan(n_seq, rows, n_head, n_kv_head, head_dim, max_len, 1, 0, false, head_dim == 64 || head_dim == 128, num_sms);
-    return p.pieces * ta_piece_bytes(p);
+    size_t bytes = 0;
+    for (int f32 = 0; f32 < 2; ++f32) {
+        const TaPlan p = ta_plan(n_seq, rows, n_head, n_kv_head, head_dim, max_len > 0 && max_len < TA_MOST ? max_len : TA_MOST, 1, 0, f32,
+                                 !f32 && (head_dim == 64 || head_dim == 128), num_sms);
+        const size_t need = p.pieces * ta_piece_bytes(p);
+        if (need > bytes) bytes = need;
+    }
+    return bytes;
 }
 
 extern "C" int ec_launch_tree_attention(const ec_kv_pages *kv, const ec_tree_attn *a, int num_sms, int *err, cudaStream_t stream) {
     long long len = a->max_len > 0 ? a->max_len : (long long)kv->pages_per_slot * PAGE;
-    TaPlan p = ta_plan(a->n_seq, a->rows, a->n_head, a->n_kv_head, a->head_dim, (int)(len < 0x7fffffff - PAGE ? len : 0x7fffffff - PAGE), kv->pages_per_slot, a->window, a->type == EC_T_F32,
+    TaPlan p = ta_plan(a->n_seq, a->rows, a->n_head, a->n_kv_head, a->head_dim, (int)(len < TA_MOST ? len : TA_MOST), kv->pages_per_slot, a->window, a->type == EC_T_F32,
                        ta_tc_takes(a->type, kv->type, a->head_dim), num_sms);
     if (p.pieces) {
         const size_t fit = a->work ? a->work_bytes / ta_piece_bytes(p) : 0;

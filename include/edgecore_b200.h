@@ -320,7 +320,8 @@ typedef struct {
 } ec_tree_attn;
 int ec_tree_attention(const ec_kv_pages *kv, const ec_tree_attn *a, void *stream);
 
-/* Bytes of `work` with which ec_tree_attention splits as far as it pays. */
+/* Bytes of `work` with which ec_tree_attention splits as far as it pays, for
+ * either type of q and any window; max_len as in the call (0: any length). */
 size_t ec_tree_attention_work(int n_seq, int rows, int n_head, int n_kv_head, int head_dim, int max_len);
 
 /* Accept the part of a drafted tree that the model confirms, and commit its

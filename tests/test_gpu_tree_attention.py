@@ -402,3 +402,28 @@ def test_window_as_long_as_a_mask_has_bits(cuda, window, far, q, kv):
         c = Case(cuda, q, kv, 8, 1, 64, sizes=(20,), bases=(base,), window=window, mask=mask, words=words, seed=window)
         c.run(max_len=far)
         c.check()
+
+
+@pytest.mark.parametrize("q,kv,heads,kv_heads,hd,seqs,nodes,lens", [
+    ("f32", "f16", 12, 2, 128, 32, 24, (450, 900)), ("f32", "bf16", 4, 2, 256, 32, 24, (560, 900)), ("f32", "f16", 14, 2, 64, 12, 9, (65, 1900)),
+    ("f16", "f16", 14, 2, 64, 3, 5, (1100, 1500)), ("bf16", "bf16", 12, 2, 128, 5, 40, (100, 1300)), ("f16", "f16", 8, 8, 80, 4, 3, (1030, 1200))])
+@pytest.mark.parametrize("said", [True, False])
+def test_the_documented_workspace_is_all_that_a_call_uses(cuda, q, kv, heads, kv_heads, hd, seqs, nodes, lens, said):
+    """With the bytes of tree_attention_work a call splits as far as with any more: the same result, bit for bit.  `said`:
+    with max_len given, or left out of both calls."""
+    rs = np.random.RandomState(seqs)
+    c = Case(cuda, q, kv, heads, kv_heads, hd, sizes=[nodes] * seqs, bases=rs.randint(lens[0], lens[1] - nodes, seqs).tolist(), seed=hd)
+    c.table = np.concatenate([c.table, np.full((seqs, max(0, 20 - c.table.shape[1])), -1, np.int32)], axis=1)   # behind the sequences: no page
+    most = lens[1] if said else 0
+    bytes_ = ec.tree_attention_work(seqs, seqs * nodes, heads, kv_heads, hd, most)
+    assert bytes_ > 0
+    outs = []
+    for n in (bytes_, bytes_ + (64 << 20)):
+        out = cuda.full_like(c.q, 7.0)
+        ec.tree_attention(out, c.q, c.k, c.v, c.dev(c.table), c.dev(c.start), c.dev(np.array(c.bases, np.int32)), c.dev(c.mask.view(np.int64)),
+                          slots=c.dev(c.slots), max_len=most, workspace=cuda.empty(n, dtype=cuda.uint8, device="cuda"))
+        cuda.cuda.synchronize()
+        assert ec.device_error_take() == 0
+        outs.append(out)
+    c.check(outs[0])
+    assert cuda.equal(outs[0], outs[1])
