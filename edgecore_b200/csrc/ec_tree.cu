@@ -769,6 +769,32 @@ TaPlan ta_plan(int n_seq, int rows, int n_head, int n_kv_head, int hd, int max_l
     return p;
 }
 
+// A workspace of only `fit` pieces.  A CTA walks its piece alone, so fewer
+// pieces than clusters would keep CTAs busy take longer than those: one tree of
+// 9 nodes at 30011 positions, 12 heads of 128 on 2, 103 us in clusters (16
+// CTAs), 753 in 2 pieces, 106 in 16; 32 fp32 sequences at 65 to 1900 positions
+// 41 us in clusters, 61 in 74 pieces, 41 in 147.  A tcgen05 piece does the work
+// of two CTAs of a cluster or more: 16 trees of 48 to 64 nodes at 6000 to 10000
+// positions 234 us in clusters, 3607 in 2 pieces, 266 in 32, 146 in 74 (heads of
+// 64: 159 in clusters, 148 in 74); one such tree 41 in clusters of 112 CTAs, 44
+// in 48 pieces, 41 in 64.
+void ta_fit(TaPlan &p, size_t fit, long long rows, int n_seq, int n_kv_head, int sms) {
+    const bool tc = p.mt == TC_ROWS;
+    TaPlan c = p;
+    if (tc) {   // clusters: the register tiles only
+        c.mt = 64;
+        c.tiles = (int)(rows * c.g.group / c.mt + n_seq);
+    }
+    long long busy = (long long)c.tiles * n_kv_head * c.g.cluster;
+    if (busy > sms) busy = sms;
+    if (fit > 1 && (long long)fit * (tc ? 2 : 1) >= busy) {
+        p.pieces = (int)fit;
+        return;
+    }
+    p = c;
+    p.pieces = 0;
+}
+
 int g_attr[64][64];
 
 template <int QT, int HDP>
@@ -848,11 +874,7 @@ extern "C" int ec_launch_tree_attention(const ec_kv_pages *kv, const ec_tree_att
                        ta_tc_takes(a->type, kv->type, a->head_dim), num_sms);
     if (p.pieces) {
         const size_t fit = a->work ? a->work_bytes / ta_piece_bytes(p) : 0;
-        if (fit < (size_t)p.pieces) p.pieces = fit > 1 ? (int)fit : 0;
-        if (!p.pieces && p.mt == TC_ROWS) {
-            p.mt = 64;
-            p.tiles = (int)(((long long)a->rows * p.g.group) / p.mt + a->n_seq);
-        }
+        if (fit < (size_t)p.pieces) ta_fit(p, fit, (long long)a->rows, a->n_seq, a->n_kv_head, num_sms);
     }
     p.g.scale2 = (a->scale > 0.0f ? a->scale : 1.0f / sqrtf((float)a->head_dim)) * LOG2E;
     p.g.part = static_cast<float *>(a->work);

@@ -300,8 +300,8 @@ int ec_model_kv(GPT2 *g, ec_kv_pages *kv);
  * rounded to the cache's type for the product with V.
  * work (NULL, or 256-byte aligned): partial sums of sequences whose positions
  * are split over CTAs; without it, or when it is smaller than
- * ec_tree_attention_work, there is less splitting and the same result up to
- * rounding.  Calls that can overlap must not share it.  max_len: about the
+ * ec_tree_attention_work, there is less splitting (one too small for a useful
+ * part of it is not used) and the same result up to rounding.  Calls that can overlap must not share it.  max_len: about the
  * most positions of a sequence (0: the page table's width); it only steers
  * the splitting. */
 typedef struct {

@@ -427,3 +427,24 @@ def test_the_documented_workspace_is_all_that_a_call_uses(cuda, q, kv, heads, kv
         outs.append(out)
     c.check(outs[0])
     assert cuda.equal(outs[0], outs[1])
+
+
+@pytest.mark.parametrize("q,kv,hd,bytes_", [("bf16", "bf16", 128, 600 << 10), ("f16", "f16", 64, 400 << 10), ("f32", "f16", 128, 200 << 10), ("f16", "f16", 128, 2 << 20)])
+def test_a_workspace_of_a_few_pieces_is_not_taken(cuda, q, kv, hd, bytes_):
+    """Two or three CTAs that walk all pages would take far longer than the clusters of a call without a workspace: it runs as
+    that one, bit for bit."""
+    c = Case(cuda, q, kv, 12, 2, hd, sizes=[40, 55, 48, 60] * 2, bases=[900, 1200, 1100, 1050] * 2, seed=19)
+    plain = c.run(0).clone()
+    c.out.fill_(7.0)
+    c.run(bytes_)
+    c.check()
+    assert cuda.equal(c.out, plain)
+
+
+def test_many_tiles_in_a_piece(cuda):
+    """More tiles than CTAs on the tcgen05 path: a CTA goes from tile to tile, with full halves, lone halves and odd pages."""
+    rs = np.random.RandomState(23)
+    seqs = 120
+    c = Case(cuda, "f16", "f16", 16, 2, 64, sizes=rs.randint(1, 40, seqs).tolist(), bases=rs.randint(0, 300, seqs).tolist(), seed=24)
+    c.run(max_len=FAR)
+    c.check()
