@@ -389,7 +389,8 @@ def tree_commit(k, v, page_table, row_start, base, mask, tokens, picked, accepte
 
 def kv_copy(k, v, page_table, src, dst, start, end, *, stream=None) -> None:
     """Copy positions [start[j], end[j]) of slot src[j] to slot dst[j] in every layer (ec_kv_copy); k, v
-    [layers][pages][64][dim], the others int32 vectors of one length."""
+    [layers][pages][64][dim], the others int32 vectors of one length.  Jobs of which one writes what the other writes or reads
+    are both skipped and reported (device_error_take), as is one with a bad slot or range."""
     kv = _layers(k, v, page_table)
     n = src.shape[0]
     if load_library().ec_kv_copy(kv, n, _vec(src, "src", 3), _vec(dst, "dst", 3, n), _vec(start, "start", 3, n),

@@ -163,17 +163,24 @@ __global__ void __launch_bounds__(PG_THREADS) k_kv_copy(const ec_kv_pages kv, in
     __shared__ long long s_warp[PG_THREADS / 32], s_sum[PG_THREADS], s_to[PG_THREADS];
     __shared__ int s_members;
     const int tid = threadIdx.x;
+    // a job refused for itself: it writes and reads nothing, so it meets no other
+    const auto refused = [&](int4 j) {
+        return j.x < 0 || j.x >= kv.n_slots || j.y < 0 || j.y >= kv.n_slots || j.z < 0 ||
+               (long long)j.w > (long long)kv.pages_per_slot * EC_KV_PAGE || (j.x == j.y && j.z < j.w);
+    };
+    const auto load = [&](int j) {   // a refused job as an empty range that is nobody's
+        const int4 v = make_int4(src[j], dst[j], start[j], end[j]);
+        return refused(v) ? make_int4(-1, -1, 0, 0) : v;
+    };
     // up to PG_THREADS jobs s_job keeps all of them
-    const auto job = [&](int j) { return n <= PG_THREADS ? s_job[j] : make_int4(src[j], dst[j], start[j], end[j]); };
+    const auto job = [&](int j) { return n <= PG_THREADS ? s_job[j] : load(j); };
     for (int j0 = 0; j0 < n; j0 += PG_THREADS) {
         const int j = j0 + tid;
-        int4 me = make_int4(0, 0, 0, 0);
-        if (j < n) me = make_int4(src[j], dst[j], start[j], end[j]);
-        bool bad = me.x < 0 || me.x >= kv.n_slots || me.y < 0 || me.y >= kv.n_slots || me.z < 0 ||
-                   (long long)me.w > (long long)kv.pages_per_slot * EC_KV_PAGE || (me.x == me.y && me.z < me.w), later = false;
+        const int4 me = j < n ? load(j) : make_int4(0, 0, 0, 0);
+        bool bad = me.x < 0, later = bad;
         for (int i0 = 0; i0 < n; i0 += PG_THREADS) {
             __syncthreads();
-            if (i0 + tid < n) s_job[tid] = i0 == j0 ? me : make_int4(src[i0 + tid], dst[i0 + tid], start[i0 + tid], end[i0 + tid]);
+            if (i0 + tid < n) s_job[tid] = i0 == j0 ? me : load(i0 + tid);
             __syncthreads();
             const int m = min(PG_THREADS, n - i0);
             for (int i = 0; i < m; ++i) {
@@ -199,7 +206,7 @@ __global__ void __launch_bounds__(PG_THREADS) k_kv_copy(const ec_kv_pages kv, in
         if (j < n && !(s_flag[j] & 2)) {
             const int4 me = job(j);
             const int p0 = me.z, p1 = me.w;
-            if (p0 >= 0 && p0 < p1 && (long long)p1 <= (long long)kv.pages_per_slot * EC_KV_PAGE)
+            if (p0 < p1)
                 units = (long long)((p1 - 1) / rows - p0 / rows + 1) * 2 * kv.n_layers;
         }
         for (int step = 1; step < 32; step *= 2) {

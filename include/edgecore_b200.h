@@ -347,10 +347,12 @@ typedef struct {
 int ec_tree_commit(const ec_kv_pages *kv, const ec_tree_path *a, void *stream);
 
 /* Copy the K and V of positions [start[j], end[j]) in every layer from slot
- * src[j] to slot dst[j], for n_copies jobs (DEVICE int arrays; at most 4096).  A job whose
- * target is written or read by another job at a common position, or is its
- * own source, is skipped and reported (code 2), and so is one with a bad
- * slot or range; an empty range copies nothing. */
+ * src[j] to slot dst[j], for n_copies jobs (DEVICE int arrays; at most 4096).
+ * A job with a bad slot or range, or whose target is its own source, is
+ * skipped and reported (code 2).  Two others meet when the target of one is
+ * the target or the source of the other at a common position: both are
+ * skipped and reported, so a chain in one call copies none of its links.  An
+ * empty range copies nothing. */
 int ec_kv_copy(const ec_kv_pages *kv, int n_copies, const int *src, const int *dst, const int *start,
                const int *end, void *stream);
 

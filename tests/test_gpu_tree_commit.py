@@ -231,3 +231,35 @@ def test_copies_of_many_jobs(cuda):
         assert ec.device_error_take() == (2 if extra else 0)
     for x, y in zip(a.host(), want):
         assert (x == y).all()
+
+
+@pytest.mark.parametrize("many", [0, 300])
+def test_copy_refused_jobs_do_not_stop_others(cuda, many):
+    """A job that is refused for itself (a bad slot or range, its own source) writes and reads nothing, so it meets nobody."""
+    a = Arena(cuda, 2, 24, 10 + many, 2, seed=13)
+    good = [(0, 1, 0, 100), (0, 2, 0, 100), (3, 4, 7, 120)] + [(0, 10 + i, 0, 100) for i in range(many)]
+    bad = [(0, 0, 0, 100), (-1, 1, 0, 100), (3, 10 + many, 7, 120), (10 + many, 4, 0, 128), (3, 4, -5, 100), (1, 0, 0, 129), (4, 4, 7, 120)]
+    jobs = bad + good
+    want = a.host()
+    for s, d, lo, hi in good:
+        for p in range(lo, hi):
+            for x in want:
+                x[:, a.at(d, p)] = x[:, a.at(s, p)]
+    ec.kv_copy(a.k, a.v, a.dev(a.table), *(a.dev(c) for c in zip(*jobs)))
+    assert ec.device_error_take() == 2
+    for x, y in zip(a.host(), want):
+        assert (x == y).all()
+
+
+def test_copy_skips_both_of_two_jobs_that_meet(cuda):
+    """A chain 0 -> 1 -> 2 over common positions: neither is done, whichever comes first; a third job goes on."""
+    for jobs in ([(0, 1, 0, 90), (1, 2, 60, 120)], [(1, 2, 60, 120), (0, 1, 0, 90)]):
+        a = Arena(cuda, 2, 64, 6, 4, seed=14)
+        want = a.host()
+        for p in range(64):
+            for x in want:
+                x[:, a.at(5, p)] = x[:, a.at(0, p)]
+        ec.kv_copy(a.k, a.v, a.dev(a.table), *(a.dev(c) for c in zip(*(jobs + [(0, 5, 0, 64)]))))
+        assert ec.device_error_take() == 2
+        for x, y in zip(a.host(), want):
+            assert (x == y).all()
