@@ -45,15 +45,26 @@ static int current_device(const char *fn, int *dev, int *sms)
     return 0;
 }
 
-typedef struct { const void *p; const char *name; int optional; } operand;
+typedef struct { const void *p; const char *name; int optional, align; } operand;
+
+/* Every operand must be there and aligned to its elements: a kernel could only
+ * answer a misaligned one with a fault. */
+static int aligned(const char *fn, const operand *o, int n)
+{
+    for (int i = 0; i < n; i++) {
+        if (!o[i].p && !o[i].optional) return refuse("%s: %s must not be NULL", fn, o[i].name);
+        if ((uintptr_t)o[i].p & (uintptr_t)(o[i].align - 1))
+            return refuse("%s: %s must be aligned to %d bytes", fn, o[i].name, o[i].align);
+    }
+    return 0;
+}
 
 /* Every operand must be memory of device `dev`. */
 static int on_device(const char *fn, int dev, const operand *o, int n)
 {
     for (int i = 0; i < n; i++) {
-        if (!o[i].p && o[i].optional) continue;
         struct cudaPointerAttributes at;
-        if (!o[i].p) return refuse("%s: %s must not be NULL", fn, o[i].name);
+        if (!o[i].p) continue;
         if (cudaPointerGetAttributes(&at, o[i].p) != cudaSuccess) {
             cudaGetLastError();
             at.type = cudaMemoryTypeUnregistered;
@@ -113,17 +124,14 @@ EC_EXPORT int ec_tree_attention(const ec_kv_pages *kv, const ec_tree_attn *a, vo
     if (a->window < 0 || a->max_len < 0) return refuse("%s: window %d, max_len %d", fn, a->window, a->max_len);
     if (!(a->scale >= 0.0f) || a->scale > 3.0e38f) return refuse("%s: scale %g", fn, (double)a->scale);
     if ((long long)a->rows * (a->n_head / a->n_kv_head) > 0x3fffffffLL || a->n_seq > 0x3fffffff) return refuse("%s: %d rows", fn, a->rows);
-    if (a->work && ((uintptr_t)a->work & 255)) return refuse("%s: work must be 256-byte aligned", fn);
     if (a->n_seq == 0 || a->rows == 0) return 0;
-    int dev, sms;
-    if (current_device(fn, &dev, &sms)) return -1;
-    const operand o[] = {{a->q, "q", 0}, {a->out, "out", 0}, {kv->k, "k", 0}, {kv->v, "v", 0},
-                         {kv->page_table, "page_table", 0}, {a->slots, "slots", 1}, {a->row_start, "row_start", 0},
-                         {a->base, "base", 0}, {a->mask, "mask", 0}, {a->work, "work", 1}};
-    if (on_device(fn, dev, o, (int)(sizeof o / sizeof o[0]))) return -1;
     const int elt = a->type == EC_T_F32 ? 4 : 2;
-    if (((uintptr_t)a->q | (uintptr_t)a->out) & (uintptr_t)(elt - 1)) return refuse("%s: q and out must be aligned to their element", fn);
-    if ((uintptr_t)a->mask & 7) return refuse("%s: mask must be 8-byte aligned", fn);
+    const operand o[] = {{a->q, "q", 0, elt}, {a->out, "out", 0, elt}, {kv->k, "k", 0, 16}, {kv->v, "v", 0, 16},
+                         {kv->page_table, "page_table", 0, 4}, {a->slots, "slots", 1, 4}, {a->row_start, "row_start", 0, 4},
+                         {a->base, "base", 0, 4}, {a->mask, "mask", 0, 8}, {a->work, "work", 1, 256}};
+    int dev, sms;
+    if (aligned(fn, o, (int)(sizeof o / sizeof o[0]))) return -1;
+    if (current_device(fn, &dev, &sms) || on_device(fn, dev, o, (int)(sizeof o / sizeof o[0]))) return -1;
     int *err = ec_error_word();
     if (!err) return refuse("%s: no device error word", fn);
     return launched(fn, ec_launch_tree_attention(kv, a, sms, err, (cudaStream_t)stream));
@@ -145,14 +153,14 @@ EC_EXPORT int ec_tree_commit(const ec_kv_pages *kv, const ec_tree_path *a, void 
     if (a->n_seq < 0 || a->n_seq > 0x0fffffff || a->rows < 0) return refuse("%s: n_seq %d, rows %d", fn, a->n_seq, a->rows);
     if (a->mask_words < 1 || a->max_path < 1) return refuse("%s: mask_words %d, max_path %d", fn, a->mask_words, a->max_path);
     if (a->n_seq == 0) return 0;
-    int dev, sms;
-    if (current_device(fn, &dev, &sms)) return -1;
     const int none = a->rows == 0;
-    const operand o[] = {{kv->k, "k", 0}, {kv->v, "v", 0}, {kv->page_table, "page_table", 0}, {a->slots, "slots", 1},
-                         {a->row_start, "row_start", 0}, {a->base, "base", 0}, {a->mask, "mask", none},
-                         {a->tokens, "tokens", none}, {a->picked, "picked", none}, {a->accepted, "accepted", 0},
-                         {a->n_accepted, "n_accepted", 0}, {a->new_base, "new_base", 0}};
-    if (on_device(fn, dev, o, (int)(sizeof o / sizeof o[0]))) return -1;
+    const operand o[] = {{kv->k, "k", 0, 16}, {kv->v, "v", 0, 16}, {kv->page_table, "page_table", 0, 4},
+                         {a->slots, "slots", 1, 4}, {a->row_start, "row_start", 0, 4}, {a->base, "base", 0, 4},
+                         {a->mask, "mask", none, 8}, {a->tokens, "tokens", none, 4}, {a->picked, "picked", none, 4},
+                         {a->accepted, "accepted", 0, 4}, {a->n_accepted, "n_accepted", 0, 4}, {a->new_base, "new_base", 0, 4}};
+    int dev, sms;
+    if (aligned(fn, o, (int)(sizeof o / sizeof o[0]))) return -1;
+    if (current_device(fn, &dev, &sms) || on_device(fn, dev, o, (int)(sizeof o / sizeof o[0]))) return -1;
     int *err = ec_error_word();
     if (!err) return refuse("%s: no device error word", fn);
     return launched(fn, ec_launch_tree_commit(kv, a, err, (cudaStream_t)stream));
@@ -165,11 +173,11 @@ EC_EXPORT int ec_kv_copy(const ec_kv_pages *kv, int n_copies, const int *src, co
     if (check_pages(fn, kv)) return -1;
     if (n_copies < 0 || n_copies > EC_KV_COPY_MAX) return refuse("%s: %d copies (at most %d)", fn, n_copies, EC_KV_COPY_MAX);
     if (n_copies == 0) return 0;
+    const operand o[] = {{kv->k, "k", 0, 16}, {kv->v, "v", 0, 16}, {kv->page_table, "page_table", 0, 4},
+                         {src, "src", 0, 4}, {dst, "dst", 0, 4}, {start, "start", 0, 4}, {end, "end", 0, 4}};
     int dev, sms;
-    if (current_device(fn, &dev, &sms)) return -1;
-    const operand o[] = {{kv->k, "k", 0}, {kv->v, "v", 0}, {kv->page_table, "page_table", 0},
-                         {src, "src", 0}, {dst, "dst", 0}, {start, "start", 0}, {end, "end", 0}};
-    if (on_device(fn, dev, o, (int)(sizeof o / sizeof o[0]))) return -1;
+    if (aligned(fn, o, (int)(sizeof o / sizeof o[0]))) return -1;
+    if (current_device(fn, &dev, &sms) || on_device(fn, dev, o, (int)(sizeof o / sizeof o[0]))) return -1;
     int *err = ec_error_word();
     if (!err) return refuse("%s: no device error word", fn);
     return launched(fn, ec_launch_kv_copy(kv, n_copies, src, dst, start, end, sms, err, (cudaStream_t)stream));
@@ -186,12 +194,12 @@ EC_EXPORT int ec_sample(int *ids, float *prob, const void *logits, int type, lon
     if (rows > 0x07ffffff) return refuse("%s: rows %d", fn, rows);
     if (rows > 1 && ld < vocab) return refuse("%s: row stride %lld below vocab %d", fn, ld, vocab);
     if (rows == 0) return 0;
+    const operand o[] = {{ids, "ids", 0, 4}, {prob, "prob", 1, 4}, {logits, "logits", 0, type == EC_T_F32 ? 4 : 2},
+                         {temperature, "temperature", 1, 4}, {top_k, "top_k", 1, 4}, {top_p, "top_p", 1, 4},
+                         {min_p, "min_p", 1, 4}, {u, "u", 0, 4}};
     int dev, sms;
-    if (current_device(fn, &dev, &sms)) return -1;
-    const operand o[] = {{ids, "ids", 0}, {prob, "prob", 1}, {logits, "logits", 0}, {temperature, "temperature", 1},
-                         {top_k, "top_k", 1}, {top_p, "top_p", 1}, {min_p, "min_p", 1}, {u, "u", 0}};
-    if (on_device(fn, dev, o, (int)(sizeof o / sizeof o[0]))) return -1;
-    if ((uintptr_t)logits & (uintptr_t)(type == EC_T_F32 ? 3 : 1)) return refuse("%s: logits must be aligned to their element", fn);
+    if (aligned(fn, o, (int)(sizeof o / sizeof o[0]))) return -1;
+    if (current_device(fn, &dev, &sms) || on_device(fn, dev, o, (int)(sizeof o / sizeof o[0]))) return -1;
     const ec_sample_args a = {ids, prob, logits, ld, type, rows, vocab, temperature, top_k, top_p, min_p, u};
     int *err = ec_error_word();
     if (!err) return refuse("%s: no device error word", fn);

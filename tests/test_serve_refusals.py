@@ -191,3 +191,53 @@ def test_model_entries_refuse_a_model_that_is_not_loaded(built):
     assert lib.ec_forward_tree(None, None, None, None, None, None) == -1 and "not loaded" in ec.last_error()
     assert lib.ec_kv_fork(None, 0, None, 0, 0) == -1 and "not loaded" in ec.last_error()
     assert lib.ec_decode_sample(None, None, None, 1, None, None, None, None, None, None, None) == -1 and "not loaded" in ec.last_error()
+
+
+def test_misaligned_operands_are_refused(built):
+    """A pointer that is not aligned to its element would fault in a kernel: refused by name, before anything asks for a device."""
+    lib = ec.load_library()
+    at = 1 << 20                                  # addresses that are looked at, never read
+    i = torch.zeros(1, 2, dtype=torch.int32)
+    k = torch.zeros(1, 5, 64, 128, dtype=torch.float16)
+    kv = ec._layers(k, k.clone(), i)
+    pages = list(ec._KV_PAGES.unpack(kv))
+    attn = [at, at, 256, 256, 1, 2, 6, 4, 2, 64, 0, 0, 1, 0.0, at, at, at, at, 0, 0]
+    path = [2, 6, 1, 4] + [at] * 9
+
+    def said(call, name):
+        assert call() == -1
+        assert f": {name} must be aligned" in ec.last_error(), (name, ec.last_error())
+
+    bad_kv = pages.copy()
+    bad_kv[5] += 2
+    bad_kv = ec._KV_PAGES.pack(*bad_kv)
+    said(lambda: lib.ec_tree_attention(bad_kv, ec._TREE_ATTN.pack(*attn), None), "page_table")
+    said(lambda: lib.ec_tree_commit(bad_kv, ec._TREE_PATH.pack(*path), None), "page_table")
+    said(lambda: lib.ec_kv_copy(bad_kv, 1, at, at, at, at, None), "page_table")
+    for n, name in ((14, "slots"), (15, "row_start"), (16, "base"), (17, "mask")):
+        for off in ((2, 4) if name == "mask" else (1, 2)):
+            args = attn.copy()
+            args[n] += off
+            said(lambda: lib.ec_tree_attention(kv, ec._TREE_ATTN.pack(*args), None), name)
+    for n, name in ((0, "q"), (1, "out")):
+        for ty, off in ((1, 1), (0, 2)):
+            args = attn.copy()
+            args[n] += off
+            args[4] = ty
+            said(lambda: lib.ec_tree_attention(kv, ec._TREE_ATTN.pack(*args), None), name)
+    for n, name in enumerate(("slots", "row_start", "base", "mask", "tokens", "picked", "accepted", "n_accepted", "new_base")):
+        args = path.copy()
+        args[4 + n] += 4 if name == "mask" else 2
+        said(lambda: lib.ec_tree_commit(kv, ec._TREE_PATH.pack(*args), None), name)
+    for n, name in enumerate(("src", "dst", "start", "end")):
+        args = [at] * 4
+        args[n] += 2
+        said(lambda: lib.ec_kv_copy(kv, 1, *args, None), name)
+    for n, name in enumerate(("ids", "prob", "logits", "temperature", "top_k", "top_p", "min_p", "u")):
+        args = {x: at for x in ("ids", "prob", "logits", "temperature", "top_k", "top_p", "min_p", "u")}
+        args[name] += 2
+        call = lambda ty=0: lib.ec_sample(args["ids"], args["prob"], args["logits"], ty, 9, 3, 9, args["temperature"], args["top_k"], args["top_p"], args["min_p"], args["u"], None)  # noqa: E731
+        said(call, name)
+    args = {x: at for x in args}
+    args["logits"] += 1
+    said(lambda: call(2), "logits")
