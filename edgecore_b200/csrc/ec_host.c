@@ -274,9 +274,11 @@ typedef struct ec_dev {
     float *h_logits;
     size_t h_logits_cap;
     /* batched decode: one captured CUDA graph per step shape (0: full greedy
-     * step, 1: hidden rows only, 2: sampled step); ws_gen counts workspace reallocations and
-     * vocab-shard changes, which invalidate the graphs */
-    struct { cudaGraphExec_t exec; int M, maxlen, chunk, hist, kernels; unsigned gen; } bg[3];
+     * step, 1: hidden rows only, 2: sampled step, 3: sampled step without
+     * top-k and top-p); ws_gen counts workspace reallocations and vocab-shard
+     * changes, which invalidate the graphs */
+    struct { cudaGraphExec_t exec; int M, maxlen, chunk, hist, kernels; unsigned gen; } bg[4];
+    int bg_sampled;            /* 2 or 3: the last one captured */
     unsigned ws_gen;
     int *d_counter;
     /* operands of tree steps, forks and sampled steps: pinned staging and its
@@ -744,7 +746,7 @@ static void ec_dev_free(ec_dev *d)
     cudaFree(d->d_hist); cudaFree(d->taps); cudaFree(d->d_counter);
     cudaFree(d->acc32); cudaFree(d->tile_cnt);
     cudaFreeHost(d->h_ops); cudaFree(d->d_ops); cudaFree(d->tree_work); cudaFree(d->d_samp);
-    for (int k = 0; k < 3; k++)
+    for (int k = 0; k < 4; k++)
         if (d->bg[k].exec) cudaGraphExecDestroy(d->bg[k].exec);
     cudaFreeHost(d->h_logits);
     if (d->prof_ready)
@@ -1801,7 +1803,8 @@ static int ec_enqueue_lm_argmax(ec_dev *d, int M, int chunk)
     return 0;
 }
 
-/* Per-row sampling settings, device arrays (ec_sample). */
+/* Per-row sampling settings, device arrays (ec_sample); top_k and top_p are
+ * NULL where the caller gave neither, which many rows are drawn faster for. */
 typedef struct {
     const float *u, *temperature, *top_p, *min_p;
     const int *top_k;
@@ -1816,17 +1819,18 @@ static int ec_enqueue_lm_sample(ec_dev *d, int M, int chunk, ec_sampling sp)
         const int rows = M - r0 < chunk ? M - r0 : chunk;
         if (ec_enqueue_lm(d, r0, rows)) return -1;
         const ec_sample_args a = {d->d_ids + r0, sp.prob ? sp.prob + r0 : NULL, d->logits, d->V, EC_T_F32, rows, d->V,
-                                  sp.temperature + r0, sp.top_k + r0, sp.top_p + r0, sp.min_p + r0, sp.u + r0};
+                                  sp.temperature + r0, sp.top_k ? sp.top_k + r0 : NULL,
+                                  sp.top_p ? sp.top_p + r0 : NULL, sp.min_p + r0, sp.u + r0};
         CK(ec_launch_sample(&a, d->num_sms, ec_error_word(), d->stream));
     }
     return 0;
 }
 
-static ec_sampling ec_batch_sampling(const ec_dev *d)
+static ec_sampling ec_batch_sampling(const ec_dev *d, int cuts)
 {
     float *f = d->d_samp;
     const size_t B = (size_t)d->B;
-    const ec_sampling sp = {f, f + B, f + 2 * B, f + 3 * B, (const int *)(f + 5 * B), f + 4 * B};
+    const ec_sampling sp = {f, f + B, cuts ? f + 2 * B : NULL, f + 3 * B, cuts ? (const int *)(f + 5 * B) : NULL, f + 4 * B};
     return sp;
 }
 
@@ -1857,7 +1861,7 @@ static int ec_batch_prepare(ec_dev *d, int M, int maxlen, int chunk)
 
 /* The captured graph of kind k (0: body + lm_head argmax + token/position
  * advance; 1: body only, normed rows left in d->h; 2: as 0 with the token
- * sampled by the settings in d_samp), rebuilt when the shape or
+ * sampled by the settings in d_samp; 3: by those without top-k and top-p), rebuilt when the shape or
  * a workspace changed. */
 static int ec_bgraph(ec_dev *d, int kind, int M, int maxlen, int chunk, int hist, cudaGraphExec_t *out)
 {
@@ -1875,7 +1879,7 @@ static int ec_bgraph(ec_dev *d, int kind, int M, int maxlen, int chunk, int hist
     int rc = 0;
     rc = ec_enqueue_body(d, M, maxlen, NULL);
     if (!rc && kind == 0) rc = ec_enqueue_lm_argmax(d, M, chunk);
-    if (!rc && kind == 2) rc = ec_enqueue_lm_sample(d, M, chunk, ec_batch_sampling(d));
+    if (!rc && kind >= 2) rc = ec_enqueue_lm_sample(d, M, chunk, ec_batch_sampling(d, kind == 2));
     if (!rc && kind != 1 &&
         ec_launch_step_advance(d->d_tok, d->d_pos, d->d_ids, M, hist ? d->d_hist : NULL, hist ? d->d_counter : NULL,
                                0, 0, d->stream))
@@ -1911,6 +1915,7 @@ static int ec_bgraph(ec_dev *d, int kind, int M, int maxlen, int chunk, int hist
     d->bg[kind].hist = hist;
     d->bg[kind].gen = d->ws_gen;
     d->bg[kind].kernels = nk;
+    if (kind >= 2) d->bg_sampled = kind;
     *out = d->bg[kind].exec;
     return 0;
 }
@@ -2072,7 +2077,7 @@ EC_EXPORT int ec_decode_sample(GPT2 *g, int *d_tokens, int *d_positions, int n_s
     CK(cudaMemcpyAsync(d->d_pos, d_positions, B * 4, cudaMemcpyDeviceToDevice, st));
     cudaGraphExec_t ex;
     if (!ec_error_word()) { ec_seterr("ec_decode_sample: no device error word"); return -1; }
-    if (ec_bgraph(d, 2, M, maxlen, chunk, 0, &ex)) return -1;
+    if (ec_bgraph(d, d_top_k || d_top_p ? 2 : 3, M, maxlen, chunk, 0, &ex)) return -1;
     for (int s = 0; s < n_steps; s++) {
         CK(cudaMemcpyAsync(f, d_u + (size_t)s * B, B * 4, cudaMemcpyDeviceToDevice, st));
         CK(cudaGraphLaunch(ex, st));
@@ -2197,7 +2202,8 @@ EC_EXPORT int ec_forward_tree(GPT2 *g, const ec_tree_step *t, int *picked, float
             h[3 * m + r] = t->min_p ? t->min_p[r] : 0.0f;
             ((int *)h)[4 * m + r] = t->top_k ? t->top_k[r] : 0;
         }
-        sp.u = f; sp.temperature = f + m; sp.top_p = f + 2 * m; sp.min_p = f + 3 * m; sp.top_k = (const int *)(f + 4 * m);
+        sp.u = f; sp.temperature = f + m; sp.min_p = f + 3 * m;
+        if (t->top_k || t->top_p) { sp.top_p = f + 2 * m; sp.top_k = (const int *)(f + 4 * m); }
         sp.prob = (float *)(d->d_ops + o_prob);
     }
     cudaStream_t st = d->stream;
@@ -2388,6 +2394,7 @@ EC_EXPORT int ec_batch_graph_kernels(GPT2 *g, int kind)
 {
     ec_dev *d = ec_lookup(g);
     if (!d || kind < 0 || kind > 2) { ec_seterr("ec_batch_graph_kernels: no model or bad kind"); return -1; }
+    if (kind == 2 && d->bg_sampled) kind = d->bg_sampled;
     return d->bg[kind].exec ? d->bg[kind].kernels : 0;
 }
 

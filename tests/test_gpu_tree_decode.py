@@ -7,6 +7,10 @@ choice is then within 2 d of the oracle's largest logit.  A weight exp(logit / T
 share of the total, and any sum of shares, by at most exp(2 d / T) - 1."""
 from __future__ import annotations
 
+import subprocess
+import sys
+from pathlib import Path
+
 import numpy as np
 import pytest
 
@@ -330,3 +334,70 @@ def test_a_step_does_not_depend_on_earlier_ones(cuda, tmp_path):
         again = step()
         assert np.array_equal(first["picked"], again["picked"]) and first["accepted"] == again["accepted"]
         assert np.array_equal(first["prob"].view(np.int32), again["prob"].view(np.int32))
+
+
+KERNELS = """
+import sys
+import numpy as np, torch
+from torch.profiler import ProfilerActivity, profile
+import edgecore_b200 as ec
+B = 160
+with ec.Model(sys.argv[1], batch_cap=B) as m:
+    m.forward(np.full(B, 5, np.int32), np.zeros(B, np.int32), np.arange(B, dtype=np.int32))
+    u = torch.rand(1, B, device="cuda")
+    def decode(**kw):
+        tok, pos = torch.full((B,), 7, dtype=torch.int32, device="cuda"), torch.ones(B, dtype=torch.int32, device="cuda")
+        m.decode_sample(tok, pos, 1, u, **kw)
+        torch.cuda.synchronize()
+    def step(**kw):
+        m.forward_tree([(np.array([7]), np.array([-1]))] * B, np.ones(B, np.int32), u=u[0].cpu().numpy(), temperature=0.7, **kw)
+    warm = torch.full((B,), 0.7, device="cuda")
+    for call, name in ((lambda: decode(temperature=warm), "decode"), (lambda: decode(temperature=warm, top_p=warm), "decode-cut"),
+                       (step, "step"), (lambda: step(top_k=50), "step-cut")):
+        call()
+        with profile(activities=[ProfilerActivity.CUDA]) as p:
+            call()
+        print(name, " ".join(sorted({k for e in p.key_averages() for k in ("k_sample_rows", "k_sample<") if k in e.key})) or "-")
+"""
+
+
+def test_many_rows_without_cuts_are_drawn_by_the_row_kernel(cuda, tmp_path):
+    """What a caller leaves out reaches the sampler as left out: a batch with a temperature alone takes k_sample_rows, in the
+    captured step and in tree steps, and one with top-k or top-p does not.  Kernel names come from the profiler, in a process
+    of its own."""
+    spec = synth.TINY_QWEN2.with_(vocab=20011)
+    path = synth.ensure_model(spec, tmp_path)
+    root = str(Path(ec.__file__).resolve().parents[1])
+    r = subprocess.run([sys.executable, "-c", KERNELS, str(path)], capture_output=True, text=True, cwd=root, timeout=300)
+    assert r.returncode == 0, r.stderr
+    said = dict(line.split(" ", 1) for line in r.stdout.splitlines() if line.count(" ") == 1)
+    if set(said.values()) == {"-"}:
+        pytest.skip("the profiler names no kernels here")
+    assert said == {"decode": "k_sample_rows", "decode-cut": "k_sample<", "step": "k_sample_rows", "step-cut": "k_sample<"}
+
+
+def test_settings_left_out_and_settings_that_are_off(tiny_models, cuda):
+    """The same draws, bit for bit, one after the other in one model: a temperature alone, and with top-k and top-p off."""
+    torch = cuda
+    spec = synth.TINY_QWEN2.with_(vocab=16400)
+    B = 150
+    rs = np.random.RandomState(12)
+    u = torch.from_numpy(rs.rand(3, B).astype(np.float32)).cuda()
+    temp = torch.from_numpy(rs.choice([0.0, 0.3, 1.0], B).astype(np.float32)).cuda()
+    off = dict(top_k=torch.zeros(B, dtype=torch.int32, device="cuda"), top_p=torch.ones(B, device="cuda"))
+    with ec.Model(synth.ensure_model(spec, Path(tiny_models["qwen2_int8"][1]).parent), batch_cap=B) as m:
+        feed(m, np.full(60, 5), 0, 0)
+        got = []
+        for kw in (dict(), off, dict(), dict(top_p=off["top_p"]), off):
+            tok = torch.arange(B, dtype=torch.int32, device="cuda")
+            pos = torch.zeros(B, dtype=torch.int32, device="cuda")
+            ids, prob = torch.zeros((3, B), dtype=torch.int32, device="cuda"), torch.zeros((3, B), device="cuda")
+            m.decode_sample(tok, pos, 3, u, temperature=temp, d_out_ids=ids, d_out_prob=prob, **kw)
+            torch.cuda.synchronize()
+            assert ec.device_error_take() == 0 and m.batch_graph_kernels(2) > 0
+            got.append((ids.cpu().numpy(), prob.cpu().numpy().view(np.int32)))
+        for ids, prob in got[1:]:
+            assert np.array_equal(ids, got[0][0]) and np.array_equal(prob, got[0][1])
+        trees = [(np.array([3 + i]), np.array([-1])) for i in range(B)]
+        a, b = (m.forward_tree(trees, np.zeros(B), u=u[0].cpu().numpy(), temperature=temp.cpu().numpy(), **kw) for kw in (dict(), dict(top_k=0, top_p=1.0)))
+        assert np.array_equal(a["picked"], b["picked"]) and np.array_equal(a["prob"].view(np.int32), b["prob"].view(np.int32))
