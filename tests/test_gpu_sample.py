@@ -217,3 +217,14 @@ def test_many_rows(cuda, kind, vocab, pad):
     for kw in (dict(), dict(temperature=temperature), dict(min_p=min_p), dict(temperature=temperature, min_p=min_p)):
         a, b = run(cuda, x, u, **kw), run(cuda, x, u, top_k=np.zeros(rows), **kw)
         assert np.array_equal(a[0], b[0]) and np.array_equal(a[1].view(np.int32), b[1].view(np.int32))
+
+
+@pytest.mark.parametrize("kind,vocab,pad", [("f32", 262144, 0), ("f32", 400001, 3), ("f32", 750000, 1), ("bf16", 400001, 5), ("f16", 750000, 0)])
+def test_vocabularies_up_to_the_largest(cuda, kind, vocab, pad):
+    """A row fills the shared memory of 16 CTAs: one CTA on an SM, clusters of 16."""
+    rows = 3
+    x = _logits(cuda, rows, vocab + pad, kind, vocab % 1000)[:, pad:]
+    rs = np.random.RandomState(vocab % 1000)
+    for kw in (dict(temperature=[0.7] * rows), dict(top_k=[50] * rows, top_p=[0.95] * rows), dict(top_p=[0.9] * rows, min_p=[0.0001] * rows),
+               dict(temperature=[3.0] * rows, top_k=[30000] * rows, top_p=[0.97] * rows), dict(temperature=[0.0, 1.0, 0.5])):
+        check(cuda, x, rs.rand(rows).astype(np.float32), **kw)

@@ -448,3 +448,68 @@ def test_many_tiles_in_a_piece(cuda):
     c = Case(cuda, "f16", "f16", 16, 2, 64, sizes=rs.randint(1, 40, seqs).tolist(), bases=rs.randint(0, 300, seqs).tolist(), seed=24)
     c.run(max_len=FAR)
     c.check()
+
+
+@pytest.mark.parametrize("q,kv,hd", [("f16", "f16", 64), ("bf16", "bf16", 128)])
+@pytest.mark.parametrize("layout", ["rows", "interleaved", "padded", "position outermost"])
+def test_strides_of_queries_outputs_and_caches_on_tcgen05(cuda, q, kv, hd, layout):
+    """Tiles of 128 rows with queries and outputs of any alignment and row stride, and caches whose pages, positions or K and
+    V lie otherwise than in one run."""
+    c = Case(cuda, q, kv, 16, 2, hd, sizes=(30, 3, 17), bases=(90, 200, 0), seed=31)
+    rows, wide = c.q.shape
+    if layout == "rows":
+        for lead, gap, tail in ((1, 13, 3), (4, 12, 4), (2, 14, 6)):      # odd; 8-byte and 4-byte aligned
+            big_q = cuda.full((rows, wide + gap), 3.0, dtype=c.q.dtype, device="cuda")
+            big_o = cuda.full((rows + 5, wide + gap + 8), 5.0, dtype=c.q.dtype, device="cuda")
+            big_q[:, lead:lead + wide] = c.q
+            out = big_o[:rows, tail:tail + wide]
+            c.run(out=out, q=big_q[:, lead:lead + wide], max_len=FAR)
+            c.check(out)
+            c.run(out=out.fill_(7.0), q=big_q[:, lead:lead + wide])
+            c.check(out)
+            out.fill_(5.0)
+            assert (big_o == 5.0).all()
+        return
+    pages = c.k.shape[0]
+    if layout == "interleaved":
+        pool = cuda.stack([c.k, c.v], dim=2)
+        k, v = pool[:, :, 0], pool[:, :, 1]
+    elif layout == "padded":
+        pool = cuda.full((2, pages + 1, 64, 2 * hd + 24), math.nan, dtype=c.k.dtype, device="cuda")
+        pool[0, :pages, :, : 2 * hd], pool[1, :pages, :, : 2 * hd] = c.k.flatten(2), c.v.flatten(2)
+        k, v = (pool[i, :pages, :, : 2 * hd].unflatten(2, (2, hd)) for i in (0, 1))
+    else:
+        pool = cuda.stack([c.k.transpose(0, 1), c.v.transpose(0, 1)]).contiguous()
+        k, v = pool[0].transpose(0, 1), pool[1].transpose(0, 1)
+    assert cuda.equal(k.isnan(), c.k.isnan()) and (k.stride() != c.k.stride())
+    for far in (FAR, None):
+        c.out.fill_(7.0)
+        c.run(k=k, v=v, max_len=far)
+        c.check()
+
+
+@pytest.mark.parametrize("kv", ["f16", "bf16"])
+@pytest.mark.parametrize("heads,kv_heads,hd", [(6, 2, 64), (4, 2, 80), (3, 1, 256)])
+@pytest.mark.parametrize("lead,gap", [(1, 3), (2, 6), (0, 1)])
+def test_fp32_rows_of_any_alignment(cuda, kv, heads, kv_heads, hd, lead, gap):
+    c = Case(cuda, "f32", kv, heads, kv_heads, hd, sizes=(9, 2), bases=(70, 129), seed=33)
+    rows, wide = c.q.shape
+    big = cuda.full((rows, wide + gap), 3.0, device="cuda")
+    out = cuda.full((rows, wide + gap), 5.0, device="cuda")
+    big[:, lead:lead + wide] = c.q
+    for far in (None, FAR):
+        c.run(q=big[:, lead:lead + wide], out=out[:, lead:lead + wide], max_len=far)
+        c.check(out[:, lead:lead + wide])
+    out[:, lead:lead + wide] = 5.0
+    assert (out == 5.0).all()
+
+
+@pytest.mark.parametrize("q,kv,hd", [("f16", "f16", 64), ("bf16", "bf16", 128), ("f32", "f16", 64), ("f32", "bf16", 128), ("f16", "f16", 256)])
+@pytest.mark.parametrize("seqs,window", [(1, 0), (1, 90), (4, 90), (12, 0), (30, 0), (30, 90), (40, 90)])
+def test_short_contexts_with_and_without_a_window(cuda, seqs, window, q, kv, hd):
+    """6 KV heads and up to 5 pages, every number of sequences with both kinds of mask."""
+    rs = np.random.RandomState(seqs)
+    sizes, bases = rs.randint(1, 40, seqs), rs.randint(0, 270, seqs)
+    c = Case(cuda, q, kv, 6, 6, hd, sizes=sizes.tolist(), bases=bases.tolist(), window=window, seed=hd + seqs)
+    c.run(max_len=310)
+    c.check()
