@@ -606,6 +606,7 @@ __global__ void __launch_bounds__(TJ_THREADS) k_tree_join(const ec_kv_pages kv, 
     line.init(kv, a, g, mt, pieces, err);
     TaTile s;
     int begin, i0 = blockIdx.x;
+    if (line.n == 0) return;
     if (SHARED) {
         if (!line.by_index(kv, a, g, mt, blockIdx.x, s, begin, err)) return;
         i0 = line.piece(begin);
@@ -760,7 +761,7 @@ TaPlan ta_plan(int n_seq, int rows, int n_head, int n_kv_head, int hd, int max_l
     while (p.g.cluster > 1 && tiles * p.g.cluster > 2 * sms) p.g.cluster /= 2;
     p.pieces = 0;
     const bool cut = pages > 16 || (pages > 8 && f32 && p.hdp > 64 && tiles * p.g.cluster > sms);
-    if (cut && tiles * slot_pages <= 0x7fffffff)
+    if (cut && tiles * slot_pages < TA_LINE)
         p.pieces = (p.mt == TC_ROWS ? 1 : p.hdp == 64 && !f32 ? 3 : p.hdp <= 128 ? 2 : 1) * sms;
     if (!p.pieces && p.mt == TC_ROWS) {   // clusters: the register tiles only
         p.mt = 64;

@@ -104,10 +104,12 @@ EC_DEV bool ta_find(const ec_kv_pages &kv, const ec_tree_attn &a, const TaGeo &g
     return false;
 }
 
-// The pages of all tiles in one line (below 2^31 of them, ta_plan): sequence
-// by sequence, KV head by KV head, tile by tile; a place on it is a page, or
-// two of them in a tile whose rows are half as many.  CTA i of the first n
-// takes [start(i), start(i + 1)), at least one place each.
+constexpr unsigned TA_LINE = 1u << 26;   // places of a line, fewer (ta_plan)
+
+// The pages of all tiles in one line: sequence by sequence, KV head by KV head,
+// tile by tile; a place on it is a page, or two of them in a tile whose rows are
+// half as many.  CTA i of the first n takes [start(i), start(i + 1)), at least
+// one place each.
 struct TaLine {
     TaSeq head;           // sequence of this lane among the first 32
     int n, total, per, more;   // the first `more` pieces have per + 1 places
@@ -116,9 +118,11 @@ struct TaLine {
     EC_DEV static int work(const TaSeq &q, int kvh) { return head_work(q) * kvh; }
     EC_DEV void init(const ec_kv_pages &kv, const ec_tree_attn &a, const TaGeo &g, int mt, int pieces, int *err) {
         head = ta_seq(kv, a, g, mt, threadIdx.x & 31, err);
-        total = __reduce_add_sync(0xffffffffu, work(head, a.n_kv_head));
+        unsigned all = __reduce_add_sync(0xffffffffu, (unsigned)work(head, a.n_kv_head));   // 32 of less than TA_LINE fit 32 bits
         for (int b0 = 32; b0 < a.n_seq; b0 += 32)
-            total += __reduce_add_sync(0xffffffffu, work(ta_seq(kv, a, g, mt, b0 + (threadIdx.x & 31), err), a.n_kv_head));
+            all = min(all, (unsigned)TA_LINE) + __reduce_add_sync(0xffffffffu, (unsigned)work(ta_seq(kv, a, g, mt, b0 + (threadIdx.x & 31), err), a.n_kv_head));
+        // row_start that falls (ta_seq reports it) and rises again counts rows more than once: a line that no plan allows is empty
+        total = all < TA_LINE ? (int)all : 0;
         n = min(pieces, total);
         per = n ? total / n : 0;
         more = total - per * n;

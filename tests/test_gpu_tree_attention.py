@@ -513,3 +513,21 @@ def test_short_contexts_with_and_without_a_window(cuda, seqs, window, q, kv, hd)
     c = Case(cuda, q, kv, 6, 6, hd, sizes=sizes.tolist(), bases=bases.tolist(), window=window, seed=hd + seqs)
     c.run(max_len=310)
     c.check()
+
+
+@pytest.mark.parametrize("q,heads", [("f16", 1), ("f16", 8), ("f32", 1)])
+def test_row_start_that_falls_and_rises_is_reported(cuda, q, heads):
+    """Thousands of sequences that all claim the same rows: more places than the line of pages can count.  Nothing is written
+    and the call reports a bad index."""
+    rows, n, hd = 100000, 3000, 64
+    start = np.zeros(n + 1, np.int32)
+    start[1::2] = rows
+    k = cuda.zeros(3, 64, 1, hd, dtype=cuda.float16, device="cuda")
+    dev = lambda x: cuda.from_numpy(np.ascontiguousarray(x)).cuda()  # noqa: E731
+    qs = cuda.zeros(rows, heads * hd, dtype=_types(cuda)[q], device="cuda")
+    out = cuda.full_like(qs, 7.0)
+    ec.tree_attention(out, qs, k, k.clone(), dev(np.arange(1600, dtype=np.int32)[None] % 3), dev(start), dev(np.zeros(n, np.int32)), cuda.zeros(rows, 1, dtype=cuda.int64, device="cuda"),
+                      slots=dev(np.zeros(n, np.int32)), workspace=cuda.empty(64 << 20, dtype=cuda.uint8, device="cuda"))
+    cuda.cuda.synchronize()
+    assert ec.device_error_take() == 2 and ec.device_error_take() == 0
+    assert (out == 7.0).all()
