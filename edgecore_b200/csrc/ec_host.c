@@ -287,6 +287,7 @@ typedef struct ec_dev {
     size_t ops_cap;
     void *tree_work;
     size_t tree_work_bytes;
+    int few_gemv;              /* set during tree and sampled steps: 16-bit linears of fewer rows than the tensor cores take by GEMV */
     float *d_samp;             /* sampled decode: u | temperature | top_p | min_p | prob | top_k, each [B] */
     /* taps */
     int taps_on;
@@ -1159,6 +1160,24 @@ static int ec_linear_rc(ec_dev *d, const ec_lin *l, const float *X, int ldx, int
         g.ldx = ldx;
     }
     g.out = out; g.ldo = ldo; g.epi = epi;
+    /* Below the rows of the tensor cores the weight-streaming GEMV (0.5B int8
+     * model, a tree of one node: 2.0 ms, 8.6 ms with the SIMT tiles).  int8 sums are
+     * exact either way; 16-bit ones differ in the last bits, so calls that had
+     * the tiles' keep them. */
+    if (M < EC_TC_MIN_M && (l->wt == EC_W_I8 || d->few_gemv)) {
+        ec_gemv_args v;
+        memset(&v, 0, sizeof v);
+        v.W = l->w; v.wscale = l->s; v.bias = l->b;
+        v.wt = l->wt; v.N = l->N; v.K = l->K; v.Kp = l->Kp; v.ldw = l->ldw; v.M = M;
+        v.out = out; v.ldo = ldo; v.epi = epi;
+        if (l->wt == EC_W_I8) { v.Xq = d->aq; v.xscale = d->as; v.ldx = l->Kp; }
+        else { v.X = X; v.ldx = ldx; }
+        if (ec_gemv_fits(&v)) {
+            const int rv = ec_launch_gemv(&v, d->num_sms, st);
+            ec_prof_end(d, pi);
+            return rv;
+        }
+    }
     g.split = d->split; g.split_bytes = d->split_bytes;
     g.acc32 = d->acc32; g.acc32_elems = d->acc32_elems; g.tile_cnt = d->tile_cnt; g.cnt_elems = EC_TILE_CNT;
     const int rc = ec_launch_gemm(&g, st);
@@ -2077,7 +2096,10 @@ EC_EXPORT int ec_decode_sample(GPT2 *g, int *d_tokens, int *d_positions, int n_s
     CK(cudaMemcpyAsync(d->d_pos, d_positions, B * 4, cudaMemcpyDeviceToDevice, st));
     cudaGraphExec_t ex;
     if (!ec_error_word()) { ec_seterr("ec_decode_sample: no device error word"); return -1; }
-    if (ec_bgraph(d, d_top_k || d_top_p ? 2 : 3, M, maxlen, chunk, 0, &ex)) return -1;
+    d->few_gemv = 1;
+    const int captured = ec_bgraph(d, d_top_k || d_top_p ? 2 : 3, M, maxlen, chunk, 0, &ex);
+    d->few_gemv = 0;
+    if (captured) return -1;
     for (int s = 0; s < n_steps; s++) {
         CK(cudaMemcpyAsync(f, d_u + (size_t)s * B, B * 4, cudaMemcpyDeviceToDevice, st));
         CK(cudaGraphLaunch(ex, st));
@@ -2222,8 +2244,11 @@ EC_EXPORT int ec_forward_tree(GPT2 *g, const ec_tree_step *t, int *picked, float
     a->slots = (const int *)(d->d_ops + o_slot); a->row_start = (const int *)(d->d_ops + o_start);
     a->base = (const int *)(d->d_ops + o_base); a->mask = (const unsigned long long *)(d->d_ops + o_mask);
     a->work = d->tree_work; a->work_bytes = work;   /* what a longer step left is not used: a result depends on its call alone */
-    if (ec_enqueue_body(d, M, longest, &tree)) return -1;
-    if (t->u ? ec_enqueue_lm_sample(d, M, chunk, sp) : ec_enqueue_lm_argmax(d, M, chunk)) return -1;
+    d->few_gemv = 1;
+    const int step = ec_enqueue_body(d, M, longest, &tree) ||
+                     (t->u ? ec_enqueue_lm_sample(d, M, chunk, sp) : ec_enqueue_lm_argmax(d, M, chunk));
+    d->few_gemv = 0;
+    if (step) return -1;
     ec_tree_path path;
     memset(&path, 0, sizeof path);
     path.n_seq = n; path.rows = M; path.mask_words = words; path.max_path = t->max_path;

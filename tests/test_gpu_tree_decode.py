@@ -401,3 +401,38 @@ def test_settings_left_out_and_settings_that_are_off(tiny_models, cuda):
         trees = [(np.array([3 + i]), np.array([-1])) for i in range(B)]
         a, b = (m.forward_tree(trees, np.zeros(B), u=u[0].cpu().numpy(), temperature=temp.cpu().numpy(), **kw) for kw in (dict(), dict(top_k=0, top_p=1.0)))
         assert np.array_equal(a["picked"], b["picked"]) and np.array_equal(a["prob"].view(np.int32), b["prob"].view(np.int32))
+
+
+FEW_ROWS = """
+import sys
+import numpy as np, torch
+from torch.profiler import ProfilerActivity, profile
+import edgecore_b200 as ec
+with ec.Model(sys.argv[1], batch_cap=3) as m:
+    m.forward(np.full(3, 5, np.int32), np.zeros(3, np.int32), np.arange(3, dtype=np.int32))
+    u = torch.rand(1, 3, device="cuda")
+    def decode():
+        tok, pos = torch.full((3,), 7, dtype=torch.int32, device="cuda"), torch.ones(3, dtype=torch.int32, device="cuda")
+        m.decode_sample(tok, pos, 1, u)
+        torch.cuda.synchronize()
+    def step(n, **kw):
+        m.forward_tree([(np.arange(n), np.arange(n) - 1)], [1], [1], **kw)
+    for name, call in (("decode", decode), ("one", lambda: step(1)), ("seven", lambda: step(7)), ("drawn", lambda: step(3, u=np.full(3, 0.5)))):
+        call()
+        with profile(activities=[ProfilerActivity.CUDA]) as p:
+            call()
+        print(name, ",".join(sorted({k for e in p.key_averages() for k in ("k_gemv", "k_gemm_i8", "k_gemm_f", "k_gemm_tc") if k in e.key})) or "-")
+"""
+
+
+@pytest.mark.parametrize("key", ["qwen2_int8", "qwen2_bf16", "gpt2_fp16"])
+def test_steps_of_few_rows_stream_their_weights(tiny_models, cuda, key):
+    """Below 8 rows the linears and the lm_head of a tree step and of a sampled step are GEMVs, not the tiles for operands
+    that the tensor cores do not take."""
+    root = str(Path(ec.__file__).resolve().parents[1])
+    r = subprocess.run([sys.executable, "-c", FEW_ROWS, str(tiny_models[key][1])], capture_output=True, text=True, cwd=root, timeout=300)
+    assert r.returncode == 0, r.stderr
+    said = dict(line.split(" ") for line in r.stdout.splitlines() if line.count(" ") == 1)
+    if set(said.values()) == {"-"}:
+        pytest.skip("the profiler names no kernels here")
+    assert said == {k: "k_gemv" for k in ("decode", "one", "seven", "drawn")}
