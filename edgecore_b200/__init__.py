@@ -247,6 +247,9 @@ def argmax_key_decode(key: int) -> tuple[float, int]:
 
 
 # ---- serving operators on device tensors --------------------------------------
+#
+# `stream` is a cudaStream_t as an int.  None is the legacy default stream, not torch's current one: inside
+# torch.cuda.stream(s), whose work it does not wait for, pass s.cuda_stream.
 
 # ec_kv_pages, ec_tree_attn and ec_tree_path, field by field: packed bytes cost
 # a quarter of a ctypes structure, on calls of a few microseconds
@@ -334,7 +337,8 @@ def tree_attention_work(n_seq: int, rows: int, n_head: int, n_kv_head: int, head
 
 def tree_attention(out, q, k, v, page_table, row_start, base, mask, *, slots=None, window: int = 0, scale: float = 0.0,
                    max_len: int = 0, workspace=None, stream=None):
-    """Attention of drafted-token trees over a paged KV arena (ec_tree_attention) on device tensors, enqueued on `stream`.
+    """Attention of drafted-token trees over a paged KV arena (ec_tree_attention) on device tensors, enqueued on `stream` (an int
+    cudaStream_t; None: the legacy default stream, not torch's current one).
 
     q, out [rows][heads * head_dim] (or [rows][heads][head_dim]) fp32 or of the cache's type, any row stride; k, v
     [pages][64][KV heads][head_dim] fp16 or bf16; page_table int32 [slots][pages per slot]; row_start int32 [sequences + 1],
@@ -370,7 +374,8 @@ def tree_attention(out, q, k, v, page_table, row_start, base, mask, *, slots=Non
 
 def tree_commit(k, v, page_table, row_start, base, mask, tokens, picked, accepted, n_accepted, new_base, *, slots=None,
                 stream=None) -> None:
-    """Accept the confirmed path of every drafted tree and move its K and V rows to the front (ec_tree_commit).
+    """Accept the confirmed path of every drafted tree and move its K and V rows to the front (ec_tree_commit), on `stream` as
+    in tree_attention.
 
     k, v [layers][pages][64][dim]; tokens, picked int32 [rows]; accepted int32 [sequences][most nodes of a path], n_accepted
     and new_base int32 [sequences] (new_base may be base) are written; the others as for tree_attention."""
@@ -388,7 +393,8 @@ def tree_commit(k, v, page_table, row_start, base, mask, tokens, picked, accepte
 
 
 def kv_copy(k, v, page_table, src, dst, start, end, *, stream=None) -> None:
-    """Copy positions [start[j], end[j]) of slot src[j] to slot dst[j] in every layer (ec_kv_copy); k, v
+    """Copy positions [start[j], end[j]) of slot src[j] to slot dst[j] in every layer (ec_kv_copy), on `stream` as in
+    tree_attention; k, v
     [layers][pages][64][dim], the others int32 vectors of one length.  Jobs of which one writes what the other writes or reads
     are both skipped and reported (device_error_take), as is one with a bad slot or range."""
     kv = _layers(k, v, page_table)
@@ -401,7 +407,7 @@ def kv_copy(k, v, page_table, src, dst, start, end, *, stream=None) -> None:
 def sample(ids, logits, u, *, temperature=None, top_k=None, top_p=None, min_p=None, prob=None, stream=None):
     """Draw one token per row of logits [rows][vocab] (fp32, fp16 or bf16, any row stride) with the uniform numbers u[rows]
     (ec_sample): temperature, top-k, top-p and min-p per row, each a vector or None for off.  Writes ids int32 [rows] and, if
-    given, prob fp32 [rows]; returns ids."""
+    given, prob fp32 [rows]; returns ids.  `stream` as in tree_attention."""
     shape, st = logits.shape, logits.stride()
     if len(shape) != 2 or (shape[1] > 1 and st[1] != 1):
         raise ValueError("logits must be [rows][vocab] with contiguous rows")

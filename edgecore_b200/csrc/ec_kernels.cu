@@ -6,8 +6,9 @@
 //                 memory, and a transposed shuffle reduction finishes each row.
 //                 int8 weights: exact int32 dp4a dot + the reference epilogue
 //                 (bias + ((float)dot*as)*ws).
-//   k_gemm_i8, k_gemm_f  SIMT tiled GEMMs for 8 < M < 32 and for operands the
-//                 tcgen05 path (ec_tc.cu) cannot take, same numerics.
+//   k_gemm_i8, k_gemm_f  SIMT tiled GEMMs for operands the tcgen05 path
+//                 (ec_tc.cu) cannot take, and for fewer than 8 rows of 16-bit
+//                 weights in the per-layer path, same numerics.
 //   k_quant       per-row activation quantisation (reference gpt2.c:446-461).
 //   k_embed, k_norm, k_norm_quant, k_qkv_split, k_swiglu, k_swiglu_quant, k_gelu,
 //   k_attn_exact, k_attn_part/combine,

@@ -86,8 +86,7 @@ struct SaShared {
 // 512] e^(f ln 2 / 512), the last as its Taylor sum to the third power
 // (0.00068^4 / 24 = 2^-46.7 of it is left out).  Nothing (2^-1000) for v below
 // `floor`, where it is less than 2^-(shift + 2), for NaN and where `is` is
-// false.  Nine double operations and no branch: the double pipe is what a
-// draw without cuts is bound by.
+// false.  Nine double operations and no branch.
 struct SaWeight {
     double mx, c;              // c: 512 log2(e) / T
     float floor;
@@ -856,13 +855,16 @@ EC_DEV int dr_find(const u64 *part, u64 target, u64 &before) {
 }
 
 // Many rows without top-k and top-p: a CTA per row, which reads it twice, for
-// the largest logit and for the sum, and then a 256th of it to find the point.
-// The second reading comes from L2: 1000 rows of 50257 fp32 logits (201 MB)
-// read 266 MB of DRAM.  They take 111 us, 1.8 TB/s, bound by the instructions
-// of the weights (about 30 for an element) and their dependence; k_sample,
-// whose SMs hold one row at a time and work on it or wait for it, takes 158.
-// Smaller CTAs (4 of 256 threads: 130 us) leave a longer tail and more rows
-// in flight than L2 holds; more than 2 CTAs of 512 have to spill.
+// the largest logit and for the sum, and then a 16th and a 256th of it to find
+// the point.  The later readings come from L2: 1000 rows of 50257 fp32 logits
+// (201 MB) read 201 MB of DRAM.  They take 111 us, 1.8 TB/s, bound by the
+// instructions of the weights (about 30 for an element) and their dependence:
+// the schedulers issue in 57 % of the cycles, the double pipe is busy in 26 %,
+// DRAM in 22 %.  k_sample, whose SMs hold one row at a time and work on it or
+// wait for it, takes 158; 16-bit logits take 100 us.  Smaller CTAs (4 of 256
+// threads: 130 us) leave a longer tail and more rows in flight than L2 holds.
+// Two CTAs of 512 threads leave 64 registers a thread, and 224 bytes spill (288
+// with 16-bit logits); three would leave 40.
 // The sums are the integers of k_sample, so the draws are the same.
 template <int T> __global__ void __launch_bounds__(DR_THREADS, 2) k_sample_rows(const ec_sample_args a, int shift) {
     EC_PDL_ENTER();

@@ -16,10 +16,13 @@
 // Measured: one token of one stream, 7 us; a tree of 9 nodes at 30011 positions,
 // 12 heads of 128 on 2 (31 MB, 1.7 GFLOP), 26 us or 1.2 TB/s, 7 us of it the
 // second launch with its wait for the first; 32 sequences of 1
-// to 17 nodes with fp32 q at 65 to 1900 positions 33 us; 24 windowed ones 20 us
-// or 1.6 TB/s.  All are bound by latency: a page is a chain of load, product,
-// maximum, exponentials and product of about a microsecond in a warp, and
-// little more than one chain of a few pages fits a call of this length.
+// to 17 nodes with fp32 q at 65 to 1900 positions 35 us; 24 windowed ones 20 us
+// or 1.6 TB/s.  All are bound by latency, not by a pipe or by memory: a CTA of
+// the long and of the fp32 call has three to five pages, an SM is busy for 64 %
+// of the first kernel's cycles (its chain of lengths, page table, queries and
+// first pages, gone through again at every change of tile, is the rest), and
+// while it is, its schedulers issue in a third of the cycles, the tensor cores
+// run in a quarter to a third and DRAM gives 8 to 17 % of its rate.
 #include "ec_tree.cuh"
 
 #include <cooperative_groups.h>
@@ -752,10 +755,10 @@ TaPlan ta_plan(int n_seq, int rows, int n_head, int n_kv_head, int hd, int max_l
     // us so and 31 us as equal pieces with a second launch; 64 sequences of one
     // token up to 900 positions, 14 heads of 64 on 2, 16 and 22 us.  Beyond,
     // ragged lengths leave clusters waiting: 32 sequences of 65 to 1900
-    // positions take 33 us as pieces, 34 to 39 us as clusters.  fp32 rows wider
+    // positions take 35 us as pieces, 41 us as clusters.  fp32 rows wider
     // than 64, with two or three products for each of the others', are better
     // cut from 9 pages on unless the clusters leave SMs idle: 32 trees of 24
-    // nodes at 450 to 900 positions 44 us, 57 as clusters.
+    // nodes at 450 to 900 positions 50 us, 57 as clusters.
     const long long tiles = (long long)p.tiles * n_kv_head;
     p.g.cluster = pages >= 8 ? 8 : pages >= 4 ? 4 : pages >= 2 ? 2 : 1;
     while (p.g.cluster > 1 && tiles * p.g.cluster > 2 * sms) p.g.cluster /= 2;

@@ -27,8 +27,10 @@
 // 128 on 2 (43.7 GFLOP), 99 us or 440 TFLOP/s, join included; the register
 // tiles of ec_tree.cu take 192.  A round of two steps takes 2.3 to 2.9 us where its exponentials and
 // products need 1.5: the rows' own instructions (scale, mask, maximum, pack)
-// are the longest link.  The join and its launch are 20 us, the ends of two
-// tiles in a piece 10.
+// are the longest link, with 282 bytes of a row's 128 scores spilled at 168
+// registers (ten warps put three on one scheduler); the tensor cores are busy in
+// 34 % of the cycles.  The join and its launch are 20 us, the ends of two tiles
+// in a piece 10.
 #include "ec_tree.cuh"
 
 #include <cuda.h>
